@@ -9,10 +9,15 @@
  * at the boundary, no panics across FFI: reference docs/error-handling.md:7-57)
  * and the variant set of `OxitorchError` (crates/oxi-core/src/lib.rs:186-211).
  *
- * All device pointers are HBM buffers obtained from `oxi_hip_alloc`. Float data
- * is fp32; ids/targets are int64. Launches are asynchronous on one per-process
- * HIP stream owned by the library; `oxi_hip_sync()` and the d2h copy wait for
- * it. Output buffers never alias inputs unless an entry point says so.
+ * All device pointers are HBM buffers of the bound device: from
+ * `oxi_hip_alloc`, or of another allocator in the same process, which the
+ * caller keeps until the library stream has passed the calls on them. Float
+ * data is fp32 at 4-byte alignment; ids/targets are int64. Launches are
+ * asynchronous on one per-process HIP stream owned by the library;
+ * `oxi_hip_sync()` and the d2h copy wait for it, and a caller that writes or
+ * reads the buffers on another stream orders it with that one
+ * (`oxi_hip_stream`). Output buffers never alias inputs unless an entry point
+ * says so.
  *
  * Strided entry points take, for each operand, strides in ELEMENTS that are
  * already broadcast-expanded to the iteration `shape` (stride 0 = broadcast),
@@ -301,6 +306,61 @@ int oxi_layer_norm_bwd_lead_sum(const float* x, const float* w, const float* b, 
                                 float* db, float* dx_sum, int64_t lead, int64_t rows, int64_t cols, int mode);
 
 /* ------------------------------------------------------------------------ */
+/* RMS norm of a residual sum. No counterpart in the reference, whose graph  */
+/* runs an add and a norm node (crates/oxi-autograd/src/ops.rs:29-37,        */
+/* python/oxitorch/nn/functional.py:236-240).                                */
+
+/* h = x + r and y = (h*inv)*w, inv = 1/sqrt(mean(h*h)+eps), in one pass: the
+ * values of oxi_binary(ADD) and oxi_rms_norm_fwd, whose row sums may round
+ * differently. `h` may be x or r itself (the residual stream updated in
+ * place); `w` may be NULL (all ones). Writes the per-row `rstd` (= inv) unless
+ * NULL. */
+int oxi_add_rms_norm_fwd(const float* x, const float* r, const float* w, float* h, float* y, float* rstd,
+                         int64_t rows, int64_t cols, float eps);
+/* Its VJP for upstream gradients gy of y and gh of h (NULL: none):
+ * dx = gh + the oxi_rms_norm_bwd of gy at h, the gradient of x and of r alike,
+ * and dw. `dx` may be gh itself; dx or dw may be NULL to skip. `workspace`:
+ * device memory of oxi_add_rms_norm_bwd_workspace bytes, 8-byte aligned, that
+ * the call alone uses until the stream has passed it, or NULL to take it from
+ * the caching allocator (a call under graph capture passes its own).
+ * Deterministic. */
+int oxi_add_rms_norm_bwd(const float* h, const float* w, const float* rstd, const float* gy, const float* gh,
+                         float* dx, float* dw, void* workspace, int64_t rows, int64_t cols, int mode);
+int oxi_add_rms_norm_bwd_workspace(int64_t rows, int64_t cols, int64_t* bytes);
+/* The forward with y in 8 bits (OCP e4m3: 1 sign, 4 exponent, 3 mantissa bits,
+ * largest 448, no infinity) for a product that takes it so. The columns of a
+ * row form groups of `group`, the last one possibly shorter; scale (rows,
+ * ceil(cols/group)) holds max|y|/448 of each, at least 2^-126, and q (rows,
+ * cols) the codes of y/scale rounded to nearest even; a NaN of y becomes the
+ * code NaN (0x7f) and is left out of the maximum. `group`: 32, 64, 128, 256 or
+ * cols. `r` NULL: no addition (then `h` may be NULL and is not written). */
+int oxi_add_rms_norm_e4m3_fwd(const float* x, const float* r, const float* w, float* h, uint8_t* q, float* scale,
+                              int64_t rows, int64_t cols, int64_t group, float eps);
+/* y = the values that q and scale stand for: code * scale. */
+int oxi_e4m3_dequantize(const uint8_t* q, const float* scale, float* y, int64_t rows, int64_t cols, int64_t group);
+
+/* ------------------------------------------------------------------------ */
+/* Rotary positions. No counterpart in the reference.                        */
+
+enum { OXI_ROTARY_HALF = 0, OXI_ROTARY_INTERLEAVED = 1 };
+
+/* Turns the pairs of the first `rot` elements (even, at most dim) of every
+ * head of x by the angle position * inv_freq[i], and copies the others:
+ *   (u, v) -> scale * (u cos a - v sin a, v cos a + u sin a),
+ * pair i < rot/2 being elements (i, i + rot/2) (OXI_ROTARY_HALF) or
+ * (2i, 2i + 1) (OXI_ROTARY_INTERLEAVED). Angles are formed and reduced in 64
+ * bits. `shape` is (batch, tokens, heads, dim), with strides in elements for x
+ * and y (0 = broadcast, x only; y's elements must be distinct); y may be x
+ * itself with x's strides. `positions` (device, with (batch, token) strides
+ * `pos_strides`, 0 = shared) holds each token's position, any int64 below
+ * 2^53; NULL: token t is at position offset + t. `offset` is added to both.
+ * `inv_freq` (device) holds rot/2 doubles. `inverse` != 0 turns by -a: the
+ * VJP. One call serves query and key heads that lie in one buffer. */
+int oxi_rotary(const float* x, const int64_t* x_strides, float* y, const int64_t* y_strides, const int64_t* shape,
+               const int64_t* positions, const int64_t* pos_strides, int64_t offset, const double* inv_freq,
+               int64_t rot, int layout, int inverse, float scale);
+
+/* ------------------------------------------------------------------------ */
 /* Softmax family over the middle dim of a contiguous (outer, len, inner)    */
 /* buffer (inner == 1 is the last-dim case).                                 */
 
@@ -339,6 +399,69 @@ int oxi_cross_entropy_bwd(const float* logits, const int64_t* targets, const flo
  * return OXI_NOT_IMPLEMENTED before any launch (take the two calls then). */
 int oxi_cross_entropy_fwd_grad(const float* logits, const int64_t* targets, float* loss, float* lse,
                                float* dlogits, int64_t n, int64_t c);
+
+/* ------------------------------------------------------------------------ */
+/* Distillation from a teacher's top logits. No counterpart in the reference; */
+/* stands next to oxi_cross_entropy_*.                                        */
+
+#define OXI_DISTILL_MAX_TOP 1024
+
+/* The loss that pulls a student's distribution q = softmax(logits/T) towards a
+ * teacher's, known by its k best entries a row: ids (n, k) and top (n, k), the
+ * teacher's logits there. An entry with a negative id or a logit of -inf is
+ * padding; a row of padding alone counts nothing and gets a zero gradient.
+ * Without `top_lse`, p = softmax(top/T) over the row's entries and
+ *   row = sum p (log p - log q[id]).
+ * With it (n floats: log sum exp(teacher logits/T) over all classes),
+ * p = exp(top/T - top_lse), and what they leave, pr = max(1 - sum p, 0), is
+ * compared with the student's mass qr on the classes not listed:
+ *   row = sum p (log p - log q[id]) + pr (log pr - log qr).
+ * row_loss (n) = T^2 row; loss (1 float) = sum of row_loss / divisor, summed
+ * in 64 bits in a fixed order (n for the plain mean, the count of rows that
+ * hold entries for padded batches). An id given twice counts with both entries.
+ * `lse` (n, log sum exp(logits/T)) and `rest` (n, log qr; 0 without top_lse)
+ * are what the backward needs. With `dlogits` (n, c) set, the same pass also
+ * writes the gradient for an upstream gradient of 1: T/divisor times q - p
+ * at the listed classes and q (1 - pr/qr) at the others (q without top_lse).
+ * 1 <= k <= OXI_DISTILL_MAX_TOP. An id >= c raises the device guard flag
+ * (oxi_hip_sync reports it) and is taken as padding. Takes no workspace. */
+int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, const float* top_lse, float* loss,
+                    float* row_loss, float* lse, float* rest, float* dlogits, int64_t n, int64_t c, int64_t k,
+                    float temperature, float divisor);
+/* dlogits for the upstream scalar gradient gloss[0] (device), from the
+ * forward's lse and rest. */
+int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, const float* top_lse,
+                    const float* lse, const float* rest, const float* gloss, float* dlogits, int64_t n, int64_t c,
+                    int64_t k, float temperature, float divisor);
+
+/* ------------------------------------------------------------------------ */
+/* Verification of drafted tokens. No counterpart in the reference.          */
+
+/* Checks the tokens that a small model drafted against the probabilities of
+ * the model it drafts for, so that what is kept is distributed as the latter's
+ * own samples. For each of `batch` sequences: target (batch, drafts + 1,
+ * vocab), the probabilities after 0, 1, .. drafts of its drafted tokens; draft
+ * (batch, drafts, vocab), those that each token was drawn from, or NULL for
+ * drafts without (each token then counts as drawn with probability 1); tokens
+ * (batch, drafts) int64; lengths (batch), how many were drafted (0 to drafts;
+ * NULL: all); uniforms (batch, drafts + 1) in [0, 1). Draft i is kept while
+ * uniforms[i] * draft[i][token] < target[i][token]. After the first that is
+ * not, position j, one more token is drawn from max(target[j] - draft[j], 0),
+ * or, after all of them, from target[j]: the lowest id whose running sum of
+ * weights is more than uniforms[drafts] times their total (sums in 64 bits).
+ * Where max(target - draft, 0) has no weight, target[j] is drawn from; a row
+ * without weight there gives -1. Probabilities need not sum to 1; a NaN or
+ * negative one weighs nothing. Outputs: accepted (batch), the number kept;
+ * out (batch, drafts + 1), the kept tokens, the drawn one, then -1. A drafted
+ * token outside [0, vocab) is not kept and, like a length outside [0, drafts],
+ * raises the device guard flag (oxi_hip_sync reports it). `workspace`: device
+ * memory of oxi_verify_drafts_workspace bytes, 8-byte aligned, that the call
+ * alone uses until the stream has passed it, or NULL to take it from the caching
+ * allocator (a call under graph capture passes its own). */
+int oxi_verify_drafts(const float* target, const float* draft, const int64_t* tokens, const int64_t* lengths,
+                      const float* uniforms, int64_t* accepted, int64_t* out, void* workspace, int64_t batch,
+                      int64_t drafts, int64_t vocab);
+int oxi_verify_drafts_workspace(int64_t batch, int64_t vocab, int64_t* bytes);
 
 /* ------------------------------------------------------------------------ */
 /* Gather / scatter-add.                                                     */

@@ -47,6 +47,8 @@ BINARY = ["add", "sub", "mul", "div", "pow", "min", "max", "eq", "ne", "lt", "le
 REDUCE = ["sum", "mean", "max", "min", "argmax", "argmin", "norm"]
 NORM_VJP = {"ref": 0, "exact": 1}
 GELU = {"tanh": 0, "none": 1, "erf": 1}
+ROTARY = {"half": 0, "interleaved": 1}
+DISTILL_MAX_TOP = 1024  # OXI_DISTILL_MAX_TOP
 ACT = {"none": -1, "gelu_tanh": 0, "gelu_erf": 1, "silu": 2, "softmax": 3, "log_softmax": 4}
 
 _SIGS = {
@@ -90,6 +92,12 @@ _SIGS = {
     "oxi_layer_norm_act_bwd": [vp, vp, vp, vp, vp, vp, c_int, vp, vp, vp, vp, c_i64, c_i64, c_int],
     "oxi_rms_norm_bwd_lead_sum": [vp, vp, vp, vp, c_int, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_int],
     "oxi_layer_norm_bwd_lead_sum": [vp, vp, vp, vp, vp, vp, c_int, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_int],
+    "oxi_add_rms_norm_fwd": [vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_float],
+    "oxi_add_rms_norm_bwd": [vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_int],
+    "oxi_add_rms_norm_bwd_workspace": [c_i64, c_i64, P_i64],
+    "oxi_add_rms_norm_e4m3_fwd": [vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float],
+    "oxi_e4m3_dequantize": [vp, vp, vp, c_i64, c_i64, c_i64],
+    "oxi_rotary": [vp, P_i64, vp, P_i64, P_i64, vp, P_i64, c_i64, vp, c_i64, c_int, c_int, c_float],
     "oxi_softmax_fwd": [vp, vp, c_i64, c_i64, c_i64],
     "oxi_softmax_bwd": [vp, vp, vp, c_i64, c_i64, c_i64],
     "oxi_log_softmax_fwd": [vp, vp, c_i64, c_i64, c_i64],
@@ -97,6 +105,10 @@ _SIGS = {
     "oxi_cross_entropy_fwd": [vp, vp, vp, vp, c_i64, c_i64],
     "oxi_cross_entropy_bwd": [vp, vp, vp, vp, vp, c_i64, c_i64],
     "oxi_cross_entropy_fwd_grad": [vp, vp, vp, vp, vp, c_i64, c_i64],
+    "oxi_distill_fwd": [vp, vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float, c_float],
+    "oxi_distill_bwd": [vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float, c_float],
+    "oxi_verify_drafts": [vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64],
+    "oxi_verify_drafts_workspace": [c_i64, c_i64, P_i64],
     "oxi_index_select": [vp, c_i64, c_i64, c_i64, vp, c_i64, vp],
     "oxi_batch_gather": [vp, c_int, c_i64, vp, c_i64],
     "oxi_index_select_bwd": [vp, c_i64, c_i64, c_i64, vp, c_i64, vp],
@@ -176,7 +188,8 @@ def _i64arr(vals) -> ctypes.Array:
 
 
 class DeviceArray:
-    """An HBM buffer of fp32 or int64 elements with a shape (row-major)."""
+    """An HBM buffer with a shape (row-major) and a numpy dtype: fp32 values,
+    int64 ids, uint8 codes, float64 rotary frequencies."""
 
     __slots__ = ("ptr", "shape", "dtype", "nbytes", "__weakref__")
 
@@ -412,6 +425,70 @@ def layer_norm_act_bwd(x, w, b, mean, rstd, g, act, mode="ref", need_dy=True, ne
     return dy, dx, dw, db
 
 
+def add_rms_norm_fwd(x: DeviceArray, r: DeviceArray, w: DeviceArray | None, eps=1e-6, h: DeviceArray | None = None):
+    """h = x + r and y = rms_norm(h); returns (h, y, rstd). `h` may be x or r
+    (the residual stream updated in place)."""
+    rows, H = _rows(x)
+    h = h if h is not None else DeviceArray(x.shape)
+    y = DeviceArray(x.shape)
+    rstd = DeviceArray((rows,))
+    call("oxi_add_rms_norm_fwd", x.ptr, r.ptr, w.ptr if w else None, h.ptr, y.ptr, rstd.ptr, rows, H, eps)
+    return h, y, rstd
+
+
+def add_rms_norm_bwd_workspace(rows: int, cols: int) -> int:
+    n = c_i64(0)
+    call("oxi_add_rms_norm_bwd_workspace", rows, cols, ctypes.byref(n))
+    return n.value
+
+
+def add_rms_norm_bwd(h, w, rstd, gy, gh=None, mode="ref", need_dx=True, need_dw=True, workspace=None):
+    """Gradients (dx, dw) of x (and r) and w for upstream gy and gh."""
+    rows, H = _rows(h)
+    dx = DeviceArray(h.shape) if need_dx else None
+    dw = DeviceArray((H,)) if need_dw else None
+    call("oxi_add_rms_norm_bwd", h.ptr, w.ptr if w else None, rstd.ptr, gy.ptr, gh.ptr if gh else None,
+         dx.ptr if dx else None, dw.ptr if dw else None, workspace.ptr if workspace else None, rows, H, NORM_VJP[mode])
+    return dx, dw
+
+
+def add_rms_norm_e4m3_fwd(x: DeviceArray, r: DeviceArray | None, w: DeviceArray | None, group: int, eps=1e-6):
+    """(h, q, scale): the forward with y as e4m3 codes (uint8) and a scale per
+    `group` columns of a row; without r, h is None."""
+    rows, H = _rows(x)
+    h = DeviceArray(x.shape) if r else None
+    q = DeviceArray(x.shape, np.uint8)
+    scale = DeviceArray((*x.shape[:-1], -(-H // group) if group > 0 else 0))
+    call("oxi_add_rms_norm_e4m3_fwd", x.ptr, r.ptr if r else None, w.ptr if w else None, h.ptr if h else None, q.ptr,
+         scale.ptr, rows, H, group, eps)
+    return h, q, scale
+
+
+def e4m3_dequantize(q: DeviceArray, scale: DeviceArray, group: int) -> DeviceArray:
+    rows, H = _rows(q)
+    y = DeviceArray(q.shape)
+    call("oxi_e4m3_dequantize", q.ptr, scale.ptr, y.ptr, rows, H, group)
+    return y
+
+
+def rotary(x: DeviceArray, inv_freq: DeviceArray, positions: DeviceArray | None = None, offset=0, layout="half",
+           inverse=False, scale=1.0, out: DeviceArray | None = None, x_strides=None, out_strides=None,
+           pos_strides=None, shape=None) -> DeviceArray:
+    """x (batch, tokens, heads, dim) with the pairs of its first
+    2*len(inv_freq) elements turned by position * inv_freq. `positions`:
+    (batch, tokens) or (tokens,) int64; None: 0, 1, .. along the tokens.
+    `out` may be x."""
+    shape = tuple(shape or x.shape)
+    out = out if out is not None else DeviceArray(shape)
+    rm = row_major_strides(shape)
+    if positions is not None and pos_strides is None:
+        pos_strides = (positions.shape[1], 1) if len(positions.shape) == 2 else (0, 1)
+    call("oxi_rotary", x.ptr, _i64arr(x_strides or rm), out.ptr, _i64arr(out_strides or rm), _i64arr(shape),
+         positions.ptr if positions else None, _i64arr(pos_strides or (0, 0)), offset, inv_freq.ptr,
+         2 * inv_freq.size, ROTARY[layout], int(bool(inverse)), scale)
+    return out
+
+
 def _oli(shape, dim):
     dim = dim % len(shape)
     outer = int(np.prod(shape[:dim], dtype=np.int64))
@@ -454,6 +531,44 @@ def cross_entropy_bwd(logits: DeviceArray, targets: DeviceArray, lse: DeviceArra
     d = DeviceArray((n, c))
     call("oxi_cross_entropy_bwd", logits.ptr, targets.ptr, lse.ptr, gloss.ptr, d.ptr, n, c)
     return d
+
+
+def distill_fwd(logits: DeviceArray, ids: DeviceArray, top: DeviceArray, temperature=1.0, top_lse=None, divisor=None,
+                need_grad=False):
+    """The distillation loss against a teacher's top entries (ids int64 and
+    logits, both (n, k)): (loss, row_loss, lse, rest, dlogits or None)."""
+    n, c = logits.shape
+    loss, row_loss, lse, rest = DeviceArray((1,)), DeviceArray((n,)), DeviceArray((n,)), DeviceArray((n,))
+    d = DeviceArray((n, c)) if need_grad else None
+    call("oxi_distill_fwd", logits.ptr, ids.ptr, top.ptr, top_lse.ptr if top_lse else None, loss.ptr, row_loss.ptr,
+         lse.ptr, rest.ptr, d.ptr if d else None, n, c, ids.shape[1], temperature, divisor if divisor else max(1, n))
+    return loss, row_loss, lse, rest, d
+
+
+def distill_bwd(logits: DeviceArray, ids: DeviceArray, top: DeviceArray, lse: DeviceArray, rest: DeviceArray,
+                gloss: DeviceArray, temperature=1.0, top_lse=None, divisor=None) -> DeviceArray:
+    n, c = logits.shape
+    d = DeviceArray((n, c))
+    call("oxi_distill_bwd", logits.ptr, ids.ptr, top.ptr, top_lse.ptr if top_lse else None, lse.ptr, rest.ptr,
+         gloss.ptr, d.ptr, n, c, ids.shape[1], temperature, divisor if divisor else max(1, n))
+    return d
+
+
+def verify_drafts_workspace(batch: int, vocab: int) -> int:
+    n = c_i64(0)
+    call("oxi_verify_drafts_workspace", batch, vocab, ctypes.byref(n))
+    return n.value
+
+
+def verify_drafts(target: DeviceArray, draft: DeviceArray | None, tokens: DeviceArray, uniforms: DeviceArray,
+                  lengths: DeviceArray | None = None, workspace: DeviceArray | None = None):
+    """(accepted, out) int64: how many of each sequence's drafted tokens are
+    kept, and the kept tokens with the one drawn after them, then -1."""
+    b, rows, v = target.shape
+    accepted, out = DeviceArray((b,), np.int64), DeviceArray((b, rows), np.int64)
+    call("oxi_verify_drafts", target.ptr, draft.ptr if draft else None, tokens.ptr, lengths.ptr if lengths else None,
+         uniforms.ptr, accepted.ptr, out.ptr, workspace.ptr if workspace else None, b, rows - 1, v)
+    return accepted, out
 
 
 def index_select(src: DeviceArray, dim: int, idx: DeviceArray) -> DeviceArray:
