@@ -116,32 +116,6 @@ __device__ __forceinline__ double block_before(double v, double* lds, double& al
 // one again. Each block of the first finds the row by itself (a gather of two
 // floats a draft).
 
-// Four neighbouring weights of the row, from v on; classes past its end weigh nothing.
-struct Four {
-  double w[4];
-};
-__device__ __forceinline__ Four weights(const Row& r, int64_t v, int64_t vocab, bool left) {
-  f4 p = {0.f, 0.f, 0.f, 0.f}, q = p;
-  if (v + 4 <= vocab) {
-    p = *reinterpret_cast<const f4u*>(r.p + v);
-    if (left && r.q) q = *reinterpret_cast<const f4u*>(r.q + v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (v + j < vocab) {
-        p[j] = r.p[v + j];
-        if (left && r.q) q[j] = r.q[v + j];
-      }
-  }
-  Four f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const double d = (double)p[j] - (double)q[j];
-    f.w[j] = d > 0.0 && !(left && v + j == r.removed) ? d : 0.0;
-  }
-  return f;
-}
-
 // A chunk's weights: what the draft leaves, and the target's own.
 struct Sums {
   double left, own;
@@ -191,13 +165,29 @@ __global__ __launch_bounds__(NT) void verify_sums_k(const VerifyArgs g, Sums* __
   if (threadIdx.x == 0) part[b * gridDim.x + blockIdx.x] = Sums{left, own};
 }
 
-// chunk: classes a chunk; chunks: of them.
-__global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Sums* __restrict__ part, int64_t chunk,
-                                                    int64_t chunks) {
+// The thread at whose weight the running sum, a thread's weight after those
+// before it, passes `limit`, and the sum before it; -1 where it passes none's.
+struct Crossing {
+  int at;
+  double before;
+};
+template <int N>
+__device__ __forceinline__ Crossing cross(double w, double before, double limit, Crossing* slot) {
+  __syncthreads();
+  if (threadIdx.x == 0) *slot = {-1, 0.0};
+  __syncthreads();
+  if (w > 0.0 && before <= limit && before + w > limit) *slot = {(int)threadIdx.x, before};  // one thread's at most
+  __syncthreads();
+  return *slot;
+}
+
+// U: float4s a thread of a chunk, as in the first launch; chunks: of a row.
+template <int U>
+__global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Sums* __restrict__ part, int64_t chunks) {
+  constexpr int64_t CHUNK = NT * 4 * U;
   __shared__ double red[NT / 64];
-  __shared__ unsigned long long found;
-  __shared__ long long last;
-  __shared__ double base;
+  __shared__ Crossing slot;
+  __shared__ int last;
   const int64_t b = blockIdx.x;
   const int t = threadIdx.x;
   const int64_t kept = g.accepted[b];
@@ -205,71 +195,106 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
   len = min(max(len, (int64_t)0), g.drafts);
   const bool rejected = kept < len;
   const Row r = row_of(g, b, kept, rejected);
+  const double u = (double)g.uniforms[b * (g.drafts + 1) + g.drafts];
   const Sums* pb = part + b * chunks;
-  double own = 0.0, left = 0.0;
+  double left = 0.0, own = 0.0;
   for (int64_t i = t; i < chunks; i += NT) {
     left += pb[i].left;
     own += pb[i].own;
   }
-  own = block_sum<NT>(own, red);
   left = block_sum<NT>(left, red);
+  own = block_sum<NT>(own, red);
   const bool use_left = rejected && left > 0.0;
-  const double limit = (double)g.uniforms[b * (g.drafts + 1) + g.drafts] * (use_left ? left : own);
-  if (t == 0) {
-    found = ~0ull;
-    last = -1;
-    base = 0.0;
-  }
-  __syncthreads();
-  // the first chunk whose end is past the limit, or the last one with weight
-  double carry = 0.0;
+  const double limit = u * (use_left ? left : own);
+  // the chunk
+  int64_t at = -1;
+  double base = 0.0, carry = 0.0;
   for (int64_t i0 = 0; i0 < chunks; i0 += NT) {
-    const int64_t i = i0 + t;
-    const double w = i < chunks ? (use_left ? pb[i].left : pb[i].own) : 0.0;
+    const double w = i0 + t < chunks ? (use_left ? pb[i0 + t].left : pb[i0 + t].own) : 0.0;
     double all;
     const double before = carry + block_before<NT>(w, red, all);
-    if (w > 0.0) {
-      if (before + w > limit) atomicMin(&found, (unsigned long long)i);
-      atomicMax(&last, (long long)i);
+    const Crossing c = cross<NT>(w, before, limit, &slot);
+    if (c.at >= 0) {
+      at = i0 + c.at;
+      base = c.before;
+      break;
     }
-    __syncthreads();
-    const unsigned long long f = found;
-    if (f != ~0ull ? f == (unsigned long long)i : i == last) base = before;
-    __syncthreads();
-    if (f != ~0ull) break;
     carry += all;
   }
-  const int64_t at = found != ~0ull ? (int64_t)found : last;
+  if (at < 0 && carry > 0.0) {  // the last chunk with weight
+    for (int64_t i0 = (chunks - 1) / NT * NT; i0 >= 0 && at < 0; i0 -= NT) {
+      __syncthreads();
+      if (t == 0) last = -1;
+      __syncthreads();
+      if (i0 + t < chunks && (use_left ? pb[i0 + t].left : pb[i0 + t].own) > 0.0) atomicMax(&last, t);
+      __syncthreads();
+      if (last >= 0) at = i0 + last;
+    }
+    base = carry;  // past every limit: the last class with weight is wanted
+  }
   int64_t token = -1;
   if (at >= 0) {
-    carry = base;
-    __syncthreads();
-    if (t == 0) {
-      found = ~0ull;
-      last = -1;
-    }
-    __syncthreads();
-    const int64_t end = min((at + 1) * chunk, g.vocab);
-    for (int64_t v0 = at * chunk; v0 < end; v0 += NT * 4) {
-      const int64_t v = v0 + t * 4;
-      const Four f = weights(r, v, g.vocab, use_left);
-      double all;
-      double run = carry + block_before<NT>((f.w[0] + f.w[1]) + (f.w[2] + f.w[3]), red, all);
+    // a thread's 4 U neighbouring classes
+    const int64_t v0 = at * CHUNK + (int64_t)t * (4 * U);
+    float p[4 * U], q[4 * U];
+    if (v0 + 4 * U <= g.vocab) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (f.w[j] > 0.0) {
-          run += f.w[j];
-          if (run > limit) atomicMin(&found, (unsigned long long)(v + j));
-          atomicMax(&last, (long long)(v + j));
+      for (int k = 0; k < U; ++k) {
+        const f4 pv = *reinterpret_cast<const f4u*>(r.p + v0 + 4 * k);
+        f4 qv = {0.f, 0.f, 0.f, 0.f};
+        if (use_left && r.q) qv = *reinterpret_cast<const f4u*>(r.q + v0 + 4 * k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[4 * k + j] = pv[j];
+          q[4 * k + j] = qv[j];
         }
-      carry += all;
-      __syncthreads();
-      if (found != ~0ull) break;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4 * U; ++j) {
+        p[j] = v0 + j < g.vocab ? r.p[v0 + j] : 0.f;
+        q[j] = v0 + j < g.vocab && use_left && r.q ? r.q[v0 + j] : 0.f;
+      }
     }
-    token = found != ~0ull ? (int64_t)found : (int64_t)last;
+    auto weight = [&](int j) {
+      const double d = (double)p[j] - (double)q[j];
+      return d > 0.0 && !(use_left && v0 + j == r.removed) ? d : 0.0;
+    };
+    double w = 0.0;
+    int mine = -1;  // this thread's last class with weight
+#pragma unroll
+    for (int j = 0; j < 4 * U; ++j) {
+      const double x = weight(j);
+      w += x;
+      if (x > 0.0) mine = j;
+    }
+    double all;
+    const double before = base + block_before<NT>(w, red, all);
+    Crossing c = cross<NT>(w, before, limit, &slot);
+    if (c.at < 0) {  // the last thread with weight, its last class
+      if (t == 0) last = -1;
+      __syncthreads();
+      if (mine >= 0) atomicMax(&last, t);
+      __syncthreads();
+      c.at = last;
+    }
+    if (t == c.at) {
+      double run = before;
+      int hit = -1;
+#pragma unroll
+      for (int j = 0; j < 4 * U; ++j) {
+        const double x = weight(j);
+        run += x;
+        if (hit < 0 && x > 0.0 && run > limit) hit = j;
+      }
+      token = v0 + (hit >= 0 ? hit : mine);
+    } else {
+      token = -2;  // another thread's
+    }
   }
+  if (token != -2 && (at >= 0 || t == 0)) g.out[b * (g.drafts + 1) + kept] = token;
   for (int64_t i = t; i <= g.drafts; i += NT)
-    g.out[b * (g.drafts + 1) + i] = i < kept ? g.tokens[b * g.drafts + i] : i == kept ? token : -1;
+    if (i != kept) g.out[b * (g.drafts + 1) + i] = i < kept ? g.tokens[b * g.drafts + i] : -1;
 }
 
 // Float4s a thread of the first launch: as many as leave two blocks a CU, so that
@@ -315,14 +340,17 @@ int oxi_verify_drafts(const float* target, const float* draft, const int64_t* to
   Sums* part = workspace ? static_cast<Sums*>(workspace) : ws.as<Sums>();
   if (!part) return fail_alloc("verify_drafts: sums");
   const dim3 grid((unsigned)chunks, (unsigned)batch);
+#define OXI_VER(U)                                                                            \
+  verify_sums_k<U><<<grid, dim3(NT), 0, stream()>>>(g, part);                                \
+  if (int rc = check_launch("verify_drafts")) return rc;                                     \
+  verify_pick_k<U><<<dim3((unsigned)batch), dim3(NT), 0, stream()>>>(g, part, chunks);
   switch (u) {
-    case 1: verify_sums_k<1><<<grid, dim3(NT), 0, stream()>>>(g, part); break;
-    case 2: verify_sums_k<2><<<grid, dim3(NT), 0, stream()>>>(g, part); break;
-    case 4: verify_sums_k<4><<<grid, dim3(NT), 0, stream()>>>(g, part); break;
-    default: verify_sums_k<8><<<grid, dim3(NT), 0, stream()>>>(g, part);
+    case 1: OXI_VER(1) break;
+    case 2: OXI_VER(2) break;
+    case 4: OXI_VER(4) break;
+    default: OXI_VER(8)
   }
-  if (int rc = check_launch("verify_drafts")) return rc;
-  verify_pick_k<<<dim3((unsigned)batch), dim3(NT), 0, stream()>>>(g, part, chunk, chunks);
+#undef OXI_VER
   return check_launch("verify_drafts");
 }
 
