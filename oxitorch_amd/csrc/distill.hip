@@ -138,6 +138,16 @@ __device__ __forceinline__ double entry_term(double p, double lp, double lq, boo
   return p > 0.0 || p != p ? p * (expm1(d) - d) : exp(lq);
 }
 
+// What entries of sum psum leave to the other classes.
+__device__ __forceinline__ double rest_of(double psum) { return psum < 1.0 ? 1.0 - psum : psum != psum ? psum : 0.0; }
+
+// The rest's share, lr the logarithm of the student's mass qr there, with what the
+// masses as rounded lack of 1.
+__device__ __forceinline__ double rest_term(double psum, double lr, double qr) {
+  const double pr = rest_of(psum), d = lr - log(pr);
+  return (pr > 0.0 || pr != pr ? pr * (expm1(d) - d) : qr) + ((psum + pr) - 1.0);
+}
+
 // The loss of the row once its maximum, its sum of exp((x - m)/T) and, with
 // the rest's term, the sum over the classes not listed are known; thread 0 writes
 // the row's results. Returns the factor of q at the classes not listed.
@@ -155,11 +165,8 @@ __device__ __forceinline__ float finish_row(const DistillArgs& g, int64_t row, c
   float factor = 1.f;
   const double lr = tail ? log(rest) - lt : 0.0;
   if (tail && some) {
-    const double pr = psum < 1.0 ? 1.0 - psum : psum != psum ? psum : 0.0;
-    const double qr = rest / total;
-    const double d = lr - log(pr);
-    s += pr > 0.0 || pr != pr ? pr * (expm1(d) - d) : qr;
-    s += (psum + pr) - 1.0;
+    const double pr = rest_of(psum), qr = rest / total;
+    s += rest_term(psum, lr, qr);
     factor = qr > 0.0 || qr != qr ? (float)((qr - pr) / qr) : 1.f;
   }
   if (threadIdx.x == 0) {
@@ -243,199 +250,218 @@ __global__ __launch_bounds__(NT) void distill_fwd_k(const DistillArgs g) {
 }
 
 // ---------------------------------------------------------------------------
-// Rows of up to RT * NV float4s at any float alignment, a row per block held in
-// registers, so the logits cross HBM once for the loss and its gradient. The row
-// group waits for its logits first, and works out the teacher's entries
-// meanwhile. Exponentials are exp2 of (x - m) * (log2(e)/T).
-
-// What an entry needs later, kept by its thread: k <= RT entries, thread j's
-// at j.
-struct Entry {
-  double p, lp;
-  float x;   // the student's logit
-  int id;    // -1: padding
-  bool dup;  // an earlier entry has this id
-};
-
-// Bits of slot c's four classes (bit j: class first + j is listed).
-template <int KIND>
-__device__ __forceinline__ uint32_t listed_bits(const uint32_t* bits, int C, int c) {
-  if constexpr (KIND == ROW_ODD) {
-    const int e = min(4 * c, C - 4);
-    const uint64_t two = (uint64_t)bits[e >> 5] | (uint64_t)bits[(e >> 5) + 1] << 32;
-    return (uint32_t)(two >> (e & 31)) & 15u;
-  } else {
-    return bits[c >> 3] >> ((c & 7) * 4) & 15u;
-  }
-}
-
+// A row a block: RT * NV float4s held in registers, so the logits cross HBM once
+// for the loss and its gradient. Rows lie at any float address (unaligned
+// float4s are single instructions); the last c % 4 classes go a float to a
+// thread. Exponentials are exp2 of (x - m) * (log2(e)/T). With the rest's term the
+// listed classes are taken out of the registers (an exponential of 0) by a
+// bitmap in LDS, and their own few are added by the entries' threads. The
+// block's stores write the row as if nothing were listed; the entries' values go
+// over that after a barrier.
+//
+// The entries are worked out in float64 before the row is loaded and their
+// terms after it is stored, from LDS, so that the registers of that code do
+// not add to the row's: two blocks of 1024 x 8 a CU need 64 (see rows_waves).
+//
 // NV = 0: longer rows, streamed twice, the first time with a running maximum; the
 // second time they come from the Infinity Cache (a block a row on every CU is
 // at most 256 rows in flight, 134 MB of 131072 classes).
 constexpr int STREAM_U = 4;         // float4s in flight a thread
-constexpr int STREAM_MAX = 400000;  // classes whose bitmap fits in LDS beside 1024 entries
+constexpr int STREAM_MAX = 300000;  // classes whose bitmap fits in LDS beside 1024 entries
+
+// Waves a SIMD that the registers must allow: 128 a lane.
+constexpr int rows_waves(int nv) { return nv ? 4 : 8; }
 
 __device__ __forceinline__ f4 exp2_4(const f4& z) {
   return f4{__builtin_amdgcn_exp2f(z.x), __builtin_amdgcn_exp2f(z.y), __builtin_amdgcn_exp2f(z.z),
             __builtin_amdgcn_exp2f(z.w)};
 }
 
-template <int RT, int NV, int KIND, bool GRAD, bool TAIL, bool NTS>
-__global__ __launch_bounds__(RT) void distill_rows_k(const DistillArgs g, const float scale2) {
-  __shared__ double red[RT / 64];
-  __shared__ float lds[2 * (RT / 64)];
+// A value that all threads hold, in a scalar register.
+__device__ __forceinline__ float uniform(float v) { return readlane_f32(v, 0); }
+
+// v with the classes of set bits at -inf.
+__device__ __forceinline__ f4 without(const f4& v, uint32_t bits) {
+  return f4{bits & 1 ? NEG_INF : v.x, bits & 2 ? NEG_INF : v.y, bits & 4 ? NEG_INF : v.z, bits & 8 ? NEG_INF : v.w};
+}
+
+template <int RT, int NV, bool GRAD, bool TAIL, bool NTS>
+__global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(NV)))) void distill_rows_k(
+    const DistillArgs g, const float scale2) {
+  __shared__ double red[RT / 64], psum_at;
+  __shared__ float lds[4 * (RT / 64)];
   __shared__ int twice;
-  extern __shared__ __align__(16) double dyn[];  // k probabilities, k ids, a bit a class
+  // k probabilities, k logarithms of them, k ids (-1: padding, -2 - id: an id
+  // that an earlier entry has), the student's logits there, a bit a class
+  extern __shared__ __align__(16) double dyn[];
   double* const ep = dyn;
-  int* const eid = reinterpret_cast<int*>(dyn + g.k);
-  uint32_t* const bits = reinterpret_cast<uint32_t*>(eid + g.k);
+  double* const elp = dyn + g.k;
+  int* const eid = reinterpret_cast<int*>(dyn + 2 * g.k);
+  float* const ex = reinterpret_cast<float*>(eid + g.k);
+  uint32_t* const bits = reinterpret_cast<uint32_t*>(ex + g.k);
   const int t = threadIdx.x;
   const int64_t row = blockIdx.x;
   const int C = g.c;
-  const int h4 = row_slots<KIND>(C);
+  const int c4 = C >> 2;
   const float* xr = g.x + row * C;
+  // float4 c of the row at a 32-bit byte offset from a uniform address: one
+  // register an access, not two
+  auto x4 = [&](int c) -> const f4u* {
+    return reinterpret_cast<const f4u*>(reinterpret_cast<const char*>(xr) + (uint32_t)c * 16u);
+  };
   // the entries' loads go first: a wait for them leaves the row's in flight
   const int64_t id64 = t < g.k ? g.ids[row * g.k + t] : -1;
   const float top = t < g.k ? g.top[row * g.k + t] : 0.f;
   const float tlse = TAIL ? g.top_lse[row] : 0.f;
-  // the plain load keeps a row that is read again in the caches
-  auto load = [&](int c) -> f4 {
-    if constexpr (KIND == ROW_ODD) return ld_odd(xr, C, c);
-    else if constexpr (NV == 0) return reinterpret_cast<const f4*>(xr)[min(c, h4 - 1)];
-    else return ld_stream(reinterpret_cast<const f4*>(xr) + min(c, h4 - 1));
-  };
   f4 v[NV ? NV : 1];
 #pragma unroll
-  for (int q = 0; q < NV; ++q) v[q] = load(q * RT + t);
-  for (int i = t; i < (C >> 5) + 2; i += RT) bits[i] = 0;
+  for (int q = 0; q < NV; ++q) v[q] = ld_stream(x4(min(q * RT + t, c4 - 1)));
+  for (int i = t; i < (C >> 5) + 1; i += RT) bits[i] = 0;
   if (t == 0) twice = 0;
-  Entry e;
-  e.id = t < g.k && id64 >= 0 && id64 < C && top != NEG_INF ? (int)id64 : -1;
-  e.dup = false;
-  e.x = e.id >= 0 ? xr[e.id] : 0.f;
-  if (t < g.k && id64 >= C) atomicOr(g.guard, 1);
-  const bool there = e.id >= 0;
-  if (t < g.k) eid[t] = e.id;
-  const bool some = __syncthreads_or(there) != 0;  // and the bitmap is clear
-  if (there) {
-    const uint32_t bit = 1u << (e.id & 31);
-    if (atomicOr(bits + (e.id >> 5), bit) & bit) twice = 1;
-  }
-  double psum;
-  if constexpr (TAIL) {
-    e.lp = there ? (double)top / g.t - (double)tlse : 0.0;
-    e.p = there ? exp(e.lp) : 0.0;
-    psum = block_sum<RT>(e.p, red);  // its barriers publish the bitmap
-  } else {
-    const float tm = group_max<RT>(there ? top : NEG_INF, lds);
-    e.lp = there ? ((double)top - (double)tm) / g.t : 0.0;
-    e.p = there ? exp(e.lp) : 0.0;
-    psum = block_sum<RT>(e.p, red);
-    e.p = there ? e.p / psum : 0.0;
-    e.lp -= log(psum);
-  }
-  if (t < g.k) ep[t] = e.p;
-  if (twice) {  // ids given twice: rare, so their order is looked up only then
-    if (there)
-      for (int i = 0; i < t && !e.dup; ++i) e.dup = eid[i] == e.id;
-  }
-  // the unlisted (TAIL) or all of slot c's exponentials
-  auto counted = [&](const f4& ev, int c) -> float {
-    f4 u = without_dup<KIND>(ev, C, c);
-    if constexpr (TAIL) {
-      const uint32_t b = listed_bits<KIND>(bits, C, c);
-      u.x = b & 1 ? 0.f : u.x;
-      u.y = b & 2 ? 0.f : u.y;
-      u.z = b & 4 ? 0.f : u.z;
-      u.w = b & 8 ? 0.f : u.w;
+  bool some;
+  float prf = 0.f;     // what the entries leave
+  {
+    double psum;
+    const bool there = id64 >= 0 && id64 < C && top != NEG_INF;
+    if (id64 >= C) atomicOr(g.guard, 1);
+    const int id = there ? (int)id64 : -1;
+    const float xe = there ? xr[id] : NEG_INF;
+    if (t < g.k) eid[t] = id;
+    some = __syncthreads_or(there) != 0;  // and the bitmap is clear
+    if (there) {
+      const uint32_t bit = 1u << (id & 31);
+      if (atomicOr(bits + (id >> 5), bit) & bit) twice = 1;
     }
-    return sum4(u);
-  };
-  float m = NEG_INF, s = 0.f;
+    double lp, p;
+    if constexpr (TAIL) {
+      lp = (double)top / g.t - (double)tlse;
+      p = there ? exp(lp) : 0.0;
+      psum = block_sum<RT>(p, red);  // its barriers publish the bitmap
+    } else {
+      const float tm = group_max<RT>(there ? top : NEG_INF, lds);
+      lp = ((double)top - (double)tm) / g.t;
+      p = there ? exp(lp) : 0.0;
+      psum = block_sum<RT>(p, red);
+      p = there ? p / psum : 0.0;
+      lp -= log(psum);
+    }
+    bool dup = false;
+    if (twice && there)  // ids given twice: rare, so their order is looked up only then
+      for (int i = 0; i < t && !dup; ++i) dup = eid[i] == id;
+    __syncthreads();  // before an id changes under that loop
+    if (t < g.k) {
+      ep[t] = p;
+      elp[t] = lp;
+      ex[t] = xe;
+      if (dup) eid[t] = -2 - id;
+    }
+    if (t == 0) psum_at = psum;
+    prf = uniform((float)rest_of(psum));
+  }
+  auto listed = [&](int c) -> uint32_t { return TAIL ? bits[c >> 3] >> ((c & 7) * 4) & 15u : 0u; };
+  auto listed1 = [&](int e) -> bool { return TAIL && (bits[e >> 5] >> (e & 31) & 1u); };
+  const int e1 = 4 * c4 + t;  // one of the row's last classes
+  float v1 = t < (C & 3) ? xr[e1] : NEG_INF;
+  float m = t < g.k ? ex[t] : NEG_INF, s = 0.f;
   if constexpr (NV > 0) {
 #pragma unroll
-    for (int q = 0; q < NV; ++q) m = fmaxf(m, max4(v[q]));  // slots past the row repeat its last
-    m = group_max<RT>(m, lds);
+    for (int q = 0; q < NV; ++q) {
+      const int c = q * RT + t;
+      v[q] = without(v[q], c < c4 ? listed(c) : 15u);
+      m = fmaxf(m, max4(v[q]));
+    }
+    if (t < (C & 3) && listed1(e1)) v1 = NEG_INF;
+    m = uniform(group_max<RT>(fmaxf(m, v1), lds));
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       v[q] = exp2_4((v[q] - m) * scale2);
-      if (q * RT + t < h4) s += counted(v[q], q * RT + t);
+      s += sum4(v[q]);
     }
+    v1 = __builtin_amdgcn_exp2f((v1 - m) * scale2);
+    s += v1;
   } else {
-    for (int c0 = t; c0 < h4; c0 += STREAM_U * RT) {
+    for (int c0 = t; c0 < c4; c0 += STREAM_U * RT) {
       f4 r[STREAM_U];
 #pragma unroll
-      for (int u = 0; u < STREAM_U; ++u) r[u] = load(c0 + u * RT);
-      float cm = max4(r[0]);
+      for (int u = 0; u < STREAM_U; ++u) r[u] = *x4(min(c0 + u * RT, c4 - 1));  // plain: the row is read again
+      float cm = NEG_INF;
 #pragma unroll
-      for (int u = 1; u < STREAM_U; ++u) cm = fmaxf(cm, max4(r[u]));
+      for (int u = 0; u < STREAM_U; ++u) {
+        const int c = c0 + u * RT;
+        r[u] = without(r[u], c < c4 ? listed(c) : 15u);
+        cm = fmaxf(cm, max4(r[u]));
+      }
       if (cm > m) {
         s *= __builtin_amdgcn_exp2f((m - cm) * scale2);
         m = cm;
       }
       const float ms = m == NEG_INF ? 0.f : m;
 #pragma unroll
-      for (int u = 0; u < STREAM_U; ++u)
-        if (c0 + u * RT < h4) s += counted(exp2_4((r[u] - ms) * scale2), c0 + u * RT);
+      for (int u = 0; u < STREAM_U; ++u) s += sum4(exp2_4((r[u] - ms) * scale2));
     }
+    if (t < (C & 3) && listed1(e1)) v1 = NEG_INF;
     const float own = m;
-    m = group_max<RT>(m, lds);
-    s *= own == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((own - m) * scale2);
+    m = uniform(group_max<RT>(fmaxf(m, v1), lds));
+    s *= own == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((own - m) * scale2);
+    v1 = __builtin_amdgcn_exp2f((v1 - m) * scale2);
+    s += v1;
   }
-  double total = (double)group_sum<RT, float>(s, lds + RT / 64);
-  const double rest = total;
-  const float ex = there ? __builtin_amdgcn_exp2f((e.x - m) * scale2) : 0.f;
-  if constexpr (TAIL) total += block_sum<RT>(e.dup ? 0.0 : (double)ex, red);
-  const double pr = psum < 1.0 ? 1.0 - psum : psum != psum ? psum : 0.0;
+  const float rest = uniform(group_sum_once<RT, float>(s, lds + RT / 64));
+  float total = rest;
+  if constexpr (TAIL) {
+    const float eq = t < g.k && eid[t] >= 0 ? __builtin_amdgcn_exp2f((ex[t] - m) * scale2) : 0.f;
+    total += uniform(group_sum_once<RT, float>(eq, lds + 2 * (RT / 64)));
+  }
   if constexpr (GRAD) {
-    float factor = some ? 1.f : 0.f;
-    if constexpr (TAIL)
-      if (some) {
-        const double qr = rest / total;
-        factor = qr > 0.0 || qr != qr ? (float)((qr - pr) / qr) : 1.f;
-      }
-    const float gs = some ? (float)(1.0 / total) * g.gscale * factor : 0.f;
-    float* dr = g.dx + row * C;
-    auto put = [&](const f4& ev, int c) {
-      const f4 d = some ? ev * gs : f4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (KIND == ROW_ODD) *reinterpret_cast<f4u*>(dr + min(4 * c, C - 4)) = d;
-      else st_stream<NTS>(d, reinterpret_cast<f4*>(dr) + c);
+    float* const dr = g.dx + row * C;
+    auto put = [&](const f4& d, int c) {
+      f4u* const p = reinterpret_cast<f4u*>(reinterpret_cast<char*>(dr) + (uint32_t)c * 16u);
+      if constexpr (NTS) __builtin_nontemporal_store(d, p);
+      else *p = d;
     };
-    if constexpr (NV > 0) {
+    if (some) {
+      float gs = g.gscale / total;
+      if constexpr (TAIL) gs *= rest > 0.f || rest != rest ? 1.f - prf * (total / rest) : 1.f;
+      if constexpr (NV > 0) {
 #pragma unroll
-      for (int q = 0; q < NV; ++q)
-        if (q * RT + t < h4) put(v[q], q * RT + t);
-    } else {
-      for (int c0 = t; c0 < h4; c0 += STREAM_U * RT) {
-        f4 r[STREAM_U];
+        for (int q = 0; q < NV; ++q)
+          if (q * RT + t < c4) put(v[q] * gs, q * RT + t);
+      } else {
+        for (int c0 = t; c0 < c4; c0 += STREAM_U * RT) {
+          f4 r[STREAM_U];
 #pragma unroll
-        for (int u = 0; u < STREAM_U; ++u) r[u] = load(c0 + u * RT);
+          for (int u = 0; u < STREAM_U; ++u) r[u] = ld_stream(x4(min(c0 + u * RT, c4 - 1)));
 #pragma unroll
-        for (int u = 0; u < STREAM_U; ++u)
-          if (c0 + u * RT < h4) put(exp2_4((r[u] - m) * scale2), c0 + u * RT);
+          for (int u = 0; u < STREAM_U; ++u)
+            if (c0 + u * RT < c4) put(exp2_4((r[u] - m) * scale2) * gs, c0 + u * RT);
+        }
       }
+      if (t < (C & 3)) dr[e1] = v1 * gs;
+    } else {
+      for (int c = t; c < c4; c += RT) put(f4{0.f, 0.f, 0.f, 0.f}, c);
+      if (t < (C & 3)) dr[e1] = 0.f;
     }
     __syncthreads();  // the entries' own values go over what the row's threads wrote
-    if (there && !e.dup) {
-      double p = e.p;
+    if (t < g.k && eid[t] >= 0) {
+      const int id = eid[t];
+      double p = ep[t];
       if (twice)
         for (int i = t + 1; i < g.k; ++i)
-          if (eid[i] == e.id) p += ep[i];
-      dr[e.id] = (float)((double)ex / total - p) * g.gscale;
+          if (eid[i] == -2 - id) p += ep[i];
+      const float eq = __builtin_amdgcn_exp2f((ex[t] - m) * scale2);
+      dr[id] = (float)((double)eq / (double)total - p) * g.gscale;
     }
   }
-  const double lt = log(total);
-  double terms = there ? entry_term(e.p, e.lp, ((double)e.x - (double)m) / g.t - lt, TAIL, e.dup) : 0.0;
+  const double lt = log((double)total);
+  double terms = 0.0;
+  if (t < g.k && eid[t] != -1)
+    terms = entry_term(ep[t], elp[t], ((double)ex[t] - (double)m) / g.t - lt, TAIL, eid[t] <= -2);
   terms = block_sum<RT>(terms, red);
   if (t == 0) {
     double lr = 0.0;
     if constexpr (TAIL) {
-      lr = log(rest) - lt;
-      if (some) {
-        const double d = lr - log(pr);
-        terms += pr > 0.0 || pr != pr ? pr * (expm1(d) - d) : rest / total;
-        terms += (psum + pr) - 1.0;
-      }
+      lr = log((double)rest) - lt;
+      if (some) terms += rest_term(psum_at, lr, (double)rest / (double)total);
     }
     g.row_loss[row] = some ? (float)(g.t * g.t * terms) : 0.f;
     g.lse[row] = (float)((double)m / g.t + lt);
@@ -456,8 +482,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(const DistillArgs g, const f
   const float l = g.lse[row];
   float factor = 1.f;
   if (g.top_lse && some) {
-    const double pr = psum < 1.0 ? 1.0 - psum : psum != psum ? psum : 0.0;
-    const double qr = exp((double)g.rest[row]);
+    const double pr = rest_of(psum), qr = exp((double)g.rest[row]);
     factor = qr > 0.0 || qr != qr ? (float)((qr - pr) / qr) : 1.f;
   }
   float* dr = g.dx + row * g.c;
@@ -493,42 +518,47 @@ int check_distill(const char* what, int64_t n, int64_t c, int64_t k, float tempe
   return OXI_OK;
 }
 
-// The register kernel for rows of c floats with k entries: 16 float4s a thread, 8
-// for rows of 16385 to 32768 floats, longer rows streamed; false when none takes them.
-template <int KIND, bool GRAD, bool TAIL, bool NTS>
+// The row kernel for c classes and k entries: as few float4s a thread as hold the
+// row, streamed past 16 on 1024 threads; false where none takes it.
+template <bool GRAD, bool TAIL, bool NTS>
 bool launch_rows(const DistillArgs& g) {
-  const int h4 = (g.c + 3) / 4;
+  const int c4 = g.c / 4;
+  if (c4 < 1 || g.c > STREAM_MAX) return false;
   const dim3 grid((unsigned)g.n);
-  const size_t lds = (size_t)g.k * (sizeof(double) + sizeof(int)) + sizeof(uint32_t) * ((size_t)(g.c >> 5) + 2);
+  const size_t lds = (size_t)g.k * (2 * sizeof(double) + sizeof(int) + sizeof(float)) + sizeof(uint32_t) * ((size_t)(g.c >> 5) + 1);
   const float scale2 = (float)(1.4426950408889634 / g.t);
-#define OXI_DR(RT, NV)                                                                              \
-  if (h4 <= RT * NV && g.k <= RT) {                                                                 \
-    distill_rows_k<RT, NV, KIND, GRAD, TAIL, NTS><<<grid, dim3(RT), lds, stream()>>>(g, scale2);    \
-    return true;                                                                                    \
+#define OXI_DR(RT, NV)                                                                        \
+  if (NV == 0 || (c4 <= RT * NV && g.k <= RT)) {                                              \
+    distill_rows_k<RT, NV, GRAD, TAIL, NTS><<<grid, dim3(RT), lds, stream()>>>(g, scale2);    \
+    return true;                                                                              \
   }
+  OXI_DR(64, 2)
   OXI_DR(64, 4)
+  OXI_DR(64, 8)
   OXI_DR(64, 16)
-  OXI_DR(128, 16)
+  OXI_DR(256, 6)
+  OXI_DR(256, 8)
+  OXI_DR(256, 12)
   OXI_DR(256, 16)
-  OXI_DR(1024, 8)
+  OXI_DR(512, 10)
+  OXI_DR(512, 12)
+  OXI_DR(512, 14)
+  OXI_DR(512, 16)
+  OXI_DR(1024, 10)
+  OXI_DR(1024, 12)
+  OXI_DR(1024, 13)
+  OXI_DR(1024, 14)
   OXI_DR(1024, 16)
+  OXI_DR(1024, 0)
 #undef OXI_DR
-  if (g.c > STREAM_MAX) return false;
-  distill_rows_k<1024, 0, KIND, GRAD, TAIL, NTS><<<grid, dim3(1024), lds, stream()>>>(g, scale2);
-  return true;
+  return false;
 }
 
-template <int KIND, bool NTS>
-bool launch_rows_kind(const DistillArgs& g) {
-  if (g.dx) return g.top_lse ? launch_rows<KIND, true, true, NTS>(g) : launch_rows<KIND, true, false, NTS>(g);
-  return g.top_lse ? launch_rows<KIND, false, true, false>(g) : launch_rows<KIND, false, false, false>(g);
-}
-
+// Non-temporal stores only where rows do not share cache lines.
+template <bool NTS>
 bool launch_rows_any(const DistillArgs& g) {
-  if (g.c < 4) return false;
-  const bool odd = g.c % 4 || (reinterpret_cast<uintptr_t>(g.x) & 15u) || (reinterpret_cast<uintptr_t>(g.dx) & 15u);
-  if (odd) return launch_rows_kind<ROW_ODD, false>(g);
-  return nt_stores(g.n * g.c * 4) ? launch_rows_kind<ROW_VEC, true>(g) : launch_rows_kind<ROW_VEC, false>(g);
+  if (g.dx) return g.top_lse ? launch_rows<true, true, NTS>(g) : launch_rows<true, false, NTS>(g);
+  return g.top_lse ? launch_rows<false, true, false>(g) : launch_rows<false, false, false>(g);
 }
 
 }  // namespace
@@ -549,7 +579,9 @@ int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, c
   if (n == 0) return oxi_fill(loss, 1, 0.f);
   const DistillArgs g{logits, ids,    top, top_lse, row_loss,           lse,         rest, dlogits, n, (int)c,
                       (int)k, 1.0f / temperature, (double)temperature, temperature / divisor, guard_flag()};
-  if (!launch_rows_any(g)) distill_fwd_k<<<dim3((unsigned)n), dim3(NT), teacher_bytes(k), stream()>>>(g);
+  const bool nt = c % 4 == 0 && !(reinterpret_cast<uintptr_t>(dlogits) & 15u) && nt_stores(n * c * 4);
+  if (!(nt ? launch_rows_any<true>(g) : launch_rows_any<false>(g)))
+    distill_fwd_k<<<dim3((unsigned)n), dim3(NT), teacher_bytes(k), stream()>>>(g);
   if (int rc = check_launch("distill_fwd")) return rc;
   distill_mean_k<<<1, 1024, 0, stream()>>>(row_loss, n, (double)divisor, loss);
   return check_launch("distill_fwd: mean");
