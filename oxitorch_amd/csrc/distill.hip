@@ -251,9 +251,9 @@ __global__ __launch_bounds__(NT) void distill_fwd_k(const DistillArgs g) {
 
 // ---------------------------------------------------------------------------
 // A row a block: RT * NV float4s held in registers, so the logits cross HBM once
-// for the loss and its gradient. Rows lie at any float address (unaligned
-// float4s are single instructions); the last c % 4 classes go a float to a
-// thread. Exponentials are exp2 of (x - m) * (log2(e)/T). With the rest's term the
+// for the loss and its gradient. The float4s are a row's 16-byte granules, at
+// whatever float it starts; the up to 3 classes before and after them go a float
+// to a thread. Exponentials are exp2 of (x - m) * (log2(e)/T). With the rest's term the
 // listed classes are taken out of the registers (an exponential of 0) by a
 // bitmap in LDS, and their own few are added by the entries' threads. The
 // block's stores write the row as if nothing were listed; the entries' values go
@@ -276,6 +276,9 @@ __device__ __forceinline__ f4 exp2_4(const f4& z) {
   return f4{__builtin_amdgcn_exp2f(z.x), __builtin_amdgcn_exp2f(z.y), __builtin_amdgcn_exp2f(z.z),
             __builtin_amdgcn_exp2f(z.w)};
 }
+
+// Words of the bitmap of C classes, which starts up to 4 bits in.
+constexpr int bitmap_words(int C) { return (C + 4 + 31) / 32 + 1; }
 
 // A value that all threads hold, in a scalar register.
 __device__ __forceinline__ float uniform(float v) { return readlane_f32(v, 0); }
@@ -302,12 +305,14 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   const int t = threadIdx.x;
   const int64_t row = blockIdx.x;
   const int C = g.c;
-  const int c4 = C >> 2;
   const float* xr = g.x + row * C;
-  // float4 c of the row at a 32-bit byte offset from a uniform address: one
-  // register an access, not two
-  auto x4 = [&](int c) -> const f4u* {
-    return reinterpret_cast<const f4u*>(reinterpret_cast<const char*>(xr) + (uint32_t)c * 16u);
+  // the row's classes before its first 16-byte address, and its float4s from there
+  const int head = (int)((0 - (reinterpret_cast<uintptr_t>(xr) >> 2)) & 3u);
+  const int c4 = (C - head) >> 2;
+  // float4 c at a 32-bit byte offset from a uniform address: one register an
+  // access, not two
+  auto x4 = [&](int c) -> const f4* {
+    return reinterpret_cast<const f4*>(reinterpret_cast<const char*>(xr + head) + (uint32_t)c * 16u);
   };
   // the entries' loads go first: a wait for them leaves the row's in flight
   const int64_t id64 = t < g.k ? g.ids[row * g.k + t] : -1;
@@ -316,7 +321,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   f4 v[NV ? NV : 1];
 #pragma unroll
   for (int q = 0; q < NV; ++q) v[q] = ld_stream(x4(min(q * RT + t, c4 - 1)));
-  for (int i = t; i < (C >> 5) + 1; i += RT) bits[i] = 0;
+  for (int i = t; i < bitmap_words(C); i += RT) bits[i] = 0;
   if (t == 0) twice = 0;
   bool some;
   float prf = 0.f;     // what the entries leave
@@ -329,8 +334,9 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     if (t < g.k) eid[t] = id;
     some = __syncthreads_or(there) != 0;  // and the bitmap is clear
     if (there) {
-      const uint32_t bit = 1u << (id & 31);
-      if (atomicOr(bits + (id >> 5), bit) & bit) twice = 1;
+      const int at = id + 4 - head;  // float4 c has the four bits from 4 (c + 1)
+      const uint32_t bit = 1u << (at & 31);
+      if (atomicOr(bits + (at >> 5), bit) & bit) twice = 1;
     }
     double lp, p;
     if constexpr (TAIL) {
@@ -358,10 +364,12 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     if (t == 0) psum_at = psum;
     prf = uniform((float)rest_of(psum));
   }
-  auto listed = [&](int c) -> uint32_t { return TAIL ? bits[c >> 3] >> ((c & 7) * 4) & 15u : 0u; };
-  auto listed1 = [&](int e) -> bool { return TAIL && (bits[e >> 5] >> (e & 31) & 1u); };
-  const int e1 = 4 * c4 + t;  // one of the row's last classes
-  float v1 = t < (C & 3) ? xr[e1] : NEG_INF;
+  auto listed = [&](int c) -> uint32_t { return TAIL ? bits[(c + 1) >> 3] >> (((c + 1) & 7) * 4) & 15u : 0u; };
+  // one of the up to 3 classes before the float4s, or after them
+  const int e1 = t < 3 ? t : head + 4 * c4 + t - 3;
+  const bool has1 = t < 3 ? t < head : t < 6 && e1 < C;
+  const bool listed1 = TAIL && has1 && (bits[(e1 + 4 - head) >> 5] >> ((e1 + 4 - head) & 31) & 1u);
+  float v1 = has1 && !listed1 ? xr[e1] : NEG_INF;
   float m = t < g.k ? ex[t] : NEG_INF, s = 0.f;
   if constexpr (NV > 0) {
 #pragma unroll
@@ -370,7 +378,6 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
       v[q] = without(v[q], c < c4 ? listed(c) : 15u);
       m = fmaxf(m, max4(v[q]));
     }
-    if (t < (C & 3) && listed1(e1)) v1 = NEG_INF;
     m = uniform(group_max<RT>(fmaxf(m, v1), lds));
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
@@ -399,7 +406,6 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
 #pragma unroll
       for (int u = 0; u < STREAM_U; ++u) s += sum4(exp2_4((r[u] - ms) * scale2));
     }
-    if (t < (C & 3) && listed1(e1)) v1 = NEG_INF;
     const float own = m;
     m = uniform(group_max<RT>(fmaxf(m, v1), lds));
     s *= own == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((own - m) * scale2);
@@ -415,7 +421,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   if constexpr (GRAD) {
     float* const dr = g.dx + row * C;
     auto put = [&](const f4& d, int c) {
-      f4u* const p = reinterpret_cast<f4u*>(reinterpret_cast<char*>(dr) + (uint32_t)c * 16u);
+      f4u* const p = reinterpret_cast<f4u*>(reinterpret_cast<char*>(dr + head) + (uint32_t)c * 16u);
       if constexpr (NTS) __builtin_nontemporal_store(d, p);
       else *p = d;
     };
@@ -436,10 +442,10 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
             if (c0 + u * RT < c4) put(exp2_4((r[u] - m) * scale2) * gs, c0 + u * RT);
         }
       }
-      if (t < (C & 3)) dr[e1] = v1 * gs;
+      if (has1) dr[e1] = v1 * gs;
     } else {
       for (int c = t; c < c4; c += RT) put(f4{0.f, 0.f, 0.f, 0.f}, c);
-      if (t < (C & 3)) dr[e1] = 0.f;
+      if (has1) dr[e1] = 0.f;
     }
     __syncthreads();  // the entries' own values go over what the row's threads wrote
     if (t < g.k && eid[t] >= 0) {
@@ -522,10 +528,10 @@ int check_distill(const char* what, int64_t n, int64_t c, int64_t k, float tempe
 // row, streamed past 16 on 1024 threads; false where none takes it.
 template <bool GRAD, bool TAIL, bool NTS>
 bool launch_rows(const DistillArgs& g) {
-  const int c4 = g.c / 4;
-  if (c4 < 1 || g.c > STREAM_MAX) return false;
+  const int c4 = g.c / 4;  // at most
+  if (g.c < 8 || g.c > STREAM_MAX) return false;
   const dim3 grid((unsigned)g.n);
-  const size_t lds = (size_t)g.k * (2 * sizeof(double) + sizeof(int) + sizeof(float)) + sizeof(uint32_t) * ((size_t)(g.c >> 5) + 1);
+  const size_t lds = (size_t)g.k * (2 * sizeof(double) + sizeof(int) + sizeof(float)) + sizeof(uint32_t) * (size_t)bitmap_words(g.c);
   const float scale2 = (float)(1.4426950408889634 / g.t);
 #define OXI_DR(RT, NV)                                                                        \
   if (NV == 0 || (c4 <= RT * NV && g.k <= RT)) {                                              \
@@ -554,7 +560,6 @@ bool launch_rows(const DistillArgs& g) {
   return false;
 }
 
-// Non-temporal stores only where rows do not share cache lines.
 template <bool NTS>
 bool launch_rows_any(const DistillArgs& g) {
   if (g.dx) return g.top_lse ? launch_rows<true, true, NTS>(g) : launch_rows<true, false, NTS>(g);
@@ -579,7 +584,7 @@ int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, c
   if (n == 0) return oxi_fill(loss, 1, 0.f);
   const DistillArgs g{logits, ids,    top, top_lse, row_loss,           lse,         rest, dlogits, n, (int)c,
                       (int)k, 1.0f / temperature, (double)temperature, temperature / divisor, guard_flag()};
-  const bool nt = c % 4 == 0 && !(reinterpret_cast<uintptr_t>(dlogits) & 15u) && nt_stores(n * c * 4);
+  const bool nt = nt_stores(n * c * 4);
   if (!(nt ? launch_rows_any<true>(g) : launch_rows_any<false>(g)))
     distill_fwd_k<<<dim3((unsigned)n), dim3(NT), teacher_bytes(k), stream()>>>(g);
   if (int rc = check_launch("distill_fwd")) return rc;
