@@ -318,6 +318,10 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   const int64_t id64 = t < g.k ? g.ids[row * g.k + t] : -1;
   const float top = t < g.k ? g.top[row * g.k + t] : 0.f;
   const float tlse = TAIL ? g.top_lse[row] : 0.f;
+  // one of the up to 3 classes before the float4s, or after them
+  const int e1 = t < 3 ? t : head + 4 * c4 + t - 3;
+  const bool has1 = t < 3 ? t < head : t < 6 && e1 < C;
+  float v1 = has1 ? xr[e1] : NEG_INF;
   f4 v[NV ? NV : 1];
 #pragma unroll
   for (int q = 0; q < NV; ++q) v[q] = ld_stream(x4(min(q * RT + t, c4 - 1)));
@@ -365,11 +369,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     prf = uniform((float)rest_of(psum));
   }
   auto listed = [&](int c) -> uint32_t { return TAIL ? bits[(c + 1) >> 3] >> (((c + 1) & 7) * 4) & 15u : 0u; };
-  // one of the up to 3 classes before the float4s, or after them
-  const int e1 = t < 3 ? t : head + 4 * c4 + t - 3;
-  const bool has1 = t < 3 ? t < head : t < 6 && e1 < C;
-  const bool listed1 = TAIL && has1 && (bits[(e1 + 4 - head) >> 5] >> ((e1 + 4 - head) & 31) & 1u);
-  float v1 = has1 && !listed1 ? xr[e1] : NEG_INF;
+  if (TAIL && has1 && (bits[(e1 + 4 - head) >> 5] >> ((e1 + 4 - head) & 31) & 1u)) v1 = NEG_INF;
   float m = t < g.k ? ex[t] : NEG_INF, s = 0.f;
   if constexpr (NV > 0) {
 #pragma unroll
