@@ -63,18 +63,109 @@ __device__ __forceinline__ Teacher teacher_at(double* lds, int k) {
   return a;
 }
 
-// Sum of doubles over the block, the same bits for every thread; `lds` holds a
-// value a wave and is free again after the call.
+// exp, log and exp(d) - 1 - d in 64 bits, from their series: loops over
+// coefficients in constant memory, so that they take few registers where a
+// row is held in the others.
+__constant__ double RECIP[24] = {0.0,       1.0,       1.0 / 2,  1.0 / 3,  1.0 / 4,  1.0 / 5,  1.0 / 6,  1.0 / 7,
+                                 1.0 / 8,   1.0 / 9,   1.0 / 10, 1.0 / 11, 1.0 / 12, 1.0 / 13, 1.0 / 14, 1.0 / 15,
+                                 1.0 / 16,  1.0 / 17,  1.0 / 18, 1.0 / 19, 1.0 / 20, 1.0 / 21, 1.0 / 22, 1.0 / 23};
+constexpr double LN2_HI = 0x1.62e42feep-1, LN2_LO = 0x1.a39ef35793c76p-33;  // ln 2, the first part of 32 bits
+
+// e^x = 2^n e^r, |r| <= ln(2)/2: 13 terms leave r^14/14! < 2^-57.
+__device__ __forceinline__ double exp64(double x) {
+  if (x < -746.0) return 0.0;
+  if (x > 710.0) return (double)__builtin_huge_valf();
+  const double n = rint(x * 1.4426950408889634);
+  const double r = fma(-n, LN2_LO, fma(-n, LN2_HI, x));
+  double p = 1.0;
+#pragma unroll 1
+  for (int k = 13; k > 0; --k) p = fma(p * r, RECIP[k], 1.0);
+  return __builtin_ldexp(p, (int)n);
+}
+
+// x = 2^e m, m in [sqrt(1/2), sqrt(2)): log m = 2 atanh s, s = (m - 1)/(m + 1), |s| < 0.172.
+__device__ __forceinline__ double log64(double x) {
+  if (x == 0.0) return (double)NEG_INF;
+  if (!(x < (double)__builtin_huge_valf())) return x;
+  double m = __builtin_amdgcn_frexp_mant(x);
+  int e = __builtin_amdgcn_frexp_exp(x);
+  if (m < 0.7071067811865476) {
+    m += m;
+    --e;
+  }
+  const double s = (m - 1.0) / (m + 1.0), z = s * s;
+  double p = RECIP[23];
+#pragma unroll 1
+  for (int k = 21; k > 0; k -= 2) p = fma(p, z, RECIP[k]);
+  return fma((double)e, LN2_HI, fma((double)e, LN2_LO, 2.0 * s * p));
+}
+
+// d^2/2 (1 + d/3 (1 + d/4 (...))) for small d.
+__device__ __forceinline__ double exp_rest(double d) {
+  if (!(fabs(d) < 0.5)) return exp64(d) - 1.0 - d;
+  double p = 1.0;
+#pragma unroll 1
+  for (int k = 15; k > 2; --k) p = fma(p * d, RECIP[k], 1.0);
+  return 0.5 * d * d * p;
+}
+
+// Reductions over a wave and over the block in a fixed order, the same bits for
+// every thread. A block's waves leave a value each in LDS, and every row of 16
+// lanes combines all of them: one LDS read a lane. The caller's next reduction
+// takes other slots (N/64 values), or a barrier comes between.
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
+}
+__device__ __forceinline__ double readlane_f64(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)lo | (uint64_t)hi << 32);
+}
+struct AddF64 {
+  typedef double T;
+  __device__ __forceinline__ static T op(T a, T b) { return a + b; }
+  template <int C> __device__ __forceinline__ static T move(T v) { return dpp_f64<C>(v); }
+  __device__ __forceinline__ static T lane(T v, int l) { return readlane_f64(v, l); }
+};
+struct AddF32 {
+  typedef float T;
+  __device__ __forceinline__ static T op(T a, T b) { return a + b; }
+  template <int C> __device__ __forceinline__ static T move(T v) { return dpp_f32<C>(v); }
+  __device__ __forceinline__ static T lane(T v, int l) { return readlane_f32(v, l); }
+};
+struct MaxF32 : AddF32 {
+  __device__ __forceinline__ static T op(T a, T b) { return fmaxf(a, b); }
+};
+template <int N, class R>
+__device__ __forceinline__ typename R::T over_block(typename R::T v, typename R::T* slots) {
+  v = R::op(v, R::template move<DPP_QUAD_XOR1>(v));
+  v = R::op(v, R::template move<DPP_QUAD_XOR2>(v));
+  v = R::op(v, R::template move<DPP_ROW_HALF_MIRROR>(v));
+  v = R::op(v, R::template move<DPP_ROW_MIRROR>(v));
+  v = R::op(R::op(R::lane(v, 0), R::lane(v, 16)), R::op(R::lane(v, 32), R::lane(v, 48)));
+  constexpr int W = N / 64;
+  static_assert(W == 1 || W == 4 || W == 8 || W == 16);
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 63) == 0) slots[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = slots[threadIdx.x & (W - 1)];
+    v = R::op(v, R::template move<DPP_QUAD_XOR1>(v));
+    v = R::op(v, R::template move<DPP_QUAD_XOR2>(v));
+    if constexpr (W > 4) v = R::op(v, R::template move<DPP_ROW_HALF_MIRROR>(v));
+    if constexpr (W > 8) v = R::op(v, R::template move<DPP_ROW_MIRROR>(v));
+    v = R::lane(v, 0);
+  }
+  return v;
+}
 template <int N>
-__device__ __forceinline__ double block_sum(double v, double* lds) {
-  v = wave_sum<double>(v);
+__device__ __forceinline__ double block_sum(double v, double* slots) {
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double s = lds[0];
-#pragma unroll
-  for (int i = 1; i < N / 64; ++i) s += lds[i];
-  return s;
+  return over_block<N, AddF64>(v, slots);
 }
 
 // Fills `a` with the row's entries; returns the sum of p, and whether there is
@@ -106,7 +197,7 @@ __device__ __forceinline__ double load_teacher(const DistillArgs& g, int64_t row
     const bool there = a.id[j] >= 0;
     const double v = a.lp[j];
     const double l = g.top_lse ? v / g.t - (double)g.top_lse[row] : (v - (double)tm) / g.t;
-    const double p = there ? exp(l) : 0.0;
+    const double p = there ? exp64(l) : 0.0;
     a.lp[j] = l;
     a.p[j] = p;
     s += p;
@@ -118,7 +209,7 @@ __device__ __forceinline__ double load_teacher(const DistillArgs& g, int64_t row
   }
   s = block_sum<N>(s, red);
   if (!g.top_lse && some) {  // divide by the sum
-    const double ls = log(s);
+    const double ls = log64(s);
     for (int j = threadIdx.x; j < g.k; j += N) {
       a.p[j] = a.p[j] / s;
       a.lp[j] -= ls;
@@ -135,7 +226,7 @@ __device__ __forceinline__ double entry_term(double p, double lp, double lq, boo
   const double d = lq - lp;  // log(q / p)
   if (!tail) return p > 0.0 || p != p ? -p * d : 0.0;
   if (dup) return p > 0.0 || p != p ? -p * d - p : 0.0;
-  return p > 0.0 || p != p ? p * (expm1(d) - d) : exp(lq);
+  return p > 0.0 || p != p ? p * exp_rest(d) : exp64(lq);
 }
 
 // What entries of sum psum leave to the other classes.
@@ -144,8 +235,8 @@ __device__ __forceinline__ double rest_of(double psum) { return psum < 1.0 ? 1.0
 // The rest's share, lr the logarithm of the student's mass qr there, with what the
 // masses as rounded lack of 1.
 __device__ __forceinline__ double rest_term(double psum, double lr, double qr) {
-  const double pr = rest_of(psum), d = lr - log(pr);
-  return (pr > 0.0 || pr != pr ? pr * (expm1(d) - d) : qr) + ((psum + pr) - 1.0);
+  const double pr = rest_of(psum), d = lr - log64(pr);
+  return (pr > 0.0 || pr != pr ? pr * exp_rest(d) : qr) + ((psum + pr) - 1.0);
 }
 
 // The loss of the row once its maximum, its sum of exp((x - m)/T) and, with
@@ -155,7 +246,7 @@ template <int N>
 __device__ __forceinline__ float finish_row(const DistillArgs& g, int64_t row, const Teacher& a, double* red,
                                             double psum, bool some, float m, double total, double rest) {
   const bool tail = g.top_lse != nullptr;
-  const double lt = log(total);
+  const double lt = log64(total);
   const float* xr = g.x + row * g.c;
   double s = 0.0;
   for (int j = threadIdx.x; j < g.k; j += N)
@@ -163,7 +254,7 @@ __device__ __forceinline__ float finish_row(const DistillArgs& g, int64_t row, c
       s += entry_term(a.p[j], a.lp[j], ((double)xr[a.id[j]] - (double)m) / g.t - lt, tail, a.dup[j] >= 0);
   s = block_sum<N>(s, red);
   float factor = 1.f;
-  const double lr = tail ? log(rest) - lt : 0.0;
+  const double lr = tail ? log64(rest) - lt : 0.0;
   if (tail && some) {
     const double pr = rest_of(psum), qr = rest / total;
     s += rest_term(psum, lr, qr);
@@ -345,15 +436,15 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     double lp, p;
     if constexpr (TAIL) {
       lp = (double)top / g.t - (double)tlse;
-      p = there ? exp(lp) : 0.0;
+      p = there ? exp64(lp) : 0.0;
       psum = block_sum<RT>(p, red);  // its barriers publish the bitmap
     } else {
-      const float tm = group_max<RT>(there ? top : NEG_INF, lds);
+      const float tm = over_block<RT, MaxF32>(there ? top : NEG_INF, lds);
       lp = ((double)top - (double)tm) / g.t;
-      p = there ? exp(lp) : 0.0;
+      p = there ? exp64(lp) : 0.0;
       psum = block_sum<RT>(p, red);
       p = there ? p / psum : 0.0;
-      lp -= log(psum);
+      lp -= log64(psum);
     }
     bool dup = false;
     if (twice && there)  // ids given twice: rare, so their order is looked up only then
@@ -378,7 +469,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
       v[q] = without(v[q], c < c4 ? listed(c) : 15u);
       m = fmaxf(m, max4(v[q]));
     }
-    m = uniform(group_max<RT>(fmaxf(m, v1), lds));
+    m = over_block<RT, MaxF32>(fmaxf(m, v1), lds + RT / 64);
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       v[q] = exp2_4((v[q] - m) * scale2);
@@ -407,16 +498,16 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
       for (int u = 0; u < STREAM_U; ++u) s += sum4(exp2_4((r[u] - ms) * scale2));
     }
     const float own = m;
-    m = uniform(group_max<RT>(fmaxf(m, v1), lds));
+    m = over_block<RT, MaxF32>(fmaxf(m, v1), lds + RT / 64);
     s *= own == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((own - m) * scale2);
     v1 = __builtin_amdgcn_exp2f((v1 - m) * scale2);
     s += v1;
   }
-  const float rest = uniform(group_sum_once<RT, float>(s, lds + RT / 64));
+  const float rest = over_block<RT, AddF32>(s, lds + 2 * (RT / 64));
   float total = rest;
   if constexpr (TAIL) {
     const float eq = t < g.k && eid[t] >= 0 ? __builtin_amdgcn_exp2f((ex[t] - m) * scale2) : 0.f;
-    total += uniform(group_sum_once<RT, float>(eq, lds + 2 * (RT / 64)));
+    total += over_block<RT, AddF32>(eq, lds + 3 * (RT / 64));
   }
   if constexpr (GRAD) {
     float* const dr = g.dx + row * C;
@@ -458,7 +549,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
       dr[id] = (float)((double)eq / (double)total - p) * g.gscale;
     }
   }
-  const double lt = log((double)total);
+  const double lt = log64((double)total);
   double terms = 0.0;
   if (t < g.k && eid[t] != -1)
     terms = entry_term(ep[t], elp[t], ((double)ex[t] - (double)m) / g.t - lt, TAIL, eid[t] <= -2);
@@ -466,7 +557,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   if (t == 0) {
     double lr = 0.0;
     if constexpr (TAIL) {
-      lr = log((double)rest) - lt;
+      lr = log64((double)rest) - lt;
       if (some) terms += rest_term(psum_at, lr, (double)rest / (double)total);
     }
     g.row_loss[row] = some ? (float)(g.t * g.t * terms) : 0.f;
@@ -488,7 +579,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(const DistillArgs g, const f
   const float l = g.lse[row];
   float factor = 1.f;
   if (g.top_lse && some) {
-    const double pr = rest_of(psum), qr = exp((double)g.rest[row]);
+    const double pr = rest_of(psum), qr = exp64((double)g.rest[row]);
     factor = qr > 0.0 || qr != qr ? (float)((qr - pr) / qr) : 1.f;
   }
   float* dr = g.dx + row * g.c;
