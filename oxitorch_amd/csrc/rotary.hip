@@ -5,12 +5,14 @@
 //
 // The angle is formed and reduced in 64 bits: at position 10^6 a 32-bit product
 // is off by up to 0.06. A block takes a few tokens with some or all of their
-// heads: its threads first form the tokens' cosines and sines, once for all
-// heads, in LDS, then stream the heads through registers in units of 2W
-// elements (W pairs, or 2W elements that are copied), four units in flight.
+// heads. A head is cut into units of 2W elements (W pairs, or 2W elements that
+// are copied); a thread has one unit, of some of the block's (token, head) rows,
+// ROWS of them in flight. The first of them are loaded before the block forms its
+// tokens' cosines and sines, once for all heads, in LDS. HBM bounds it.
 #include <algorithm>
 
 #include "internal.h"
+#include "launch_limits.h"
 #include "rowtile.h"
 
 namespace oxi {
@@ -20,19 +22,13 @@ constexpr int BS = 256;
 constexpr int MAX_DIM = 8192;    // elements a head
 constexpr int MAX_TOKENS = 64;   // tokens a block
 constexpr int ANGLES = 2048;     // cosines a block forms, when one token's fit
-
-// n / d for n * d < 2^32: the high half of n * ceil(2^32 / d).
-struct Divider {
-  uint32_t d, m;
-};
-Divider divider(uint32_t d) { return {d, d > 1 ? (uint32_t)((((uint64_t)1 << 32) + d - 1) / d) : 0}; }
-__device__ __forceinline__ uint32_t quotient(uint32_t n, const Divider& v) { return v.d > 1 ? __umulhi(n, v.m) : n; }
+constexpr int ROWS = 2;
 
 struct RotaryArgs {
   const float* x;
   float* y;
   int64_t xs[4], ys[4];  // strides of (batch, token, head, element)
-  int64_t tokens, all;   // tokens a sequence, and of all of them
+  uint32_t tokens, all;  // tokens a sequence, and of all of them
   int64_t ps[2];         // strides of the positions
   const int64_t* positions;
   int64_t offset;
@@ -41,8 +37,8 @@ struct RotaryArgs {
   int interleaved;
   float scale, sin_scale;
   int block_tokens, block_heads;
-  int token_first;         // units go through a head's tokens before its next head
-  Divider units, inner;    // units a head; tokens or heads, whichever go first
+  int units;        // units a head
+  int token_first;  // a thread's rows go through a head's tokens before its next head
 };
 
 // cos and sin of 2 pi r, |r| <= 1/2: the nearest quarter turn taken off, both
@@ -69,10 +65,11 @@ __device__ __forceinline__ void cos_sin_turn(double r, float& c, float& s) {
 template <int W>
 struct Vec {
   typedef float T __attribute__((ext_vector_type(W), aligned(4)));
+  typedef float Whole __attribute__((ext_vector_type(W)));  // at its own alignment: LDS
 };
 template <>
 struct Vec<1> {
-  typedef float T;
+  typedef float T, Whole;
 };
 
 template <int W, bool NTS>
@@ -82,107 +79,143 @@ __device__ __forceinline__ void put(typename Vec<W>::T v, float* p) {
   else *reinterpret_cast<V*>(p) = v;
 }
 
+template <int W>
+__device__ __forceinline__ typename Vec<W>::T get(const float* p) {
+  typedef typename Vec<W>::T V;
+  return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+}
+
+// The W/2 neighbouring pairs of x turned.
+template <int W, class H>
+__device__ __forceinline__ typename Vec<W>::T turned(typename Vec<W>::T x, H c, H s) {
+  if constexpr (W == 2) {
+    return {x.x * c - x.y * s, x.y * c + x.x * s};
+  } else if constexpr (W == 4) {
+    return {x.x * c.x - x.y * s.x, x.y * c.x + x.x * s.x, x.z * c.y - x.w * s.y, x.w * c.y + x.z * s.y};
+  } else {
+    return x;
+  }
+}
+
 // W: pairs a unit. STRIDED: elements lie apart (W = 1 only).
 template <int W, bool STRIDED, bool NTS>
 __global__ __launch_bounds__(BS) void rotary_k(const RotaryArgs g) {
   typedef typename Vec<W>::T V;
-  constexpr int U = 4;  // units in flight a thread
   extern __shared__ __align__(16) float lds[];  // block_tokens x half cosines, then as many sines
   __shared__ int64_t xbase[MAX_TOKENS], ybase[MAX_TOKENS];
-  const int64_t i0 = (int64_t)blockIdx.x * g.block_tokens;
-  const int nt = (int)min((int64_t)g.block_tokens, g.all - i0);
+  const uint32_t i0 = blockIdx.x * (uint32_t)g.block_tokens;
+  const int nt = min(g.block_tokens, (int)(g.all - i0));
   const int head0 = blockIdx.y * g.block_heads;
   const int nh = min(g.block_heads, g.heads - head0);
+  const int unit0 = blockIdx.z * BS;
+  const int nu = min(g.units - unit0, BS);
   float* const cs = lds;
   float* const sn = lds + g.block_tokens * g.half;
+  auto position = [&](int k) -> int64_t {
+    const uint32_t b = (i0 + k) / g.tokens, t = (i0 + k) % g.tokens;
+    return g.offset + (g.positions ? g.positions[b * g.ps[0] + t * g.ps[1]] : (int64_t)t);
+  };
+  const int angles = nt * g.half;
+  int64_t pos = 0;
+  double freq = 0.0;
+  if ((int)threadIdx.x < angles) {
+    pos = position(threadIdx.x / g.half);
+    freq = g.inv_freq[threadIdx.x % g.half];
+  }
   for (int j = threadIdx.x; j < nt; j += BS) {
-    const int64_t b = (i0 + j) / g.tokens, t = (i0 + j) % g.tokens;
+    const uint32_t b = (i0 + j) / g.tokens, t = (i0 + j) % g.tokens;
     xbase[j] = b * g.xs[0] + t * g.xs[1] + head0 * g.xs[2];
     ybase[j] = b * g.ys[0] + t * g.ys[1] + head0 * g.ys[2];
   }
-  for (int j = threadIdx.x; j < nt * g.half; j += BS) {
-    const int k = j / g.half, i = j - k * g.half;
-    const int64_t b = (i0 + k) / g.tokens, t = (i0 + k) % g.tokens;
-    const int64_t pos = g.offset + (g.positions ? g.positions[b * g.ps[0] + t * g.ps[1]] : t);
-    const double a = (double)pos * g.inv_freq[i] * 0.15915494309189535;  // turns
+  // this thread's unit and the first of its rows; `step` rows on is the next
+  const int step = BS / nu;
+  const int first = threadIdx.x / nu;
+  const int unit = unit0 + threadIdx.x - first * nu;
+  const int inner = g.token_first ? nt : nh, outer = g.token_first ? nh : nt;
+  const int turning = g.half / W;
+  const bool turn = unit < turning;
+  // The unit's two vectors: W elements each of the head's turning (or copied)
+  // half and of its other half, in the interleaved layout too (W/2 pairs each), so
+  // that neighbouring threads read neighbouring vectors; single pairs as they lie.
+  const int p = unit * W;
+  const int c0 = p - g.half;  // a copied unit's first element past the turning ones
+  const int rest = g.dim - 2 * g.half;
+  const int e0 = !turn ? 2 * g.half + c0 : W == 1 && g.interleaved ? 2 * p : p;
+  const int e1 = !turn ? 2 * g.half + (rest + 1) / 2 + c0 : W == 1 && g.interleaved ? 2 * p + 1 : p + g.half;
+  const bool has1 = W > 1 || e1 < g.dim;  // an odd count of copied elements
+  int i = first % inner, o = first < step ? first / inner : outer;  // threads past the last whole row: none
+  const int di = step % inner, dq = step / inner;
+  __syncthreads();
+  V a[ROWS], b[ROWS];
+  int tok[ROWS], head[ROWS];
+  bool in[ROWS];
+  auto load = [&]() {
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      in[u] = o < outer;
+      tok[u] = g.token_first ? i : o;
+      head[u] = g.token_first ? o : i;
+      i += di;
+      o += dq;
+      if (i >= inner) {
+        i -= inner;
+        ++o;
+      }
+      if (!in[u]) continue;
+      const float* x = g.x + xbase[tok[u]] + head[u] * g.xs[2];
+      if constexpr (STRIDED) {
+        a[u] = x[e0 * g.xs[3]];
+        if (has1) b[u] = x[e1 * g.xs[3]];
+      } else {
+        a[u] = get<W>(x + e0);
+        if (has1) b[u] = get<W>(x + e1);
+      }
+    }
+  };
+  load();
+  for (int j = threadIdx.x; j < angles; j += BS) {
+    if (j != (int)threadIdx.x) {
+      pos = position(j / g.half);
+      freq = g.inv_freq[j % g.half];
+    }
+    const double a = (double)pos * freq * 0.15915494309189535;  // turns
     float c, s;
     cos_sin_turn(a - rint(a), c, s);
     cs[j] = c * g.scale;
     sn[j] = s * g.sin_scale;
   }
   __syncthreads();
-  const uint32_t nu = g.units.d;
-  const uint32_t turning = g.half / W;
-  // a last block's tokens, or heads, may be fewer than the divider's
-  for (uint32_t n0 = threadIdx.x; n0 < (uint32_t)g.block_tokens * g.block_heads * nu; n0 += U * BS) {
-    V a[U], b[U];
-    const float* xp[U];
-    float* yp[U];
-    int tok[U];
-    int e0[U], e1[U];
-    uint32_t unit[U];
-    bool in[U];
+  while (in[0]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t q = n0 + u * BS;
-      const uint32_t r = quotient(q, g.units);
-      unit[u] = q - r * nu;
-      const uint32_t o = quotient(r, g.inner), i = r - o * g.inner.d;
-      tok[u] = g.token_first ? i : o;
-      const int head = g.token_first ? o : i;
-      in[u] = tok[u] < nt && head < nh;
-      const bool turn = unit[u] < turning;
-      const int p = unit[u] * W;  // first pair, or half the first element of a copied unit
-      e0[u] = turn && !g.interleaved ? p : 2 * p;
-      e1[u] = turn && !g.interleaved ? p + g.half : 2 * p + W;
+    for (int u = 0; u < ROWS; ++u) {
       if (!in[u]) continue;
-      xp[u] = g.x + xbase[tok[u]] + head * g.xs[2];
-      yp[u] = g.y + ybase[tok[u]] + head * g.ys[2];
-      if constexpr (STRIDED) {
-        a[u] = xp[u][e0[u] * g.xs[3]];
-        if (e1[u] < g.dim) b[u] = xp[u][e1[u] * g.xs[3]];
-      } else {
-        a[u] = *reinterpret_cast<const V*>(xp[u] + e0[u]);
-        if (W > 1 || e1[u] < g.dim) b[u] = *reinterpret_cast<const V*>(xp[u] + e1[u]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (!in[u]) continue;
-      if (unit[u] < turning) {
-        const float* c = cs + tok[u] * g.half + unit[u] * W;
-        const float* s = sn + tok[u] * g.half + unit[u] * W;
-        if constexpr (W == 1) {
-          const float p = a[u], q = b[u];
-          a[u] = p * c[0] - q * s[0];
-          b[u] = q * c[0] + p * s[0];
-        } else if (g.interleaved) {
-#pragma unroll
-          for (int j = 0; j < W; j += 2) {
-            const float p = a[u][j], q = a[u][j + 1];
-            a[u][j] = p * c[j / 2] - q * s[j / 2];
-            a[u][j + 1] = q * c[j / 2] + p * s[j / 2];
-            const float p2 = b[u][j], q2 = b[u][j + 1];
-            b[u][j] = p2 * c[(W + j) / 2] - q2 * s[(W + j) / 2];
-            b[u][j + 1] = q2 * c[(W + j) / 2] + p2 * s[(W + j) / 2];
-          }
+      if (turn) {
+        const float* ct = cs + tok[u] * g.half;
+        const float* st = sn + tok[u] * g.half;
+        if (W > 1 && g.interleaved) {
+          typedef typename Vec<(W > 1 ? W / 2 : 1)>::Whole H;
+          const H ca = *reinterpret_cast<const H*>(ct + p / 2), sa = *reinterpret_cast<const H*>(st + p / 2);
+          const H cb = *reinterpret_cast<const H*>(ct + (g.half + p) / 2), sb = *reinterpret_cast<const H*>(st + (g.half + p) / 2);
+          a[u] = turned<W>(a[u], ca, sa);
+          b[u] = turned<W>(b[u], cb, sb);
         } else {
-#pragma unroll
-          for (int j = 0; j < W; ++j) {
-            const float p = a[u][j], q = b[u][j];
-            a[u][j] = p * c[j] - q * s[j];
-            b[u][j] = q * c[j] + p * s[j];
-          }
+          const V c = *reinterpret_cast<const typename Vec<W>::Whole*>(ct + p);
+          const V s = *reinterpret_cast<const typename Vec<W>::Whole*>(st + p);
+          const V x = a[u], y = b[u];
+          a[u] = x * c - y * s;
+          b[u] = y * c + x * s;
         }
       }
+      float* y = g.y + ybase[tok[u]] + head[u] * g.ys[2];
       if constexpr (STRIDED) {
-        yp[u][e0[u] * g.ys[3]] = a[u];
-        if (e1[u] < g.dim) yp[u][e1[u] * g.ys[3]] = b[u];
+        y[e0 * g.ys[3]] = a[u];
+        if (has1) y[e1 * g.ys[3]] = b[u];
       } else {
-        put<W, NTS>(a[u], yp[u] + e0[u]);
-        if (W > 1 || e1[u] < g.dim) put<W, NTS>(b[u], yp[u] + e1[u]);
+        put<W, NTS>(a[u], y + e0);
+        if (has1) put<W, NTS>(b[u], y + e1);
       }
     }
+    load();
   }
 }
 
@@ -205,9 +238,8 @@ int oxi_rotary(const float* x, const int64_t* x_strides, float* y, const int64_t
     n *= shape[d] ? shape[d] : 1;
   }
   const int64_t dim = shape[3];
-  if (dim > MAX_DIM || shape[2] > ((int64_t)1 << 20))
-    return fail(OXI_INVALID_ARGUMENT, "rotary: %lld heads of %lld elements exceed the kernel limits",
-                (long long)shape[2], (long long)dim);
+  if (dim > MAX_DIM || shape[2] > ((int64_t)1 << 20) || shape[0] * (shape[1] ? shape[1] : 1) >= (int64_t)1 << 31)
+    return fail(OXI_INVALID_ARGUMENT, "rotary: size exceeds the kernel limits");
   if (rot < 0 || rot > dim || rot % 2)
     return fail(OXI_INVALID_ARGUMENT, "rotary: %lld elements of a head of %lld to turn: an even number, at most all",
                 (long long)rot, (long long)dim);
@@ -230,8 +262,8 @@ int oxi_rotary(const float* x, const int64_t* x_strides, float* y, const int64_t
     a.xs[d] = x_strides[d];
     a.ys[d] = y_strides[d];
   }
-  a.tokens = shape[1];
-  a.all = shape[0] * shape[1];
+  a.tokens = (uint32_t)shape[1];
+  a.all = (uint32_t)(shape[0] * shape[1]);
   a.ps[0] = positions ? pos_strides[0] : 0;
   a.ps[1] = positions ? pos_strides[1] : 0;
   a.positions = positions;
@@ -247,25 +279,28 @@ int oxi_rotary(const float* x, const int64_t* x_strides, float* y, const int64_t
   int w = strided ? 1 : 4;
   while (w > 1 && (a.half % w || (dim - rot) % (2 * w))) w /= 2;
   const int64_t units = ceil_div(dim - rot, 2 * w) + a.half / w;
-  // A block's work: tokens and heads of about 8 units a thread where there are
-  // enough blocks for every CU at that, down to one unit a thread.
-  int64_t goal = 8 * BS;
-  while (goal > BS && a.all * a.heads * units < goal * 2 * cu_count()) goal /= 2;
-  int64_t heads = std::min<int64_t>(a.heads, std::max<int64_t>(1, goal / units));
-  int64_t tokens = std::max<int64_t>(1, goal / (heads * units));
+  // A block's work: tokens and heads of ROWS units a thread, a load of each and
+  // the end, or of one where there are too few for two blocks a CU: 8 units a
+  // thread, loaded four at a time behind the stores before them, took 203 us
+  // for (4, 4096, 32, 128) both ways, 4 at once 190, 2 179, 1 189.
+  const int64_t wide = std::min<int64_t>(units, BS);
+  const int64_t goal = (int64_t)a.all * a.heads * wide < (int64_t)ROWS * BS * 2 * cu_count() ? BS : ROWS * BS;
+  int64_t heads = std::min<int64_t>(a.heads, std::max<int64_t>(1, goal / wide));
+  int64_t tokens = std::max<int64_t>(1, goal / (heads * wide));
   tokens = std::min<int64_t>(std::min<int64_t>(tokens, MAX_TOKENS), a.half ? std::max(1, ANGLES / a.half) : MAX_TOKENS);
   tokens = std::min<int64_t>(tokens, a.all);
   a.block_tokens = (int)tokens;
   a.block_heads = (int)heads;
+  a.units = (int)units;
   a.token_first = shape[1] > 1 && x_strides[1] < x_strides[2];
-  a.units = divider((uint32_t)units);
-  a.inner = divider((uint32_t)(a.token_first ? tokens : heads));
   const int64_t bx = ceil_div(a.all, tokens), by = ceil_div(a.heads, heads);
   if (!grid_fits(bx, BS) || by > 65535)
     return fail(OXI_INVALID_ARGUMENT, "rotary: size exceeds the kernel limits");
-  const dim3 grid((unsigned)bx, (unsigned)by);
+  const dim3 grid((unsigned)bx, (unsigned)by, (unsigned)ceil_div(units, BS));
   const size_t lds = sizeof(float) * 2 * (size_t)tokens * (size_t)a.half;
-  const bool nts = nt_stores(n * 4);
+  // Non-temporal stores for small outputs and for those over half the Infinity
+  // Cache: of 268 MB 173 us against 179 both ways, of 50 MB 50 against 45.
+  const bool nts = n * 4 < (int64_t)OXI_NT_STORE_LO || n * 4 > (int64_t)128 << 20;
 #define OXI_ROT(W, STRIDED)                                                          \
   if (nts) rotary_k<W, STRIDED, true><<<grid, dim3(BS), lds, stream()>>>(a);         \
   else rotary_k<W, STRIDED, false><<<grid, dim3(BS), lds, stream()>>>(a);
