@@ -554,7 +554,7 @@ int oxi_add_rms_norm_fwd(const float* x, const float* r, const float* w, float* 
   OXI_CHECK_INIT();
   const int cfg = norm_fwd_cfg(rows, cols);
   const bool odd = !vec_ok(cols, {x, r, w, h, y});
-  const bool done = nt_stores(rows * cols * 4)
+  const bool done = nt_stream_stores(rows * cols * 8)
                         ? launch_fwd<OUT_F32, true>(cfg, odd, x, r, w, h, y, rstd, rows, (int)cols, eps, 0, 0)
                         : launch_fwd<OUT_F32, false>(cfg, odd, x, r, w, h, y, rstd, rows, (int)cols, eps, 0, 0);
   if (!done)
@@ -600,7 +600,7 @@ int oxi_add_rms_norm_bwd(const float* h, const float* w, const float* rstd, cons
   if (parts && !part) return fail_alloc("add_rms_norm_bwd: column partials");
   const bool odd = !vec_ok(cols, {h, w, gy, gh, dx, part});
   const int H = (int)cols;
-  const bool nt = nt_stores(rows * cols * 4);
+  const bool nt = nt_stream_stores(rows * cols * 4);
 #define OXI_AB_MODE(MODE)                                                                         \
   if (nt) launch_bwd_cfg<MODE, true>(b, odd, h, w, rstd, gy, gh, dx, part, rows, H, dw);          \
   else launch_bwd_cfg<MODE, false>(b, odd, h, w, rstd, gy, gh, dx, part, rows, H, dw);
@@ -630,7 +630,7 @@ int oxi_add_rms_norm_e4m3_fwd(const float* x, const float* r, const float* w, fl
   const bool odd = !vec_ok(cols, {x, r, w, r ? h : nullptr}) || (reinterpret_cast<uintptr_t>(q) & 3u);
   const int lanes = log_lanes_of(group, groups);
   const bool done =
-      nt_stores(rows * cols * 4)
+      nt_stream_stores(rows * cols * (r ? 5 : 1))
           ? launch_fwd<OUT_E4M3, true>(cfg, odd, x, r, w, h, q, scale, rows, (int)cols, eps, lanes, (int)groups)
           : launch_fwd<OUT_E4M3, false>(cfg, odd, x, r, w, h, q, scale, rows, (int)cols, eps, lanes, (int)groups);
   if (done) return check_launch("add_rms_norm_e4m3_fwd");

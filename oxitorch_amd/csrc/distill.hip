@@ -594,8 +594,16 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(const DistillArgs g, const f
 __global__ __launch_bounds__(1024) void distill_mean_k(const float* __restrict__ row_loss, int64_t n, double divisor,
                                                        float* __restrict__ loss) {
   __shared__ double red[1024 / 64];
+  constexpr int U = 8;  // loads in flight a thread
   double acc = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) acc += (double)row_loss[i];
+  for (int64_t i0 = threadIdx.x; i0 < n; i0 += U * 1024) {
+    float v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = row_loss[min(i0 + u * 1024, n - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * 1024 < n) acc += (double)v[u];
+  }
   acc = block_sum<1024>(acc, red);
   if (threadIdx.x == 0) loss[0] = (float)(acc / divisor);
 }
@@ -675,7 +683,7 @@ int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, c
   if (n == 0) return oxi_fill(loss, 1, 0.f);
   const DistillArgs g{logits, ids,    top, top_lse, row_loss,           lse,         rest, dlogits, n, (int)c,
                       (int)k, 1.0f / temperature, (double)temperature, temperature / divisor, guard_flag()};
-  const bool nt = nt_stores(n * c * 4);
+  const bool nt = nt_stream_stores(n * c * 4);
   if (!(nt ? launch_rows_any<true>(g) : launch_rows_any<false>(g)))
     distill_fwd_k<<<dim3((unsigned)n), dim3(NT), teacher_bytes(k), stream()>>>(g);
   if (int rc = check_launch("distill_fwd")) return rc;

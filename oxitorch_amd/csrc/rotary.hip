@@ -298,9 +298,7 @@ int oxi_rotary(const float* x, const int64_t* x_strides, float* y, const int64_t
     return fail(OXI_INVALID_ARGUMENT, "rotary: size exceeds the kernel limits");
   const dim3 grid((unsigned)bx, (unsigned)by, (unsigned)ceil_div(units, BS));
   const size_t lds = sizeof(float) * 2 * (size_t)tokens * (size_t)a.half;
-  // Non-temporal stores for small outputs and for those over half the Infinity
-  // Cache: of 268 MB 173 us against 179 both ways, of 50 MB 50 against 45.
-  const bool nts = n * 4 < (int64_t)OXI_NT_STORE_LO || n * 4 > (int64_t)128 << 20;
+  const bool nts = nt_stream_stores(n * 4);
 #define OXI_ROT(W, STRIDED)                                                          \
   if (nts) rotary_k<W, STRIDED, true><<<grid, dim3(BS), lds, stream()>>>(a);         \
   else rotary_k<W, STRIDED, false><<<grid, dim3(BS), lds, stream()>>>(a);

@@ -110,32 +110,32 @@ __device__ __forceinline__ double block_before(double v, double* lds, double& al
 }
 
 // ---------------------------------------------------------------------------
-// Two launches: the first cuts each sequence's row into chunks of NT threads x
-// U float4s, a block a chunk, which sums its weights; the second, a block a
-// sequence, finds the chunk that the drawn number falls into and reads that
+// Two launches: the first cuts each sequence's row into pieces of 64 lanes x U
+// float4s, a wave a piece, which sums its weights; the second, a block a
+// sequence, finds the piece that the drawn number falls into and reads that
 // one again. Each block of the first finds the row by itself (a gather of two
 // floats a draft).
 
-// A chunk's weights: what the draft leaves, and the target's own.
+// A piece's weights: what the draft leaves, and the target's own.
 struct Sums {
   double left, own;
 };
 
 template <int U>
-__global__ __launch_bounds__(NT) void verify_sums_k(const VerifyArgs g, Sums* __restrict__ part) {
+__global__ __launch_bounds__(NT) void verify_sums_k(const VerifyArgs g, Sums* __restrict__ part, int64_t pieces) {
   __shared__ unsigned long long slot;
-  __shared__ double red[NT / 64];
   const int64_t b = blockIdx.y;
   bool rejected;
   const int64_t kept = count_kept<NT>(g, b, &slot, rejected);
   if (blockIdx.x == 0 && threadIdx.x == 0) g.accepted[b] = kept;
   const Row r = row_of(g, b, kept, rejected);
-  const int64_t v0 = (int64_t)blockIdx.x * (NT * 4 * U);
+  const int64_t piece = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+  const int64_t v0 = piece * (256 * U) + (threadIdx.x & 63) * 4;
   double own = 0.0, left = 0.0;
   f4 p[U], q[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t v = v0 + (int64_t)(u * NT + threadIdx.x) * 4;
+    const int64_t v = v0 + u * 256;
     p[u] = q[u] = f4{0.f, 0.f, 0.f, 0.f};
     if (v + 4 <= g.vocab) {
       p[u] = *reinterpret_cast<const f4u*>(r.p + v);
@@ -151,18 +151,17 @@ __global__ __launch_bounds__(NT) void verify_sums_k(const VerifyArgs g, Sums* __
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t v = v0 + (int64_t)(u * NT + threadIdx.x) * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double pd = p[u][j] > 0.f ? (double)p[u][j] : 0.0;
       const double d = (double)p[u][j] - (double)q[u][j];
       own += pd;
-      left += d > 0.0 && v + j != r.removed ? d : 0.0;
+      left += d > 0.0 && v0 + u * 256 + j != r.removed ? d : 0.0;
     }
   }
-  own = block_sum<NT>(own, red);
-  left = block_sum<NT>(left, red);
-  if (threadIdx.x == 0) part[b * gridDim.x + blockIdx.x] = Sums{left, own};
+  own = wave_sum<double>(own);
+  left = wave_sum<double>(left);
+  if ((threadIdx.x & 63) == 0 && piece < pieces) part[b * pieces + piece] = Sums{left, own};
 }
 
 // The thread at whose weight the running sum, a thread's weight after those
@@ -181,10 +180,10 @@ __device__ __forceinline__ Crossing cross(double w, double before, double limit,
   return *slot;
 }
 
-// U: float4s a thread of a chunk, as in the first launch; chunks: of a row.
+// U: as in the first launch, the classes of a piece that each thread has.
 template <int U>
-__global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Sums* __restrict__ part, int64_t chunks) {
-  constexpr int64_t CHUNK = NT * 4 * U;
+__global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Sums* __restrict__ part, int64_t pieces) {
+  static_assert(NT == 256, "a piece is 256 U classes");
   __shared__ double red[NT / 64];
   __shared__ Crossing slot;
   __shared__ int last;
@@ -196,9 +195,9 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
   const bool rejected = kept < len;
   const Row r = row_of(g, b, kept, rejected);
   const double u = (double)g.uniforms[b * (g.drafts + 1) + g.drafts];
-  const Sums* pb = part + b * chunks;
+  const Sums* pb = part + b * pieces;
   double left = 0.0, own = 0.0;
-  for (int64_t i = t; i < chunks; i += NT) {
+  for (int64_t i = t; i < pieces; i += NT) {
     left += pb[i].left;
     own += pb[i].own;
   }
@@ -206,11 +205,11 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
   own = block_sum<NT>(own, red);
   const bool use_left = rejected && left > 0.0;
   const double limit = u * (use_left ? left : own);
-  // the chunk
+  // the piece
   int64_t at = -1;
   double base = 0.0, carry = 0.0;
-  for (int64_t i0 = 0; i0 < chunks; i0 += NT) {
-    const double w = i0 + t < chunks ? (use_left ? pb[i0 + t].left : pb[i0 + t].own) : 0.0;
+  for (int64_t i0 = 0; i0 < pieces; i0 += NT) {
+    const double w = i0 + t < pieces ? (use_left ? pb[i0 + t].left : pb[i0 + t].own) : 0.0;
     double all;
     const double before = carry + block_before<NT>(w, red, all);
     const Crossing c = cross<NT>(w, before, limit, &slot);
@@ -221,12 +220,12 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
     }
     carry += all;
   }
-  if (at < 0 && carry > 0.0) {  // the last chunk with weight
-    for (int64_t i0 = (chunks - 1) / NT * NT; i0 >= 0 && at < 0; i0 -= NT) {
+  if (at < 0 && carry > 0.0) {  // the last piece with weight
+    for (int64_t i0 = (pieces - 1) / NT * NT; i0 >= 0 && at < 0; i0 -= NT) {
       __syncthreads();
       if (t == 0) last = -1;
       __syncthreads();
-      if (i0 + t < chunks && (use_left ? pb[i0 + t].left : pb[i0 + t].own) > 0.0) atomicMax(&last, t);
+      if (i0 + t < pieces && (use_left ? pb[i0 + t].left : pb[i0 + t].own) > 0.0) atomicMax(&last, t);
       __syncthreads();
       if (last >= 0) at = i0 + last;
     }
@@ -234,24 +233,26 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
   }
   int64_t token = -1;
   if (at >= 0) {
-    // a thread's 4 U neighbouring classes
-    const int64_t v0 = at * CHUNK + (int64_t)t * (4 * U);
-    float p[4 * U], q[4 * U];
-    if (v0 + 4 * U <= g.vocab) {
+    // a thread's U neighbouring classes
+    const int64_t v0 = at * (256 * U) + (int64_t)t * U;
+    float p[U], q[U];
+    if (v0 + U <= g.vocab) {
+      typedef float V __attribute__((ext_vector_type(U < 4 ? U : 4), aligned(4)));
+      constexpr int W = U < 4 ? U : 4;
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const f4 pv = *reinterpret_cast<const f4u*>(r.p + v0 + 4 * k);
-        f4 qv = {0.f, 0.f, 0.f, 0.f};
-        if (use_left && r.q) qv = *reinterpret_cast<const f4u*>(r.q + v0 + 4 * k);
+      for (int k = 0; k < U; k += W) {
+        const V pv = *reinterpret_cast<const V*>(r.p + v0 + k);
+        V qv = {};
+        if (use_left && r.q) qv = *reinterpret_cast<const V*>(r.q + v0 + k);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          p[4 * k + j] = pv[j];
-          q[4 * k + j] = qv[j];
+        for (int j = 0; j < W; ++j) {
+          p[k + j] = pv[j];
+          q[k + j] = qv[j];
         }
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4 * U; ++j) {
+      for (int j = 0; j < U; ++j) {
         p[j] = v0 + j < g.vocab ? r.p[v0 + j] : 0.f;
         q[j] = v0 + j < g.vocab && use_left && r.q ? r.q[v0 + j] : 0.f;
       }
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
     double w = 0.0;
     int mine = -1;  // this thread's last class with weight
 #pragma unroll
-    for (int j = 0; j < 4 * U; ++j) {
+    for (int j = 0; j < U; ++j) {
       const double x = weight(j);
       w += x;
       if (x > 0.0) mine = j;
@@ -282,7 +283,7 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
       double run = before;
       int hit = -1;
 #pragma unroll
-      for (int j = 0; j < 4 * U; ++j) {
+      for (int j = 0; j < U; ++j) {
         const double x = weight(j);
         run += x;
         if (hit < 0 && x > 0.0 && run > limit) hit = j;
@@ -297,9 +298,11 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
     if (i != kept) g.out[b * (g.drafts + 1) + i] = i < kept ? g.tokens[b * g.drafts + i] : -1;
 }
 
+int64_t pieces_of(int64_t vocab, int64_t u) { return ceil_div(vocab, 256 * u); }
+
 // Float4s a thread of the first launch: as many as leave two blocks a CU, so that
 // a small batch's rows are cut finer.
-int64_t chunk_units(int64_t batch, int64_t vocab) {
+int64_t piece_units(int64_t batch, int64_t vocab) {
   int64_t u = 8;
   while (u > 1 && batch * ceil_div(vocab, NT * 4 * u) < 512) u /= 2;
   return u;
@@ -317,7 +320,7 @@ int oxi_verify_drafts_workspace(int64_t batch, int64_t vocab, int64_t* bytes) {
   if (vocab > ((int64_t)1 << 30) || batch > 65535)
     return fail(OXI_INVALID_ARGUMENT, "verify_drafts_workspace: size exceeds the kernel limits");
   if (!bytes) return fail(OXI_INVALID_ARGUMENT, "verify_drafts_workspace: NULL result pointer");
-  *bytes = vocab > 0 ? batch * ceil_div(vocab, NT * 4 * chunk_units(batch, vocab)) * (int64_t)sizeof(Sums) : 0;
+  *bytes = vocab > 0 ? batch * pieces_of(vocab, piece_units(batch, vocab)) * (int64_t)sizeof(Sums) : 0;
   return OXI_OK;
 }
 
@@ -335,15 +338,15 @@ int oxi_verify_drafts(const float* target, const float* draft, const int64_t* to
     return fail(OXI_INVALID_ARGUMENT, "verify_drafts: the workspace at %p is not 8-byte aligned", workspace);
   OXI_CHECK_INIT();
   const VerifyArgs g{target, draft, tokens, lengths, uniforms, accepted, out, batch, drafts, vocab, guard_flag()};
-  const int64_t u = chunk_units(batch, vocab), chunk = NT * 4 * u, chunks = ceil_div(vocab, chunk);
-  Workspace ws(workspace ? 0 : sizeof(Sums) * (size_t)(batch * chunks));
+  const int64_t u = piece_units(batch, vocab), pieces = pieces_of(vocab, u);
+  Workspace ws(workspace ? 0 : sizeof(Sums) * (size_t)(batch * pieces));
   Sums* part = workspace ? static_cast<Sums*>(workspace) : ws.as<Sums>();
   if (!part) return fail_alloc("verify_drafts: sums");
-  const dim3 grid((unsigned)chunks, (unsigned)batch);
+  const dim3 grid((unsigned)ceil_div(pieces, NT / 64), (unsigned)batch);
 #define OXI_VER(U)                                                                            \
-  verify_sums_k<U><<<grid, dim3(NT), 0, stream()>>>(g, part);                                \
+  verify_sums_k<U><<<grid, dim3(NT), 0, stream()>>>(g, part, pieces);                                \
   if (int rc = check_launch("verify_drafts")) return rc;                                     \
-  verify_pick_k<U><<<dim3((unsigned)batch), dim3(NT), 0, stream()>>>(g, part, chunks);
+  verify_pick_k<U><<<dim3((unsigned)batch), dim3(NT), 0, stream()>>>(g, part, pieces);
   switch (u) {
     case 1: OXI_VER(1) break;
     case 2: OXI_VER(2) break;
