@@ -6,6 +6,7 @@
 // Gradients produced inside VJPs keep the common dense layout of their
 // operands (result_strides): a gradient flowing through a permuted view stays
 // permuted, so the permute VJP hands the next node a contiguous tensor.
+#include <algorithm>
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
@@ -416,6 +417,62 @@ Var rms_norm(const Var& x, const Var& w, float eps, NormVjp mode) {
   return v;
 }
 
+std::pair<Var, Var> add_rms_norm(const Var& x, const Var& r, const Var& w, float eps, NormVjp mode) {
+  const int64_t H = last_dim(x.value(), "add_rms_norm");
+  if (r.value().shape != x.value().shape) err_shape(fmt_shape(x.value().shape), fmt_shape(r.value().shape));
+  check_param(w.value(), H, "weight");
+  Tensor xc = t_contiguous(x.value());
+  Tensor rc = t_contiguous(r.value());
+  Tensor wc = t_contiguous(w.value());
+  const int64_t rows = H ? xc.numel() / H : 0;
+  Tensor h = Tensor::empty(xc.shape, Dev::Hip);
+  Tensor y = Tensor::empty(xc.shape, Dev::Hip);
+  Tensor rstd = Tensor::empty({rows}, Dev::Hip);
+  hip_check(oxi_add_rms_norm_fwd(xc.data(), rc.data(), wc.data(), h.data(), y.data(), rstd.data(), rows, H, eps));
+  Var hv = Var::op(h, "add", {x, r}, [](const Tensor& g, const std::vector<bool>& need) {
+    Grads d(2);
+    if (need[0]) d[0] = g;
+    if (need[1]) d[1] = g;
+    return d;
+  });
+  auto saved = std::make_shared<NormSaved>();
+  saved->x = h;
+  saved->w = wc;
+  saved->has_w = true;
+  saved->rstd = rstd;
+  saved->rows = rows;
+  saved->H = H;
+  saved->mode = (int)mode;
+  saved->residual = true;
+  saved->wi = 1;
+  Var yv = Var::op(y, "rms_norm", {hv, w}, [h, wc, rstd, rows, H, mode](const Tensor& g, const std::vector<bool>& need) {
+    Grads d(2);
+    if (!need[0] && !need[1]) return d;
+    Tensor gc = t_contiguous(g);
+    Tensor dx = need[0] ? Tensor::empty(h.shape, Dev::Hip) : Tensor();
+    Tensor dw = need[1] ? Tensor::empty({H}, Dev::Hip) : Tensor();
+    hip_check(oxi_add_rms_norm_bwd(h.data(), wc.data(), rstd.data(), gc.data(), nullptr, need[0] ? dx.data() : nullptr,
+                                   need[1] ? dw.data() : nullptr, nullptr, rows, H, (int)mode));
+    if (need[0]) d[0] = dx;
+    if (need[1]) d[1] = dw;
+    return d;
+  });
+  if (yv.node->op) yv.node->norm = std::move(saved);
+  return {yv, hv};
+}
+
+void add_rms_norm_vjp(const NormSaved& s, const Tensor& g, const Tensor& gh, bool need_dw, Tensor* total,
+                      Grads& grads) {
+  grads.assign(2, std::nullopt);
+  const Tensor gc = t_contiguous(g), hc = t_contiguous(gh);
+  Tensor dx = Tensor::empty(s.x.shape, Dev::Hip);
+  Tensor dw = need_dw ? Tensor::empty({s.H}, Dev::Hip) : Tensor();
+  hip_check(oxi_add_rms_norm_bwd(s.x.data(), s.w.data(), s.rstd.data(), gc.data(), hc.data(), dx.data(),
+                                 need_dw ? dw.data() : nullptr, nullptr, s.rows, s.H, s.mode));
+  *total = dx;
+  if (need_dw) grads[1] = dw;
+}
+
 Var layer_norm(const Var& x, const std::optional<Var>& w, const std::optional<Var>& b, float eps, NormVjp mode) {
   const int64_t H = last_dim(x.value(), "layer_norm");
   if (w) check_param(w->value(), H, "weight");
@@ -625,5 +682,193 @@ Var cross_entropy(const Var& logits, const std::vector<int64_t>& targets) {
                  });
 }
 
+// ---- rotary positions ---------------------------------------------------------------
+
+Var rotary(const Var& x, const RotaryFrequencies& f, const std::optional<std::vector<int64_t>>& positions,
+           int64_t offset, int layout) {
+  const Tensor& xv = x.value();
+  require_hip(xv, "rotary_embedding");
+  if (xv.ndim() != 3 && xv.ndim() != 4)
+    err_invalid("rotary_embedding expects (batch, tokens, heads, dim) or (tokens, heads, dim), got " +
+                fmt_shape(xv.shape));
+  if (2 * f.pairs > xv.shape.back())
+    err_invalid("rotary_embedding: " + std::to_string(f.pairs) + " pairs do not fit in heads of " +
+                std::to_string(xv.shape.back()));
+  const bool batched = xv.ndim() == 4;
+  const int64_t B = batched ? xv.shape[0] : 1, T = xv.shape[batched ? 1 : 0];
+  std::shared_ptr<Storage> pos;
+  Shape ps{0, 0};
+  if (positions) {
+    const int64_t n = (int64_t)positions->size();
+    if (n != T && n != B * T)
+      err_invalid("rotary_embedding: " + std::to_string(n) + " positions for " + std::to_string(B) + " x " +
+                  std::to_string(T) + " tokens");
+    pos = device_i64(*positions);
+    ps = n == B * T ? Shape{T, 1} : Shape{0, 1};
+  }
+  auto freq = f.values;
+  const int64_t rot = 2 * f.pairs;
+  const float scale = f.scale;
+  auto turn = [pos, ps, freq, rot, scale, layout, offset, batched](const Tensor& in, bool inverse) {
+    Tensor out = Tensor::empty(in.shape, Dev::Hip);
+    out.strides = result_strides(in.shape, {&in});
+    auto four = [batched](const Shape& v, int64_t first) {
+      Shape s = v;
+      if (!batched) s.insert(s.begin(), first);
+      return s;
+    };
+    const Shape shape = four(in.shape, 1), xs = four(in.strides, 0), ys = four(out.strides, 0);
+    hip_check(oxi_rotary(in.data(), xs.data(), out.data(), ys.data(), shape.data(),
+                         pos ? static_cast<const int64_t*>(pos->ptr) : nullptr, ps.data(), offset,
+                         rot ? static_cast<const double*>(freq->ptr) : nullptr, rot, layout, inverse ? 1 : 0, scale));
+    return out;
+  };
+  const Shape xshape = xv.shape;
+  return Var::op(turn(xv, false), "rotary_embedding", {x},
+                 [turn, xshape](const Tensor& g, const std::vector<bool>& need) -> Grads {
+                   if (!need[0]) return {std::nullopt};
+                   return {turn(g.shape == xshape ? g : t_broadcast_to(g, xshape), true)};
+                 });
+}
+
+// ---- distillation ---------------------------------------------------------------------
+
+Var distillation_loss(const Var& logits, const std::vector<int64_t>& ids, const Tensor& top,
+                      const std::optional<Tensor>& top_lse, float temperature, float divisor) {
+  const Tensor& lv = logits.value();
+  if (lv.ndim() != 2) err_invalid("distillation_loss expects (batch, classes) logits, got " + fmt_shape(lv.shape));
+  const int64_t n = lv.shape[0], c = lv.shape[1];
+  if (top.ndim() != 2 || top.shape[0] != n) err_shape(fmt_shape(lv.shape), fmt_shape(top.shape));
+  const int64_t k = top.shape[1];
+  if ((int64_t)ids.size() != n * k)
+    err_invalid(std::to_string(ids.size()) + " teacher ids for logits of shape " + fmt_shape(top.shape));
+  if (top_lse && top_lse->shape != Shape{n}) err_shape(fmt_shape({n}), fmt_shape(top_lse->shape));
+  for (int64_t i : ids)
+    if (i >= c)
+      err_oob("index " + std::to_string(i) + " is out of bounds for axis 1 with size " + std::to_string(c));
+  require_hip(lv, "distillation_loss");
+  require_hip(top, "distillation_loss");
+  if (top_lse) require_hip(*top_lse, "distillation_loss");
+  Tensor lc = t_contiguous(lv), tc = t_contiguous(top);
+  std::optional<Tensor> ec;
+  if (top_lse) ec = t_contiguous(*top_lse);
+  auto id = device_i64(ids);
+  Tensor loss = Tensor::empty({}, Dev::Hip), row = Tensor::empty({n}, Dev::Hip), lse = Tensor::empty({n}, Dev::Hip),
+         rest = Tensor::empty({n}, Dev::Hip);
+  // With a gradient to come, the forward pass also forms the gradient for
+  // loss.backward()'s seed, as cross_entropy does (and the same switch turns off).
+  std::optional<Tensor> unit;
+  if (logits.requires_grad() && is_grad_enabled() && ce_one_pass()) unit = Tensor::empty({n, c}, Dev::Hip);
+  const int64_t* ip = static_cast<const int64_t*>(id->ptr);
+  hip_check(oxi_distill_fwd(lc.data(), ip, tc.data(), ec ? ec->data() : nullptr, loss.data(), row.data(), lse.data(),
+                            rest.data(), unit ? unit->data() : nullptr, n, c, k, temperature, divisor));
+  auto fresh = std::make_shared<std::atomic<bool>>(unit.has_value());
+  return Var::op(loss, "distillation_loss", {logits},
+                 [lc, tc, ec, id, lse, rest, n, c, k, temperature, divisor, unit, fresh](
+                     const Tensor& g, const std::vector<bool>& need) -> Grads {
+                   if (!need[0]) return {std::nullopt};
+                   if (is_implicit_seed(g) && fresh->exchange(false)) return {*unit};
+                   Tensor gs = t_contiguous(g);
+                   Tensor d = Tensor::empty({n, c}, Dev::Hip);
+                   hip_check(oxi_distill_bwd(lc.data(), static_cast<const int64_t*>(id->ptr), tc.data(),
+                                             ec ? ec->data() : nullptr, lse.data(), rest.data(), gs.data(), d.data(), n, c,
+                                             k, temperature, divisor));
+                   return {d};
+                 });
+}
+
 }  // namespace aops
+
+RotaryFrequencies::RotaryFrequencies(const std::vector<double>& inv_freq, float s)
+    : pairs((int64_t)inv_freq.size()), scale(s) {
+  if (inv_freq.empty()) return;
+  values = std::make_shared<Storage>(Dev::Hip, sizeof(double) * inv_freq.size());
+  hip_check(oxi_hip_upload(values->ptr, inv_freq.data(), sizeof(double) * inv_freq.size()));
+}
+
+// ---- serving ------------------------------------------------------------------------------
+
+E4m3Rows t_add_rms_norm_e4m3(const Tensor& x, const std::optional<Tensor>& r, const Tensor& w, float eps,
+                             int64_t group, Tensor* h) {
+  require_hip(x, "add_rms_norm_e4m3");
+  if (x.ndim() == 0) err_invalid("add_rms_norm_e4m3 needs at least one dim");
+  const int64_t H = x.shape.back();
+  if (r && r->shape != x.shape) err_shape(fmt_shape(x.shape), fmt_shape(r->shape));
+  if (w.ndim() != 1 || w.shape[0] != H) err_shape(fmt_shape(w.shape), fmt_shape({H}));
+  if (group < 1) err_invalid("add_rms_norm_e4m3: groups of " + std::to_string(group) + " columns");
+  const Tensor xc = t_contiguous(x), wc = t_contiguous(w);
+  Tensor rc;
+  if (r) {
+    rc = t_contiguous(*r);
+    *h = Tensor::empty(x.shape, Dev::Hip);
+  }
+  E4m3Rows q;
+  q.shape = x.shape;
+  q.group = group;
+  const int64_t rows = H ? xc.numel() / H : 0;
+  Shape ss = x.shape;
+  ss.back() = (H + group - 1) / group;
+  q.scale = Tensor::empty(ss, Dev::Hip);
+  q.codes = std::make_shared<Storage>(Dev::Hip, (size_t)xc.numel());
+  hip_check(oxi_add_rms_norm_e4m3_fwd(xc.data(), r ? rc.data() : nullptr, wc.data(), r ? h->data() : nullptr,
+                                      static_cast<uint8_t*>(q.codes->ptr), q.scale.data(), rows, H, group, eps));
+  return q;
+}
+
+Tensor t_dequantize(const E4m3Rows& q) {
+  Tensor y = Tensor::empty(q.shape, Dev::Hip);
+  const int64_t H = q.shape.back();
+  hip_check(oxi_e4m3_dequantize(static_cast<const uint8_t*>(q.codes->ptr), q.scale.data(), y.data(),
+                                H ? y.numel() / H : 0, H, q.group));
+  return y;
+}
+
+std::pair<std::vector<int64_t>, std::vector<int64_t>> t_verify_drafts(
+    const Tensor& target, const std::optional<Tensor>& draft, const std::vector<int64_t>& tokens,
+    const std::optional<std::vector<int64_t>>& lengths, const Tensor& uniforms) {
+  if (target.ndim() != 3)
+    err_invalid("verify_drafts expects (batch, drafts + 1, classes) probabilities, got " + fmt_shape(target.shape));
+  const int64_t b = target.shape[0], rows = target.shape[1], v = target.shape[2];
+  if (rows < 1) err_invalid("verify_drafts: no row of target probabilities");
+  const int64_t k = rows - 1;
+  if (draft && draft->shape != Shape{b, k, v}) err_shape(fmt_shape(draft->shape), fmt_shape({b, k, v}));
+  if (uniforms.shape != Shape{b, rows}) err_shape(fmt_shape(uniforms.shape), fmt_shape({b, rows}));
+  if ((int64_t)tokens.size() != b * k)
+    err_invalid(std::to_string(tokens.size()) + " drafted tokens for " + std::to_string(b) + " x " +
+                std::to_string(k) + " drafts");
+  if (lengths && (int64_t)lengths->size() != b)
+    err_invalid(std::to_string(lengths->size()) + " lengths for batch of " + std::to_string(b));
+  if (lengths)
+    for (int64_t n : *lengths)
+      if (n < 0 || n > k)
+        err_invalid("verify_drafts: a length of " + std::to_string(n) + " of " + std::to_string(k) + " drafts");
+  for (int64_t s = 0; s < b; ++s)
+    for (int64_t i = 0; i < (lengths ? (*lengths)[(size_t)s] : k); ++i) {
+      const int64_t x = tokens[(size_t)(s * k + i)];
+      if (x < 0 || x >= v)
+        err_oob("index " + std::to_string(x) + " is out of bounds for axis 2 with size " + std::to_string(v));
+    }
+  require_hip(target, "verify_drafts");
+  if (draft) require_hip(*draft, "verify_drafts");
+  require_hip(uniforms, "verify_drafts");
+  const Tensor tc = t_contiguous(target), uc = t_contiguous(uniforms);
+  Tensor dc;
+  if (draft) dc = t_contiguous(*draft);
+  std::vector<int64_t> accepted((size_t)b), out((size_t)(b * rows));
+  if (b == 0) return {accepted, out};
+  auto td = device_i64(tokens);
+  std::shared_ptr<Storage> ld;
+  if (lengths) ld = device_i64(*lengths);
+  // one buffer, and one copy to the host
+  Storage res(Dev::Hip, sizeof(int64_t) * (size_t)(b + b * rows));
+  int64_t* rp = static_cast<int64_t*>(res.ptr);
+  hip_check(oxi_verify_drafts(tc.data(), draft ? dc.data() : nullptr, static_cast<const int64_t*>(td->ptr),
+                              ld ? static_cast<const int64_t*>(ld->ptr) : nullptr, uc.data(), rp, rp + b, nullptr, b, k, v));
+  std::vector<int64_t> all((size_t)(b + b * rows));
+  hip_check(oxi_hip_memcpy_d2h(all.data(), res.ptr, sizeof(int64_t) * all.size()));
+  std::copy(all.begin(), all.begin() + b, accepted.begin());
+  std::copy(all.begin() + b, all.end(), out.begin());
+  return {accepted, out};
+}
+
 }  // namespace oxt

@@ -610,6 +610,86 @@ PYBIND11_MODULE(_native, m) {
     return PyTensor(aops::embedding(int_ids(indices), w.v));
   });
 
+  m.def(
+      "add_rms_norm",
+      [](const PyTensor& x, const PyTensor& r, const PyTensor& w, float eps, const py::object& mode) {
+        aops::NormVjp md = mode.is_none() ? aops::norm_vjp_mode()
+                                          : (mode.cast<std::string>() == "exact" ? aops::NormVjp::Exact : aops::NormVjp::Ref);
+        auto [y, h] = aops::add_rms_norm(x.v, r.v, w.v, eps, md);
+        return py::make_tuple(PyTensor(y), PyTensor(h));
+      },
+      py::arg("x"), py::arg("residual"), py::arg("weight"), py::arg("eps") = 1e-6f, py::arg("vjp") = py::none());
+
+  py::class_<E4m3Rows>(m, "E4m3Rows", "Rows in 8-bit floating point (OCP e4m3) with a scale per group of columns.")
+      .def_property_readonly("shape", [](const E4m3Rows& q) { return q.shape; })
+      .def_property_readonly("group", [](const E4m3Rows& q) { return q.group; })
+      .def_property_readonly("scale", [](const E4m3Rows& q) { return leaf(q.scale); })
+      .def("codes",
+           [](const E4m3Rows& q) {
+             std::vector<py::ssize_t> shape(q.shape.begin(), q.shape.end());
+             py::array_t<uint8_t> a(shape);
+             if (a.nbytes()) hip_check(oxi_hip_memcpy_d2h(a.mutable_data(), q.codes->ptr, (size_t)a.nbytes()));
+             return a;
+           })
+      .def("dequantize", [](const E4m3Rows& q) { return leaf(t_dequantize(q)); });
+  m.def(
+      "add_rms_norm_e4m3",
+      [](const PyTensor& x, const py::object& r, const PyTensor& w, float eps, int64_t group) {
+        std::optional<Tensor> rv;
+        if (!r.is_none()) rv = r.cast<PyTensor&>().value();
+        Tensor h;
+        E4m3Rows q = t_add_rms_norm_e4m3(x.value(), rv, w.value(), eps, group, &h);
+        return py::make_tuple(std::move(q), rv ? py::cast(leaf(h)) : py::none());
+      },
+      py::arg("x"), py::arg("residual"), py::arg("weight"), py::arg("eps") = 1e-6f, py::arg("group") = 128);
+
+  py::class_<RotaryFrequencies>(m, "RotaryFrequencies", "Angles per position of the rotated pairs, kept on the device.")
+      .def(py::init<const std::vector<double>&, float>(), py::arg("inv_freq"), py::arg("scale") = 1.0f)
+      .def_readonly("pairs", &RotaryFrequencies::pairs)
+      .def_readonly("scale", &RotaryFrequencies::scale);
+  m.def(
+      "rotary_embedding",
+      [](const PyTensor& x, const RotaryFrequencies& f, const py::object& positions, int64_t offset,
+         const std::string& layout) {
+        int l;
+        if (layout == "half") l = OXI_ROTARY_HALF;
+        else if (layout == "interleaved") l = OXI_ROTARY_INTERLEAVED;
+        else err_invalid("rotary layout must be \"half\" or \"interleaved\", got \"" + layout + "\"");
+        std::optional<std::vector<int64_t>> pos;
+        if (!positions.is_none()) pos = int_ids(positions);
+        return PyTensor(aops::rotary(x.v, f, pos, offset, l));
+      },
+      py::arg("x"), py::arg("frequencies"), py::arg("positions") = py::none(), py::arg("offset") = 0,
+      py::arg("layout") = "half");
+
+  m.def(
+      "distillation_loss",
+      [](const PyTensor& logits, const py::object& ids, const PyTensor& top, const py::object& lse, float temperature,
+         float divisor) {
+        std::optional<Tensor> l;
+        if (!lse.is_none()) l = lse.cast<PyTensor&>().value();
+        return PyTensor(aops::distillation_loss(logits.v, int_ids(ids), top.value(), l, temperature, divisor));
+      },
+      py::arg("logits"), py::arg("teacher_ids"), py::arg("teacher_logits"), py::arg("teacher_lse"),
+      py::arg("temperature"), py::arg("divisor"));
+
+  m.def(
+      "verify_drafts",
+      [](const py::object& tokens, const py::object& draft, const PyTensor& target, const PyTensor& uniforms,
+         const py::object& lengths) {
+        std::optional<Tensor> d;
+        if (!draft.is_none()) d = draft.cast<PyTensor&>().value();
+        std::optional<std::vector<int64_t>> n;
+        if (!lengths.is_none()) n = int_ids(lengths);
+        auto [accepted, out] = t_verify_drafts(target.value(), d, int_ids(tokens), n, uniforms.value());
+        const py::ssize_t b = target.value().shape[0], rows = target.value().shape[1];
+        py::array_t<int64_t> a(std::vector<py::ssize_t>{b}), o(std::vector<py::ssize_t>{b, rows});
+        std::copy(accepted.begin(), accepted.end(), a.mutable_data());
+        std::copy(out.begin(), out.end(), o.mutable_data());
+        return py::make_tuple(a, o);
+      },
+      py::arg("tokens"), py::arg("draft_probs"), py::arg("target_probs"), py::arg("uniforms"), py::arg("lengths"));
+
   // Elementwise clamp on the device (binary max then min against scalar
   // constants), for gradient-value clipping; detached.
   m.def("clamp", [](const PyTensor& x, float lo, float hi) {

@@ -261,7 +261,11 @@ std::vector<std::optional<Tensor>> add_grads(const LeadSum& ls, const std::optio
 //   the permute's), so reading it gives the node-by-node values;
 // - when the norm's input is r = p + q with q broadcast over the leading dim
 //   (a positional table) and r feeds nothing else, the norm pass also forms
-//   q's gradient (oxi_*_norm_bwd_lead_sum), held for the add node.
+//   q's gradient (oxi_*_norm_bwd_lead_sum), held for the add node;
+// - when the norm's input is a residual sum (add_rms_norm) that already has a
+//   gradient from its other uses, the norm pass adds its own to it
+//   (oxi_add_rms_norm_bwd): the sum that accumulation would form, in the same
+//   order.
 namespace {
 thread_local const Storage* t_implicit_seed = nullptr;
 
@@ -381,6 +385,16 @@ void backward(const Var& root, std::optional<Tensor> seed, bool retain_graph) {
           held[ls.add] = add_grads(ls, grads[0], dsum);
           done = true;
           g_fused_passes.fetch_add(1);
+        } else if (n.node->norm->residual && needs[0]) {
+          // the residual stream's gradient so far joins the norm's in one pass
+          Node* h = n.node->inputs[0].node.get();
+          if (const std::optional<Tensor> gh = read_grad(*h)) {
+            Tensor total;
+            aops::add_rms_norm_vjp(*n.node->norm, *up, *gh, needs[1], &total, grads);
+            std::lock_guard<std::mutex> lk(h->mu);
+            h->grad = total;
+            done = true;
+          }
         }
       }
       if (!done) grads = f(*up, needs);

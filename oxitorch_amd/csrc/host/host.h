@@ -180,6 +180,7 @@ struct NormSaved {
   bool has_w = false, has_b = false;
   int64_t rows = 0, H = 0;
   int mode = 0;         // OXI_NORM_VJP_*
+  bool residual = false;  // x is a residual sum formed by add_rms_norm
   int wi = -1, bi = -1;  // input slots of w and b, -1 when absent
 };
 
@@ -247,6 +248,15 @@ uint64_t fused_norm_act_passes();  // fused passes run so far in this process
 
 // ---- differentiable ops (crates/oxi-autograd/src/ops.rs) ------------------------
 
+// Angles per position of the rotated pairs, in 64 bits on the device, and the
+// factor on what they turn.
+struct RotaryFrequencies {
+  std::shared_ptr<Storage> values;
+  int64_t pairs = 0;
+  float scale = 1.f;
+  RotaryFrequencies(const std::vector<double>& inv_freq, float scale);
+};
+
 namespace aops {
 Var add(const Var& a, const Var& b);
 Var sub(const Var& a, const Var& b);
@@ -287,13 +297,46 @@ NormVjp norm_vjp_mode();  // OXI_NORM_VJP=ref|exact (default ref)
 bool norm_vjp_fused(const NormSaved& s, int act, const Tensor& g, const std::vector<bool>& need, Tensor* dy,
                     std::vector<std::optional<Tensor>>& grads, int64_t lead = 0, Tensor* lsum = nullptr);
 Var rms_norm(const Var& x, const Var& w, float eps, NormVjp mode);
+// (y, h): h = x + r and y = rms_norm(h), one forward kernel; x, r of one shape.
+// In backward, a gradient that h already has joins the norm's VJP in its kernel.
+std::pair<Var, Var> add_rms_norm(const Var& x, const Var& r, const Var& w, float eps, NormVjp mode);
+// Its VJP for upstream g of y with h's gradient so far: *total receives their
+// sum, grads[1] w's gradient if asked for.
+void add_rms_norm_vjp(const NormSaved& s, const Tensor& g, const Tensor& gh, bool need_dw, Tensor* total,
+                      std::vector<std::optional<Tensor>>& grads);
 Var layer_norm(const Var& x, const std::optional<Var>& w, const std::optional<Var>& b, float eps, NormVjp mode);
 Var gelu(const Var& x, int approximate);
 Var silu(const Var& x);
 Var softmax(const Var& x, int64_t dim, bool log);
 Var cross_entropy(const Var& logits, const std::vector<int64_t>& targets);
 Var embedding(const std::vector<int64_t>& indices, const Var& weight);
+// x (batch, tokens, heads, dim) or (tokens, heads, dim) with its pairs turned;
+// positions: one per token, one per batch and token, or none (0, 1, ..).
+Var rotary(const Var& x, const RotaryFrequencies& f, const std::optional<std::vector<int64_t>>& positions,
+           int64_t offset, int layout);
+// The distillation loss of logits (n, c) against the teacher's ids and logits (n,
+// k each), and its log-sum-exp (n) if given; the sum over the rows / divisor.
+Var distillation_loss(const Var& logits, const std::vector<int64_t>& ids, const Tensor& top,
+                      const std::optional<Tensor>& top_lse, float temperature, float divisor);
 }  // namespace aops
+
+// ---- serving: no gradients -----------------------------------------------------------
+
+// Rows in 8-bit floating point: e4m3 codes and a scale per `group` columns.
+struct E4m3Rows {
+  std::shared_ptr<Storage> codes;
+  Tensor scale;
+  Shape shape;
+  int64_t group = 0;
+};
+// add_rms_norm with y in 8 bits; without r (unset) the norm of x alone, *h untouched.
+E4m3Rows t_add_rms_norm_e4m3(const Tensor& x, const std::optional<Tensor>& r, const Tensor& w, float eps,
+                             int64_t group, Tensor* h);
+Tensor t_dequantize(const E4m3Rows& q);
+// accepted (batch) and tokens (batch, drafts + 1), on the host (waits for the device).
+std::pair<std::vector<int64_t>, std::vector<int64_t>> t_verify_drafts(
+    const Tensor& target, const std::optional<Tensor>& draft, const std::vector<int64_t>& tokens,
+    const std::optional<std::vector<int64_t>>& lengths, const Tensor& uniforms);
 
 // ---- optimizers (crates/oxi-autograd/src/optim.rs) ------------------------------
 // All state (velocities, moments, per-parameter step counters) lives here as

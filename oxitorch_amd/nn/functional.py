@@ -69,6 +69,14 @@ def log_softmax(x, dim=-1):
 
 # ---- normalization (functional.py:227-240) ----------------------------------------
 
+def _flat_ints(values, what):
+    """A flat int64 array of `values` (numbers in any nesting), refusing what is not an integer."""
+    a = np.asarray(values)
+    if a.size and a.dtype.kind not in "iu":
+        raise TypeError(f"{what} must be integers, got {a.dtype}")
+    return a.astype(np.int64).ravel()
+
+
 def _is_vec(t, H):
     return t is not None and len(t.shape) == 1 and t.shape[0] == H
 
@@ -102,6 +110,98 @@ def rms_norm(x, weight, eps=1e-6, vjp=None):
     ms = (x * x).mean(-1, True)
     inv = (ms + float(eps)).apply("rsqrt")
     return x * inv * weight
+
+
+def add_rms_norm(x, residual, weight, eps=1e-6, vjp=None):
+    """The residual stream's step of a pre-norm layer: h = x + residual and
+    y = rms_norm(h, weight, eps) in one pass. Returns (y, h): y goes into the
+    layer, h on along the stream. `vjp` as in layer_norm.
+
+    In backward, the gradient that h has from its later uses joins the norm's
+    in one pass (OXI_FUSE_NORM_ACT=0 runs the add by itself)."""
+    if list(residual.shape) == list(x.shape) and _is_vec(weight, x.shape[-1]):
+        return _native.add_rms_norm(x, residual, weight, eps, vjp)
+    h = x + residual
+    return rms_norm(h, weight, eps, vjp), h
+
+
+def add_rms_norm_e4m3(x, residual, weight, eps=1e-6, group=128):
+    """add_rms_norm for serving, with y in 8-bit floating point (OCP e4m3) and a
+    scale for each `group` columns of a row (32, 64, 128, 256 or the row's
+    length): max|y|/448 of the group. Returns (q, h); q holds `codes()` (numpy
+    uint8), `scale` and `dequantize()`, and carries no gradient. `residual` None:
+    the norm of x alone, and h is None."""
+    return _native.add_rms_norm_e4m3(x, residual, weight, eps, group)
+
+
+# ---- rotary positions -----------------------------------------------------------------
+
+def rotary_frequencies(dim, base=10000.0, scaling=None):
+    """(inv_freq, scale): the angle per position of each of the dim/2 pairs,
+    base**(-2i/dim), as float64, and the factor on what they turn.
+
+    `scaling` stretches them for contexts longer than the trained one:
+    {"type": "linear", "factor": s} divides all of them by s;
+    {"type": "ntk", "factor": s} raises the base to base * s**(dim/(dim-2)), so
+    that the slowest pair is divided by s and the fastest is kept;
+    {"type": "yarn", "factor": s, "original_length": L} divides the pairs that
+    turn less than `slow` (1) times within L positions by s, keeps those that
+    turn more than `fast` (32) times, and blends in between; its scale is
+    0.1 ln(s) + 1 ("scale" overrides)."""
+    dim = int(dim)
+    if dim < 0 or dim % 2:
+        raise ValueError(f"rotary positions turn pairs: {dim} elements is not an even number")
+    base = float(base)
+    if not base > 0 or np.isinf(base):
+        raise ValueError(f"the rotary base must be positive, got {base}")
+    half = dim // 2
+    exponent = -np.arange(half, dtype=np.float64) / max(half, 1)
+    inv = base ** exponent
+    if scaling is None:
+        return inv, 1.0
+    kind, s = scaling.get("type"), float(scaling.get("factor", 1.0))
+    if not s > 0 or np.isinf(s):
+        raise ValueError(f"the rotary scaling factor must be positive, got {s}")
+    if kind == "linear":
+        return inv / s, 1.0
+    if kind == "ntk":
+        if dim <= 2:
+            return inv, 1.0
+        return (base * s ** (dim / (dim - 2))) ** exponent, 1.0
+    if kind == "yarn":
+        length = float(scaling["original_length"])
+        slow, fast = float(scaling.get("slow", 1.0)), float(scaling.get("fast", 32.0))
+        if not fast > slow:
+            raise ValueError(f"rotary scaling: fast ({fast}) must be above slow ({slow})")
+        keep = np.clip((length * inv / (2 * np.pi) - slow) / (fast - slow), 0.0, 1.0)
+        scale = scaling.get("scale", 0.1 * np.log(s) + 1.0 if s > 1 else 1.0)
+        return (1 - keep) * inv / s + keep * inv, float(scale)
+    raise ValueError(f"unknown rotary scaling {kind!r}: linear, ntk or yarn")
+
+
+def _frequencies(f):
+    if isinstance(f, _native.RotaryFrequencies):
+        return f
+    inv, scale = f if isinstance(f, tuple) else (f, 1.0)
+    return _native.RotaryFrequencies([float(v) for v in np.asarray(inv, dtype=np.float64).ravel()], scale)
+
+
+def rotary_embedding(x, frequencies, positions=None, offset=0, layout="half"):
+    """x (batch, tokens, heads, dim) or (tokens, heads, dim) with the pairs of
+    each head's first elements turned by position * frequency: (u, v) to
+    scale * (u cos a - v sin a, v cos a + u sin a); elements past the pairs are
+    copied. Pair i is elements (i, i + pairs) in the "half" layout,
+    (2i, 2i + 1) in the "interleaved" one.
+
+    `frequencies`: what rotary_frequencies returns, an array of angles per
+    position, or a _native.RotaryFrequencies that holds them on the device (as
+    nn.RotaryEmbedding keeps one). `positions`: integers, one per token or one
+    per batch and token; None counts from 0. `offset` is added to them. Angles
+    are formed in 64 bits. x may be any view (heads before tokens, a slice of a
+    fused projection); one call serves query and key heads side by side."""
+    if positions is not None:
+        positions = _flat_ints(positions, "positions")
+    return _native.rotary_embedding(x, _frequencies(frequencies), positions, int(offset), layout)
 
 
 # ---- embedding (functional.py:245-247) -----------------------------------------------
@@ -149,6 +249,70 @@ def cross_entropy(logits, targets):
         raise IndexError(f"index {int(t[bad][0])} is out of bounds for axis 1 with size {classes}")
     t = np.where(t < 0, t + classes, t)
     return _native.cross_entropy(logits, t)
+
+
+def _device_values(v):
+    """A tensor as it is, anything else as a float32 tensor on the default device."""
+    return v if isinstance(v, _native.Tensor) else _native_from_numpy(np.asarray(v, dtype=np.float32))
+
+
+def distillation_loss(logits, teacher_ids, teacher_logits, temperature=1.0, teacher_lse=None):
+    """How far a student's distribution q = softmax(logits/T) is from a
+    teacher's that is known by its k best entries a row: T^2 times the mean over
+    the rows of sum p (log p - log q[id]).
+
+    `teacher_ids` (batch, k): the entries' classes as integers; a negative one is
+    padding, and rows of padding alone count neither in the sum nor in the mean
+    (padded tokens). `teacher_logits` (batch, k): the teacher's logits there, a
+    tensor or an array; no gradient goes to them. p is their softmax at
+    temperature T over the row's entries; with `teacher_lse` (batch: the
+    log-sum-exp of all of the teacher's logits/T) p are the teacher's own
+    probabilities, and what they leave to the other classes is compared with
+    what the student leaves there.
+
+    Fused as cross_entropy is: one pass over the logits writes the loss and the
+    gradient for backward()'s implicit seed."""
+    n, classes = logits.shape
+    ids = np.asarray(teacher_ids)
+    if ids.ndim != 2 or ids.shape[0] != n:
+        raise ValueError(f"teacher_ids of shape {list(ids.shape)} for a batch of {n}: (batch, k) is expected")
+    flat = _flat_ints(ids, "teacher_ids")
+    if flat.size and flat.max() >= classes:
+        raise IndexError(f"index {int(flat.max())} is out of bounds for axis 1 with size {classes}")
+    top = _device_values(teacher_logits)
+    if list(top.shape) != list(ids.shape):
+        raise ValueError(f"teacher_logits of shape {list(top.shape)} for teacher_ids of shape {list(ids.shape)}")
+    lse = None if teacher_lse is None else _device_values(teacher_lse)
+    rows = int((flat.reshape(ids.shape) >= 0).any(axis=1).sum())
+    return _native.distillation_loss(logits, flat, top, lse, float(temperature), float(max(rows, 1)))
+
+
+# ---- serving: drafted tokens ------------------------------------------------------------
+
+def verify_drafts(draft_tokens, draft_probs, target_probs, uniforms, lengths=None):
+    """Which of the tokens that a small model drafted are kept, so that what is
+    kept is distributed as the large model's own samples.
+
+    `draft_tokens` (batch, k) integers; `draft_probs` (batch, k, classes): what
+    each was drawn from, or None for drafts without probabilities (a lookup, a
+    greedy model); `target_probs` (batch, k + 1, classes): the large model's,
+    after 0, 1, .. k of them; `uniforms` (batch, k + 1) in [0, 1), a tensor or an
+    array; `lengths` (batch): how many tokens were drafted, None for k.
+
+    Draft i is kept while uniforms[i] * draft_probs[i][token] <
+    target_probs[i][token]; after the first that is not, one token is drawn from
+    max(target - draft, 0) by uniforms[k], after all of them from the target's
+    next row. Returns numpy int64 arrays (accepted (batch,), tokens (batch,
+    k + 1)): the kept tokens, the drawn one, then -1. Waits for the device."""
+    tokens = np.asarray(draft_tokens)
+    b, rows, classes = target_probs.shape
+    if tokens.shape != (b, rows - 1):
+        raise ValueError(f"draft_tokens of shape {list(tokens.shape)} for target_probs of shape "
+                         f"{list(target_probs.shape)}: {[b, rows - 1]} is expected")
+    flat = _flat_ints(tokens, "draft_tokens")
+    if lengths is not None:
+        lengths = _flat_ints(lengths, "lengths")
+    return _native.verify_drafts(flat, draft_probs, target_probs, _device_values(uniforms), lengths)
 
 
 def _outside(what):

@@ -34,6 +34,33 @@ class RMSNorm(Module):
         return F.rms_norm(x, self.weight.tensor, self.eps)
 
 
+class AddRMSNorm(Module):
+    """F.add_rms_norm with its own weight (ones) of `normalized_shape`: called
+    with (x, residual), returns (y, h); `seed` as in LayerNorm."""
+
+    def __init__(self, normalized_shape, eps=1e-6, seed=None):
+        self.eps = eps
+        self.weight = Parameter(F._native_from_numpy(np.ones(normalized_shape, dtype=np.float32), True))
+
+    def forward(self, x, residual):
+        return F.add_rms_norm(x, residual, self.weight.tensor, self.eps)
+
+
+class RotaryEmbedding(Module):
+    """F.rotary_embedding with the frequencies of `dim` turning elements kept on
+    the device (no parameters); `base` and `scaling` as rotary_frequencies takes
+    them. Called with x and, optionally, positions and an offset."""
+
+    def __init__(self, dim, base=10000.0, scaling=None, layout="half"):
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"rotary layout must be \"half\" or \"interleaved\", got {layout!r}")
+        self.layout = layout
+        self.frequencies = F._frequencies(F.rotary_frequencies(dim, base, scaling))
+
+    def forward(self, x, positions=None, offset=0):
+        return F.rotary_embedding(x, self.frequencies, positions, offset, self.layout)
+
+
 class Embedding(Module):
     """F.embedding over its own (num_embeddings, embedding_dim) table, drawn
     as standard normals * 0.05 from default_rng(seed); forward takes a flat

@@ -138,3 +138,78 @@ def test_verify(capi):
     with pytest.raises(ValueError, match="NULL result"):
         capi.call("oxi_verify_drafts_workspace", 2, 50, None)
     assert capi.verify_drafts_workspace(0, 50) == 0
+
+
+# ---- the Python surface, on host tensors ----------------------------------------------
+
+def test_rotary_frequencies():
+    from oxitorch_amd.nn import functional as F
+
+    inv, scale = F.rotary_frequencies(64)
+    assert scale == 1.0 and inv.dtype == np.float64
+    assert np.allclose(inv, [10000.0 ** (-2 * i / 64) for i in range(32)], rtol=1e-15)
+    lin, _ = F.rotary_frequencies(64, scaling={"type": "linear", "factor": 8})
+    assert np.array_equal(lin, inv / 8)
+    # the slowest pair is divided by the factor, the fastest kept
+    ntk, _ = F.rotary_frequencies(64, scaling={"type": "ntk", "factor": 8.0})
+    assert ntk[0] == 1.0 and np.isclose(ntk[-1], inv[-1] / 8, rtol=1e-12)
+    assert (ntk <= inv).all() and (ntk >= inv / 8 * (1 - 1e-12)).all()
+    yarn, m = F.rotary_frequencies(64, scaling={"type": "yarn", "factor": 8.0, "original_length": 4096})
+    turns = 4096 * inv / (2 * np.pi)
+    assert np.allclose(yarn[turns >= 32], inv[turns >= 32]) and np.allclose(yarn[turns <= 1], inv[turns <= 1] / 8)
+    mid = (turns > 1) & (turns < 32)
+    assert mid.any() and (yarn[mid] < inv[mid]).all() and (yarn[mid] > inv[mid] / 8).all()
+    assert np.isclose(m, 0.1 * np.log(8) + 1)
+    assert F.rotary_frequencies(64, scaling={"type": "yarn", "factor": 8.0, "original_length": 4096, "scale": 1.0})[1] == 1.0
+    assert F.rotary_frequencies(2, scaling={"type": "ntk", "factor": 8.0})[0].tolist() == [1.0]
+    assert F.rotary_frequencies(0)[0].size == 0
+
+
+def test_python_refusals():
+    import oxitorch_amd as ox
+    from oxitorch_amd import nn
+    from oxitorch_amd.nn import functional as F
+
+    for dim in (3, -2):
+        with pytest.raises(ValueError, match="even number"):
+            F.rotary_frequencies(dim)
+    for base in (0, -1, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="base"):
+            F.rotary_frequencies(8, base)
+    for kw in ({"type": "linear", "factor": 0}, {"type": "ntk", "factor": -1}):
+        with pytest.raises(ValueError, match="factor"):
+            F.rotary_frequencies(8, scaling=kw)
+    with pytest.raises(ValueError, match="unknown rotary scaling"):
+        F.rotary_frequencies(8, scaling={"type": "cubic", "factor": 2})
+    with pytest.raises(ValueError, match="above slow"):
+        F.rotary_frequencies(8, scaling={"type": "yarn", "factor": 2, "original_length": 64, "slow": 4, "fast": 2})
+    with pytest.raises(KeyError):
+        F.rotary_frequencies(8, scaling={"type": "yarn", "factor": 2})
+    with pytest.raises(ValueError, match="layout"):
+        nn.RotaryEmbedding(8, layout="both")
+    cpu = lambda *s: ox.from_numpy(np.zeros(s, np.float32), device="cpu")  # noqa: E731
+    ids = np.zeros((3, 2), np.int64)
+    with pytest.raises(ValueError, match="teacher_ids"):
+        F.distillation_loss(cpu(3, 8), ids[0], cpu(3, 2))
+    with pytest.raises(IndexError, match="index 8 is out of bounds"):
+        F.distillation_loss(cpu(3, 8), ids + 8, cpu(3, 2))
+    with pytest.raises(TypeError, match="integers"):
+        F.distillation_loss(cpu(3, 8), ids * 1.0, cpu(3, 2))
+    with pytest.raises(ValueError, match="teacher_logits"):
+        F.distillation_loss(cpu(3, 8), ids, cpu(3, 3))
+    with pytest.raises(NotImplementedError):  # host tensors do not reach device compute
+        F.distillation_loss(cpu(3, 8), ids, cpu(3, 2))
+    with pytest.raises(ValueError, match="draft_tokens"):
+        F.verify_drafts(ids, None, cpu(3, 2, 8), cpu(3, 2))
+    with pytest.raises(TypeError, match="integers"):
+        F.verify_drafts(ids * 1.0, None, cpu(3, 3, 8), cpu(3, 3))
+    with pytest.raises(ValueError, match="shape mismatch"):
+        F.verify_drafts(ids, None, cpu(3, 3, 8), cpu(3, 2))
+    with pytest.raises(ValueError, match="a length of 3 of 2"):
+        F.verify_drafts(ids, None, cpu(3, 3, 8), cpu(3, 3), [0, 3, 0])
+    with pytest.raises(ValueError, match="2 lengths for batch of 3"):
+        F.verify_drafts(ids, None, cpu(3, 3, 8), cpu(3, 3), [0, 1])
+    with pytest.raises(RuntimeError, match="index 8 is out of bounds"):
+        F.verify_drafts(ids + 8, None, cpu(3, 3, 8), cpu(3, 3))
+    with pytest.raises(NotImplementedError):
+        F.verify_drafts(ids, None, cpu(3, 3, 8), cpu(3, 3))
