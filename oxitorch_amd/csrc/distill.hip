@@ -239,6 +239,14 @@ __device__ __forceinline__ double rest_term(double psum, double lr, double qr) {
   return (pr > 0.0 || pr != pr ? pr * exp_rest(d) : qr) + ((psum + pr) - 1.0);
 }
 
+// (qr - pr) / qr, the factor of q at the classes not listed: from the masses ql
+// and psum of the listed ones where those are the smaller, 1 where nothing is
+// left to share.
+__device__ __forceinline__ float rest_factor(double psum, double ql, double qr) {
+  if (!(qr > 0.0) && qr == qr) return 1.f;
+  return (float)((psum < 0.5 ? psum - ql : qr - rest_of(psum)) / qr);
+}
+
 // The loss of the row once its maximum, its sum of exp((x - m)/T) and, with
 // the rest's term, the sum over the classes not listed are known; thread 0 writes
 // the row's results. Returns the factor of q at the classes not listed.
@@ -256,9 +264,9 @@ __device__ __forceinline__ float finish_row(const DistillArgs& g, int64_t row, c
   float factor = 1.f;
   const double lr = tail ? log64(rest) - lt : 0.0;
   if (tail && some) {
-    const double pr = rest_of(psum), qr = rest / total;
+    const double qr = rest / total;
     s += rest_term(psum, lr, qr);
-    factor = qr > 0.0 || qr != qr ? (float)((qr - pr) / qr) : 1.f;
+    factor = rest_factor(psum, 1.0 - qr, qr);
   }
   if (threadIdx.x == 0) {
     g.row_loss[row] = some ? (float)(g.t * g.t * s) : 0.f;
@@ -405,9 +413,10 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   auto x4 = [&](int c) -> const f4* {
     return reinterpret_cast<const f4*>(reinterpret_cast<const char*>(xr + head) + (uint32_t)c * 16u);
   };
-  // the entries' loads go first: a wait for them leaves the row's in flight
-  const int64_t id64 = t < g.k ? g.ids[row * g.k + t] : -1;
-  const float top = t < g.k ? g.top[row * g.k + t] : 0.f;
+  // the entries' loads go first (a thread's first one; the rest of long lists
+  // later): a wait for them leaves the row's in flight
+  const int64_t id0 = t < g.k ? g.ids[row * g.k + t] : -1;
+  const float top0 = t < g.k ? g.top[row * g.k + t] : 0.f;
   const float tlse = TAIL ? g.top_lse[row] : 0.f;
   // one of the up to 3 classes before the float4s, or after them
   const int e1 = t < 3 ? t : head + 4 * c4 + t - 3;
@@ -418,50 +427,88 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   for (int q = 0; q < NV; ++q) v[q] = ld_stream(x4(min(q * RT + t, c4 - 1)));
   for (int i = t; i < bitmap_words(C); i += RT) bits[i] = 0;
   if (t == 0) twice = 0;
+  // the student's logit at this thread's first entry: last of the loads, waited
+  // for after the entries' arithmetic
+  const float x0 = id0 >= 0 && id0 < C ? xr[id0] : NEG_INF;
   bool some;
-  float prf = 0.f;     // what the entries leave
+  float psumf = 0.f, prf = 0.f;  // the entries' mass, and what they leave
   {
-    double psum;
-    const bool there = id64 >= 0 && id64 < C && top != NEG_INF;
-    if (id64 >= C) atomicOr(g.guard, 1);
-    const int id = there ? (int)id64 : -1;
-    const float xe = there ? xr[id] : NEG_INF;
-    if (t < g.k) eid[t] = id;
-    some = __syncthreads_or(there) != 0;  // and the bitmap is clear
-    if (there) {
+    // the thread's first entry in registers, the others of a long list through LDS
+    const bool there0 = id0 >= 0 && id0 < C && top0 != NEG_INF;
+    bool any = there0;
+    float tm = there0 ? top0 : NEG_INF;
+    if (id0 >= C) atomicOr(g.guard, 1);
+    if (t < g.k) eid[t] = there0 ? (int)id0 : -1;
+#pragma unroll 1
+    for (int j = t + RT; j < g.k; j += RT) {
+      const int64_t id = g.ids[row * g.k + j];
+      const float top = g.top[row * g.k + j];
+      const bool there = id >= 0 && id < C && top != NEG_INF;
+      if (id >= C) atomicOr(g.guard, 1);
+      eid[j] = there ? (int)id : -1;
+      elp[j] = (double)top;
+      any |= there;
+      tm = fmaxf(tm, there ? top : NEG_INF);
+    }
+    some = __syncthreads_or(any) != 0;  // and the bitmap is clear
+    if constexpr (!TAIL) tm = over_block<RT, MaxF32>(tm, lds);
+    auto mark = [&](int id) {
       const int at = id + 4 - head;  // float4 c has the four bits from 4 (c + 1)
       const uint32_t bit = 1u << (at & 31);
       if (atomicOr(bits + (at >> 5), bit) & bit) twice = 1;
+    };
+    auto log_of = [&](double top) { return TAIL ? top / g.t - (double)tlse : (top - (double)tm) / g.t; };
+    if (there0) mark((int)id0);
+    double l0 = log_of((double)top0);
+    double p0 = there0 ? exp64(l0) : 0.0;
+    double psum = p0;
+#pragma unroll 1
+    for (int j = t + RT; j < g.k; j += RT) {
+      if (eid[j] >= 0) mark(eid[j]);
+      const double l = log_of(elp[j]);
+      const double p = eid[j] >= 0 ? exp64(l) : 0.0;
+      elp[j] = l;
+      ep[j] = p;
+      psum += p;
     }
-    double lp, p;
-    if constexpr (TAIL) {
-      lp = (double)top / g.t - (double)tlse;
-      p = there ? exp64(lp) : 0.0;
-      psum = block_sum<RT>(p, red);  // its barriers publish the bitmap
-    } else {
-      const float tm = over_block<RT, MaxF32>(there ? top : NEG_INF, lds);
-      lp = ((double)top - (double)tm) / g.t;
-      p = there ? exp64(lp) : 0.0;
-      psum = block_sum<RT>(p, red);
-      p = there ? p / psum : 0.0;
-      lp -= log64(psum);
+    psum = block_sum<RT>(psum, red);  // its barriers publish the bitmap and the entries
+    if constexpr (!TAIL) {
+      const double ls = log64(psum);
+      p0 = there0 ? p0 / psum : 0.0;
+      l0 -= ls;
+#pragma unroll 1
+      for (int j = t + RT; j < g.k; j += RT) {
+        ep[j] = eid[j] >= 0 ? ep[j] / psum : 0.0;
+        elp[j] -= ls;
+      }
     }
-    bool dup = false;
-    if (twice && there)  // ids given twice: rare, so their order is looked up only then
-      for (int i = 0; i < t && !dup; ++i) dup = eid[i] == id;
-    __syncthreads();  // before an id changes under that loop
     if (t < g.k) {
-      ep[t] = p;
-      elp[t] = lp;
-      ex[t] = xe;
-      if (dup) eid[t] = -2 - id;
+      ep[t] = p0;
+      elp[t] = l0;
     }
+    if (twice) {  // ids given twice: rare, so their order is looked up only then
+      // (an entry's code changes once, from id to -2 - id, and either names the id)
+#pragma unroll 1
+      for (int j = t; j < g.k; j += RT) {
+        const int id = eid[j];
+        bool dup = false;
+        for (int i = 0; i < j && !dup; ++i) dup = id >= 0 && (eid[i] == id || eid[i] == -2 - id);
+        if (dup) eid[j] = -2 - id;
+      }
+      __syncthreads();
+    }
+    if (t < g.k) ex[t] = there0 ? x0 : NEG_INF;
+#pragma unroll 1
+    for (int j = t + RT; j < g.k; j += RT) ex[j] = eid[j] == -1 ? NEG_INF : xr[eid[j] < 0 ? -2 - eid[j] : eid[j]];
     if (t == 0) psum_at = psum;
+    psumf = uniform((float)psum);
     prf = uniform((float)rest_of(psum));
   }
   auto listed = [&](int c) -> uint32_t { return TAIL ? bits[(c + 1) >> 3] >> (((c + 1) & 7) * 4) & 15u : 0u; };
   if (TAIL && has1 && (bits[(e1 + 4 - head) >> 5] >> ((e1 + 4 - head) & 31) & 1u)) v1 = NEG_INF;
-  float m = t < g.k ? ex[t] : NEG_INF, s = 0.f;
+  float m = NEG_INF, s = 0.f;
+#pragma unroll 1
+  for (int j = t; j < g.k; j += RT) m = fmaxf(m, ex[j]);
   if constexpr (NV > 0) {
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
@@ -504,10 +551,13 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     s += v1;
   }
   const float rest = over_block<RT, AddF32>(s, lds + 2 * (RT / 64));
-  float total = rest;
+  float total = rest, mine = 0.f;
   if constexpr (TAIL) {
-    const float eq = t < g.k && eid[t] >= 0 ? __builtin_amdgcn_exp2f((ex[t] - m) * scale2) : 0.f;
-    total += over_block<RT, AddF32>(eq, lds + 3 * (RT / 64));
+#pragma unroll 1
+    for (int j = t; j < g.k; j += RT)
+      if (eid[j] >= 0) mine += __builtin_amdgcn_exp2f((ex[j] - m) * scale2);
+    mine = over_block<RT, AddF32>(mine, lds + 3 * (RT / 64));
+    total += mine;
   }
   if constexpr (GRAD) {
     float* const dr = g.dx + row * C;
@@ -518,7 +568,10 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     };
     if (some) {
       float gs = g.gscale / total;
-      if constexpr (TAIL) gs *= rest > 0.f || rest != rest ? 1.f - prf * (total / rest) : 1.f;
+      // (qr - pr) / qr, from the entries' masses where those are the smaller
+      if constexpr (TAIL)
+        if (rest > 0.f || rest != rest)
+          gs *= (psumf < 0.5f ? psumf - mine / total : rest / total - prf) * (total / rest);
       if constexpr (NV > 0) {
 #pragma unroll
         for (int q = 0; q < NV; ++q)
@@ -539,20 +592,23 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
       if (has1) dr[e1] = 0.f;
     }
     __syncthreads();  // the entries' own values go over what the row's threads wrote
-    if (t < g.k && eid[t] >= 0) {
-      const int id = eid[t];
-      double p = ep[t];
+#pragma unroll 1
+    for (int j = t; j < g.k; j += RT) {
+      const int id = eid[j];
+      if (id < 0) continue;
+      double p = ep[j];
       if (twice)
-        for (int i = t + 1; i < g.k; ++i)
+        for (int i = j + 1; i < g.k; ++i)
           if (eid[i] == -2 - id) p += ep[i];
-      const float eq = __builtin_amdgcn_exp2f((ex[t] - m) * scale2);
+      const float eq = __builtin_amdgcn_exp2f((ex[j] - m) * scale2);
       dr[id] = (float)((double)eq / (double)total - p) * g.gscale;
     }
   }
   const double lt = log64((double)total);
   double terms = 0.0;
-  if (t < g.k && eid[t] != -1)
-    terms = entry_term(ep[t], elp[t], ((double)ex[t] - (double)m) / g.t - lt, TAIL, eid[t] <= -2);
+#pragma unroll 1
+  for (int j = t; j < g.k; j += RT)
+    if (eid[j] != -1) terms += entry_term(ep[j], elp[j], ((double)ex[j] - (double)m) / g.t - lt, TAIL, eid[j] <= -2);
   terms = block_sum<RT>(terms, red);
   if (t == 0) {
     double lr = 0.0;
@@ -579,8 +635,11 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(const DistillArgs g, const f
   const float l = g.lse[row];
   float factor = 1.f;
   if (g.top_lse && some) {
-    const double pr = rest_of(psum), qr = exp64((double)g.rest[row]);
-    factor = qr > 0.0 || qr != qr ? (float)((qr - pr) / qr) : 1.f;
+    double ql = 0.0;
+    for (int j = threadIdx.x; j < g.k; j += NT)
+      if (a.id[j] >= 0 && a.dup[j] < 0) ql += (double)expf(xr[a.id[j]] * g.inv_t - l);
+    ql = block_sum<NT>(ql, red);
+    factor = rest_factor(psum, ql, exp64((double)g.rest[row]));
   }
   float* dr = g.dx + row * g.c;
   for (int c = threadIdx.x; c < g.c; c += NT) {
@@ -633,7 +692,7 @@ bool launch_rows(const DistillArgs& g) {
   const size_t lds = (size_t)g.k * (2 * sizeof(double) + sizeof(int) + sizeof(float)) + sizeof(uint32_t) * (size_t)bitmap_words(g.c);
   const float scale2 = (float)(1.4426950408889634 / g.t);
 #define OXI_DR(RT, NV)                                                                        \
-  if (NV == 0 || (c4 <= RT * NV && g.k <= RT)) {                                              \
+  if (NV == 0 || c4 <= RT * NV) {                                                             \
     distill_rows_k<RT, NV, GRAD, TAIL, NTS><<<grid, dim3(RT), lds, stream()>>>(g, scale2);    \
     return true;                                                                              \
   }

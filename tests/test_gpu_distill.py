@@ -273,3 +273,32 @@ def test_buffers_at_any_float(hip, shift, c):
     w = oracle(x, ids, top, 1.0)
     assert (np.abs(got[shift:shift + n * c].reshape(n, c) - w["grad"]) <= w["bgrad"]).all()
     assert (np.abs(row.numpy() - w["rows"]) <= w["brow"]).all()
+
+
+@pytest.mark.parametrize("c", [300, 5001, 70001])
+def test_gradient_where_nearly_everything_is_left_over(hip, c):
+    """A few entries of small mass: q (1 - pr/qr) at the other classes is a small part of q, known to the accuracy of
+    the masses listed (psum and ql), not of 1 less them."""
+    T = 4.0
+    x, ids, top, teacher = student_and_teacher(4, c, 3, c)
+    lse = teacher_lse(teacher, T)
+    D = hip.DeviceArray.from_numpy
+    _, _, slse, rest, d = hip.distill_fwd(D(x), D(ids), D(top), T, D(lse), need_grad=True)
+    back = hip.distill_bwd(D(x), D(ids), D(top), slse, rest, D(np.ones(1, np.float32)), T, D(lse)).numpy()
+    d = d.numpy()
+    z = x.astype(np.float64) / T
+    for r in range(4):
+        lq = z[r] - z[r].max() - np.log(np.exp(z[r] - z[r].max()).sum())
+        q = np.exp(lq)
+        eps = U * (3 * np.abs(z[r] - z[r].max()) + 6)
+        dl = (q * eps).sum() + (c / 64 + 26) * U
+        p = np.exp(top[r].astype(np.float64) / T - float(lse[r]))
+        psum, ql = p.sum(), q[ids[r]].sum()
+        assert psum < 0.25
+        out = np.ones(c, bool)
+        out[ids[r]] = False
+        want = T / 4 * q * (psum - ql) / (1 - ql)
+        # the masses' errors, then the product's; the backward has lse and the logits at float32's steps too
+        for got, more in ((d[r], 0.0), (back[r], U * (3 * np.abs(z[r]).max() + 3 * abs(float(slse.numpy()[r]))))):
+            bound = T / 4 * q * ((dl + more + 8 * U) * (psum + ql) / (1 - ql) + np.abs(psum - ql) * (eps + dl + more + 8 * U))
+            assert (np.abs(got - want)[out] <= bound[out]).all()
