@@ -51,8 +51,18 @@ struct Teacher {
   double* lp;
   int* id;
   int* dup;
+  int* seen;   // a hash table of the ids, seen_slots(k) of them
+  bool twice;  // whether any id is given twice
 };
-constexpr size_t teacher_bytes(int64_t k) { return (size_t)k * (2 * sizeof(double) + 2 * sizeof(int)); }
+// A power of two, at least twice the entries: a probe always ends at a free slot.
+constexpr int seen_slots(int64_t k) {
+  int n = 2;
+  while (n < 2 * k) n *= 2;
+  return n;
+}
+constexpr size_t teacher_bytes(int64_t k) {
+  return (size_t)k * (2 * sizeof(double) + 2 * sizeof(int)) + (size_t)seen_slots(k) * sizeof(int);
+}
 
 __device__ __forceinline__ Teacher teacher_at(double* lds, int k) {
   Teacher a;
@@ -60,6 +70,7 @@ __device__ __forceinline__ Teacher teacher_at(double* lds, int k) {
   a.lp = lds + k;
   a.id = reinterpret_cast<int*>(lds + 2 * k);
   a.dup = a.id + k;
+  a.seen = a.dup + k;
   return a;
 }
 
@@ -168,16 +179,20 @@ __device__ __forceinline__ double block_sum(double v, double* slots) {
   return over_block<N, AddF64>(v, slots);
 }
 
-// Fills `a` with the row's entries; returns the sum of p, and whether there is
-// any entry in `some`. All threads of the block; the entries are published.
+// Fills `a` with the row's entries; returns the sum of p, and in `some` whether
+// there is any entry. All threads of the block; the entries are published. Ids
+// given twice are rare: the entries' order is looked up only where the hash table
+// met one.
 template <int N>
-__device__ __forceinline__ double load_teacher(const DistillArgs& g, int64_t row, const Teacher& a, double* red,
+__device__ __forceinline__ double load_teacher(const DistillArgs& g, int64_t row, Teacher& a, double* red,
                                                bool& some) {
   const int64_t* ids = g.ids + row * g.k;
   const float* top = g.top + row * g.k;
   float* redf = reinterpret_cast<float*>(red);
   float tm = NEG_INF;
   int any = 0;
+  const int slots = seen_slots(g.k);
+  for (int i = threadIdx.x; i < slots; i += N) a.seen[i] = -1;
   for (int j = threadIdx.x; j < g.k; j += N) {
     const int64_t id = ids[j];
     const float v = top[j];
@@ -192,6 +207,7 @@ __device__ __forceinline__ double load_teacher(const DistillArgs& g, int64_t row
   }
   some = __syncthreads_or(any) != 0;
   tm = group_max<N>(tm, redf);
+  int met = 0;
   double s = 0.0;
   for (int j = threadIdx.x; j < g.k; j += N) {
     const bool there = a.id[j] >= 0;
@@ -201,13 +217,27 @@ __device__ __forceinline__ double load_teacher(const DistillArgs& g, int64_t row
     a.lp[j] = l;
     a.p[j] = p;
     s += p;
-    int d = -1;
-    if (there)
-      for (int i = 0; i < j && d < 0; ++i)
-        if (a.id[i] == a.id[j]) d = i;
-    a.dup[j] = d;
+    a.dup[j] = -1;
+    if (there) {
+      const int id = a.id[j];
+      for (int h = (int)((uint32_t)id * 2654435761u >> 16) & (slots - 1);; h = (h + 1) & (slots - 1)) {
+        const int old = atomicCAS(a.seen + h, -1, id);
+        if (old == -1) break;
+        if (old == id) {
+          met = 1;
+          break;
+        }
+      }
+    }
   }
   s = block_sum<N>(s, red);
+  a.twice = __syncthreads_or(met) != 0;
+  if (a.twice) {
+    for (int j = threadIdx.x; j < g.k; j += N)
+      if (a.id[j] >= 0)
+        for (int i = 0; i < j && a.dup[j] < 0; ++i)
+          if (a.id[i] == a.id[j]) a.dup[j] = i;
+  }
   if (!g.top_lse && some) {  // divide by the sum
     const double ls = log64(s);
     for (int j = threadIdx.x; j < g.k; j += N) {
@@ -285,9 +315,10 @@ __device__ __forceinline__ void write_entries(const DistillArgs& g, int64_t row,
   for (int j = threadIdx.x; j < g.k; j += N) {
     const int id = a.id[j];
     if (id < 0 || a.dup[j] >= 0) continue;
-    double p = 0.0;
-    for (int i = j; i < g.k; ++i)
-      if (a.id[i] == id) p += a.p[i];
+    double p = a.p[j];
+    if (a.twice)
+      for (int i = j + 1; i < g.k; ++i)
+        if (a.dup[i] == j) p += a.p[i];
     dr[id] = (float)(q(id) - p) * gscale;
   }
 }
@@ -310,7 +341,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_k(const DistillArgs g) {
   extern __shared__ __align__(16) double dyn[];
   __shared__ double red[NT / 64];
   __shared__ uint32_t bits[STRETCH / 32];
-  const Teacher a = teacher_at(dyn, g.k);
+  Teacher a = teacher_at(dyn, g.k);
   const int t = threadIdx.x;
   const int64_t row = blockIdx.x;
   const float* xr = g.x + row * g.c;
@@ -622,31 +653,56 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   }
 }
 
-// The gradient from the forward's log-sum-exp and rest, for an upstream scalar.
-__global__ __launch_bounds__(NT) void distill_bwd_k(const DistillArgs g, const float* __restrict__ gloss) {
+// The gradient from the forward's log-sum-exp and rest, for an upstream scalar: a
+// block a row, BWD_U granules in flight a thread (the up to 3
+// classes before the first and after the last go one to a thread). HBM bounds
+// it: it reads the logits once and writes the gradient.
+constexpr int BWD_U = 4;
+
+template <int N, bool NTS>
+__global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const float* __restrict__ gloss,
+                                                   const float scale2) {
   extern __shared__ __align__(16) double dyn[];
-  __shared__ double red[NT / 64];
-  const Teacher a = teacher_at(dyn, g.k);
+  __shared__ double red[N / 64];
+  Teacher a = teacher_at(dyn, g.k);
+  const int t = threadIdx.x;
   const int64_t row = blockIdx.x;
   const float* xr = g.x + row * g.c;
+  float* dr = g.dx + row * g.c;
+  const int head = min((int)((0 - (reinterpret_cast<uintptr_t>(xr) >> 2)) & 3u), g.c);
+  const int c4 = (g.c - head) >> 2;
   bool some;
-  const double psum = load_teacher<NT>(g, row, a, red, some);
+  const double psum = load_teacher<N>(g, row, a, red, some);
   const float scale = g.gscale * gloss[0];
-  const float l = g.lse[row];
+  const float l2 = g.lse[row] * 1.4426950408889634f;
+  auto prob = [&](float x) { return __builtin_amdgcn_exp2f(x * scale2 - l2); };
   float factor = 1.f;
   if (g.top_lse && some) {
     double ql = 0.0;
-    for (int j = threadIdx.x; j < g.k; j += NT)
-      if (a.id[j] >= 0 && a.dup[j] < 0) ql += (double)expf(xr[a.id[j]] * g.inv_t - l);
-    ql = block_sum<NT>(ql, red);
+    for (int j = t; j < g.k; j += N)
+      if (a.id[j] >= 0 && a.dup[j] < 0) ql += (double)prob(xr[a.id[j]]);
+    ql = block_sum<N>(ql, red);
     factor = rest_factor(psum, ql, exp64((double)g.rest[row]));
   }
-  float* dr = g.dx + row * g.c;
-  for (int c = threadIdx.x; c < g.c; c += NT) {
-    const float e = expf(xr[c] * g.inv_t - l) * scale;
-    dr[c] = some ? e * factor : 0.f;
+  const float gs = scale * factor;
+  auto out = [&](float x) { return some ? prob(x) * gs : 0.f; };
+  const f4* x4 = reinterpret_cast<const f4*>(xr + head);
+  f4u* d4 = reinterpret_cast<f4u*>(dr + head);
+  for (int c0 = t; c0 < c4; c0 += BWD_U * N) {
+    f4 v[BWD_U];
+#pragma unroll
+    for (int u = 0; u < BWD_U; ++u) v[u] = ld_stream(x4 + min(c0 + u * N, c4 - 1));
+#pragma unroll
+    for (int u = 0; u < BWD_U; ++u) {
+      if (c0 + u * N >= c4) continue;
+      const f4 d = {out(v[u].x), out(v[u].y), out(v[u].z), out(v[u].w)};
+      if constexpr (NTS) __builtin_nontemporal_store(d, d4 + c0 + u * N);
+      else d4[c0 + u * N] = d;
+    }
   }
-  write_entries<NT>(g, row, a, scale, [&](int id) { return (double)expf(xr[id] * g.inv_t - l); });
+  const int e1 = t < 3 ? t : head + 4 * c4 + t - 3;
+  if (t < 3 ? t < head : t < 6 && e1 < g.c) dr[e1] = out(xr[e1]);
+  write_entries<N>(g, row, a, scale, [&](int id) { return (double)prob(xr[id]); });
 }
 
 // loss[0] = sum of the rows' losses / divisor, in float64 in a fixed order.
@@ -760,7 +816,19 @@ int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, c
   OXI_CHECK_INIT();
   const DistillArgs g{logits, ids,    top, top_lse, nullptr, const_cast<float*>(lse), const_cast<float*>(rest), dlogits, n,
                       (int)c, (int)k, 1.0f / temperature, (double)temperature, temperature / divisor, guard_flag()};
-  distill_bwd_k<<<dim3((unsigned)n), dim3(NT), teacher_bytes(k), stream()>>>(g, gloss);
+  const float scale2 = (float)(1.4426950408889634 / g.t);
+  const dim3 grid((unsigned)n);
+  const size_t lds = teacher_bytes(k);
+  const bool nt = nt_stream_stores(n * c * 4);
+#define OXI_DB(N)                                                                       \
+  if (nt) distill_bwd_k<N, true><<<grid, dim3(N), lds, stream()>>>(g, gloss, scale2);   \
+  else distill_bwd_k<N, false><<<grid, dim3(N), lds, stream()>>>(g, gloss, scale2);
+  if (c > 16384) {
+    OXI_DB(1024)
+  } else {
+    OXI_DB(256)
+  }
+#undef OXI_DB
   return check_launch("distill_bwd");
 }
 
