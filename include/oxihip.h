@@ -320,7 +320,7 @@ int oxi_add_rms_norm_fwd(const float* x, const float* r, const float* w, float* 
 /* Its VJP for upstream gradients gy of y and gh of h (NULL: none):
  * dx = gh + the oxi_rms_norm_bwd of gy at h, the gradient of x and of r alike,
  * and dw. `dx` may be gh itself; dx or dw may be NULL to skip. `workspace`:
- * device memory of oxi_add_rms_norm_bwd_workspace bytes, 8-byte aligned, that
+ * device memory of oxi_add_rms_norm_bwd_workspace bytes, 16-byte aligned, that
  * the call alone uses until the stream has passed it, or NULL to take it from
  * the caching allocator (a call under graph capture passes its own).
  * Deterministic. */

@@ -422,12 +422,24 @@ __global__ __launch_bounds__(BS) void add_norm_bwd_loop_k(const float* __restric
   }
 }
 
+// Four columns a thread, one where the row's are not whole 4-byte words.
+template <int W>
 __global__ __launch_bounds__(BS) void e4m3_dequantize_k(const uint8_t* __restrict__ q, const float* __restrict__ scale,
                                                         float* __restrict__ y, int64_t rows, int H, int group,
                                                         int groups) {
+  const int c = (blockIdx.x * BS + threadIdx.x) * W;
+  if (c >= H) return;
+  const int g = c / group;  // groups are multiples of 4 columns, or the row
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-    const int c = blockIdx.x * BS + threadIdx.x;
-    if (c < H) y[row * H + c] = __builtin_amdgcn_cvt_f32_fp8(q[row * H + c], 0) * scale[row * groups + c / group];
+    const float s = scale[row * groups + g];
+    if constexpr (W == 4) {
+      const int p = *reinterpret_cast<const int*>(q + row * H + c);
+      const f4 v = {__builtin_amdgcn_cvt_f32_fp8(p, 0), __builtin_amdgcn_cvt_f32_fp8(p, 1),
+                    __builtin_amdgcn_cvt_f32_fp8(p, 2), __builtin_amdgcn_cvt_f32_fp8(p, 3)};
+      *reinterpret_cast<f4u*>(y + row * H + c) = v * s;
+    } else {
+      y[row * H + c] = __builtin_amdgcn_cvt_f32_fp8(q[row * H + c], 0) * s;
+    }
   }
 }
 
@@ -466,6 +478,7 @@ bool launch_fwd(int cfg, bool odd, const float* x, const float* r, const float* 
       x, r, w, h, out, stat, rows, H, eps, log_lanes, groups)
 #define OXI_AF(TPR, NV)                                                                                         \
   case TPR * 10 + NV:                                                                                           \
+    if (!grid_fits(ceil_div(rows, row_block_threads(TPR) / TPR), row_block_threads(TPR))) return false;         \
     if (odd) OXI_AF_GO(TPR, NV, ROW_ODD, false, row_block_threads(TPR));                                        \
     else if (H == 4 * TPR * NV) OXI_AF_GO(TPR, NV, ROW_FULL, NTS, row_block_threads(TPR));                      \
     else OXI_AF_GO(TPR, NV, ROW_VEC, NTS, row_block_threads(TPR));                                              \
@@ -582,8 +595,8 @@ int oxi_add_rms_norm_bwd(const float* h, const float* w, const float* rstd, cons
   if (rows && cols) {
     if (!h || !rstd || !gy) return fail(OXI_INVALID_ARGUMENT, "add_rms_norm_bwd: NULL tensor pointer");
     if (dx && (dx == h || dx == gy)) return fail(OXI_INVALID_ARGUMENT, "add_rms_norm_bwd: dx must not be h or gy");
-    if (reinterpret_cast<uintptr_t>(workspace) & 7u)
-      return fail(OXI_INVALID_ARGUMENT, "add_rms_norm_bwd: the workspace at %p is not 8-byte aligned", workspace);
+    if (reinterpret_cast<uintptr_t>(workspace) & 15u)
+      return fail(OXI_INVALID_ARGUMENT, "add_rms_norm_bwd: the workspace at %p is not 16-byte aligned", workspace);
   }
   OXI_CHECK_INIT();
   if (rows == 0 || cols == 0) return dw && cols ? oxi_fill(dw, cols, 0.f) : OXI_OK;
@@ -598,7 +611,7 @@ int oxi_add_rms_norm_bwd(const float* h, const float* w, const float* rstd, cons
   Workspace ws(parts && !workspace ? sizeof(float) * (size_t)b.nblk * (size_t)cols : 0);
   float* part = !parts ? nullptr : workspace ? static_cast<float*>(workspace) : ws.as<float>();
   if (parts && !part) return fail_alloc("add_rms_norm_bwd: column partials");
-  const bool odd = !vec_ok(cols, {h, w, gy, gh, dx, part});
+  const bool odd = !vec_ok(cols, {h, w, gy, gh, dx});
   const int H = (int)cols;
   const bool nt = nt_stream_stores(rows * cols * 4);
 #define OXI_AB_MODE(MODE)                                                                         \
@@ -645,9 +658,14 @@ int oxi_e4m3_dequantize(const uint8_t* q, const float* scale, float* y, int64_t 
   if (int rc = check_group("e4m3_dequantize", cols, group)) return rc;
   if (!q || !scale || !y) return fail(OXI_INVALID_ARGUMENT, "e4m3_dequantize: NULL tensor pointer");
   OXI_CHECK_INIT();
-  const dim3 grid((unsigned)ceil_div(cols, BS), (unsigned)std::min<int64_t>(rows, 16384));
-  e4m3_dequantize_k<<<grid, dim3(BS), 0, stream()>>>(q, scale, y, rows, (int)cols, (int)group,
-                                                     (int)ceil_div(cols, group));
+  const int groups = (int)ceil_div(cols, group);
+  const unsigned gy = (unsigned)std::min<int64_t>(rows, 16384);
+  if (cols % 4 == 0 && !(reinterpret_cast<uintptr_t>(q) & 3u))
+    e4m3_dequantize_k<4><<<dim3((unsigned)ceil_div(cols, 4 * BS), gy), dim3(BS), 0, stream()>>>(
+        q, scale, y, rows, (int)cols, (int)group, groups);
+  else
+    e4m3_dequantize_k<1><<<dim3((unsigned)ceil_div(cols, BS), gy), dim3(BS), 0, stream()>>>(
+        q, scale, y, rows, (int)cols, (int)group, groups);
   return check_launch("e4m3_dequantize");
 }
 

@@ -137,7 +137,8 @@ def check(hip, x, ids, top, T, lse=None, divisor=None, what=""):
 @pytest.mark.parametrize("n,c,k", [
     (1, 1, 1), (2, 2, 1), (3, 3, 3), (5, 7, 2), (4, 31, 8), (6, 64, 5), (3, 255, 200), (9, 256, 8), (2, 1000, 64), (5, 1003, 50),
     (3, 4096, 100), (2, 4097, 256), (3, 16385, 8), (2, 32000, 64), (3, 32001, 7), (2, 50257, 50), (2, 65536, 16), (2, 65537, 3),
-    (1, 70001, 1024), (2, 131072, 64), (1, 200003, 33), (300, 515, 4), (1100, 96, 6)])
+    (1, 70001, 1024), (2, 131072, 64), (1, 200003, 33), (1, 300001, 5), (1, 310003, 1024), (300, 515, 4), (1100, 96, 6), (40, 9, 8), (7, 600, 300),
+    (3, 2050, 1000)])
 @pytest.mark.parametrize("T,tail", [(1.0, False), (2.0, True), (0.7, True), (4.0, False)])
 def test_loss_and_gradient(hip, n, c, k, T, tail):
     print("[case] distill", n, c, k, T, tail, flush=True)
@@ -256,23 +257,30 @@ def test_no_rows(hip):
     assert loss.numpy()[0] == 0
 
 
-@pytest.mark.parametrize("shift", [1, 2, 3])
-@pytest.mark.parametrize("c", [64, 515, 4096, 70000])
-def test_buffers_at_any_float(hip, shift, c):
+@pytest.mark.parametrize("shift,to", [(1, 1), (2, 2), (3, 3), (0, 1), (2, 0), (1, 3)])
+@pytest.mark.parametrize("c", [6, 64, 515, 4096, 70000])
+def test_buffers_at_any_float(hip, shift, to, c):
+    """Logits and gradient `shift` and `to` floats past a 16-byte address."""
     n, k = 3, 5
     x, ids, top, _ = student_and_teacher(n, c, k, c)
     D = hip.DeviceArray.from_numpy
     src = D(np.concatenate([np.zeros(shift, np.float32), x.ravel()]))
-    dst = D(np.full(n * c + 8, 7, np.float32))
-    di, dt = D(ids), D(top)
+    dst, dst2 = (D(np.full(n * c + 8, 7, np.float32)) for _ in range(2))
+    di, dt, one = D(ids), D(top), D(np.ones(1, np.float32))
     loss, row, lse, rest = (hip.DeviceArray((m,)) for m in (1, n, n, n))
     hip.call("oxi_distill_fwd", src.ptr + 4 * shift, di.ptr, dt.ptr, None, loss.ptr, row.ptr, lse.ptr, rest.ptr,
-             dst.ptr + 4 * shift, n, c, k, 1.0, float(n))
-    got = dst.numpy()
-    assert (got[:shift] == 7).all() and (got[shift + n * c:] == 7).all()
+             dst.ptr + 4 * to, n, c, k, 1.0, float(n))
+    hip.call("oxi_distill_bwd", src.ptr + 4 * shift, di.ptr, dt.ptr, None, lse.ptr, rest.ptr, one.ptr, dst2.ptr + 4 * to, n,
+             c, k, 1.0, float(n))
     w = oracle(x, ids, top, 1.0)
-    assert (np.abs(got[shift:shift + n * c].reshape(n, c) - w["grad"]) <= w["bgrad"]).all()
     assert (np.abs(row.numpy() - w["rows"]) <= w["brow"]).all()
+    q = np.exp(x - w["lse"][:, None])
+    # the backward's exponent: the logit's and lse's own float32 steps
+    more = q / n * U * (3 * np.abs(w["lse"][:, None]) + 3 * np.abs(x) + 16)
+    for buf, extra in ((dst, 0.0), (dst2, more)):
+        got = buf.numpy()
+        assert (got[:to] == 7).all() and (got[to + n * c:] == 7).all()
+        assert (np.abs(got[to:to + n * c].reshape(n, c) - w["grad"]) <= w["bgrad"] + extra).all()
 
 
 @pytest.mark.parametrize("c", [300, 5001, 70001])

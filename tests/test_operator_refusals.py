@@ -41,8 +41,8 @@ def test_add_rms_norm(capi):
         call(bwd, P, P, None, P, P, P, P, None, 2, 4, 0)
     with pytest.raises(ValueError, match="dx must not be"):
         call(bwd, P, P, P, P + 64, P, P, P, None, 2, 4, 0)
-    with pytest.raises(ValueError, match="8-byte aligned"):
-        call(bwd, P, P, P, P, P, P + 64, P, P + 4, 2, 4, 0)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        call(bwd, P, P, P, P, P, P + 64, P, P + 8, 2, 4, 0)
     for g in (0, -1, 1, 16, 96, 512, 5000):
         with pytest.raises(ValueError, match="groups of"):
             call(q8, P, P, P, P, P, P, 2, 4096, g, 1e-6)
