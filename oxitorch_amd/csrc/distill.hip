@@ -381,9 +381,8 @@ __global__ __launch_bounds__(NT) void distill_fwd_k(const DistillArgs g) {
 
 // ---------------------------------------------------------------------------
 // A row a block: RT * NV float4s held in registers, so the logits cross HBM once
-// for the loss and its gradient. The float4s are a row's 16-byte granules, at
-// whatever float it starts; the up to 3 classes before and after them go a float
-// to a thread. Exponentials are exp2 of (x - m) * (log2(e)/T). With the rest's term the
+// for the loss and its gradient. The float4s begin at a row's first 128-byte line;
+// the classes before and after them go a float to a thread. Exponentials are exp2 of (x - m) * (log2(e)/T). With the rest's term the
 // listed classes are taken out of the registers (an exponential of 0) by a
 // bitmap in LDS, and their own few are added by the entries' threads. The
 // block's stores write the row as if nothing were listed; the entries' values go
@@ -407,8 +406,15 @@ __device__ __forceinline__ f4 exp2_4(const f4& z) {
             __builtin_amdgcn_exp2f(z.w)};
 }
 
-// Words of the bitmap of C classes, which starts up to 4 bits in.
-constexpr int bitmap_words(int C) { return (C + 4 + 31) / 32 + 1; }
+// Classes of a row before its float4s: up to the first 128-byte line, so that a
+// wave's accesses are whole lines ((4096, 50257) from the first 16 bytes on: 327
+// us), or to the first 16 bytes in short rows.
+__device__ __forceinline__ int row_head(const float* row, int C) {
+  return (int)((0 - (reinterpret_cast<uintptr_t>(row) >> 2)) & (C >= 256 ? 31u : 3u));
+}
+
+// Words of the bitmap of C classes, which starts up to 32 bits in.
+constexpr int bitmap_words(int C) { return (C + 32 + 31) / 32 + 1; }
 
 // A value that all threads hold, in a scalar register.
 __device__ __forceinline__ float uniform(float v) { return readlane_f32(v, 0); }
@@ -437,7 +443,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   const int C = g.c;
   const float* xr = g.x + row * C;
   // the row's classes before its first 16-byte address, and its float4s from there
-  const int head = (int)((0 - (reinterpret_cast<uintptr_t>(xr) >> 2)) & 3u);
+  const int head = row_head(xr, C);
   const int c4 = (C - head) >> 2;
   // float4 c at a 32-bit byte offset from a uniform address: one register an
   // access, not two
@@ -449,9 +455,9 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   const int64_t id0 = t < g.k ? g.ids[row * g.k + t] : -1;
   const float top0 = t < g.k ? g.top[row * g.k + t] : 0.f;
   const float tlse = TAIL ? g.top_lse[row] : 0.f;
-  // one of the up to 3 classes before the float4s, or after them
-  const int e1 = t < 3 ? t : head + 4 * c4 + t - 3;
-  const bool has1 = t < 3 ? t < head : t < 6 && e1 < C;
+  // one of the up to 31 classes before the float4s, or the 3 after them
+  const int e1 = t < 32 ? t : head + 4 * c4 + t - 32;
+  const bool has1 = t < 32 ? t < head : t < 35 && e1 < C;
   float v1 = has1 ? xr[e1] : NEG_INF;
   f4 v[NV ? NV : 1];
 #pragma unroll
@@ -484,7 +490,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     some = __syncthreads_or(any) != 0;  // and the bitmap is clear
     if constexpr (!TAIL) tm = over_block<RT, MaxF32>(tm, lds);
     auto mark = [&](int id) {
-      const int at = id + 4 - head;  // float4 c has the four bits from 4 (c + 1)
+      const int at = id + 32 - head;  // float4 c has the four bits from 32 + 4 c
       const uint32_t bit = 1u << (at & 31);
       if (atomicOr(bits + (at >> 5), bit) & bit) twice = 1;
     };
@@ -535,8 +541,8 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     psumf = uniform((float)psum);
     prf = uniform((float)rest_of(psum));
   }
-  auto listed = [&](int c) -> uint32_t { return TAIL ? bits[(c + 1) >> 3] >> (((c + 1) & 7) * 4) & 15u : 0u; };
-  if (TAIL && has1 && (bits[(e1 + 4 - head) >> 5] >> ((e1 + 4 - head) & 31) & 1u)) v1 = NEG_INF;
+  auto listed = [&](int c) -> uint32_t { return TAIL ? bits[(c >> 3) + 1] >> ((c & 7) * 4) & 15u : 0u; };
+  if (TAIL && has1 && (bits[(e1 + 32 - head) >> 5] >> ((e1 + 32 - head) & 31) & 1u)) v1 = NEG_INF;
   float m = NEG_INF, s = 0.f;
 #pragma unroll 1
   for (int j = t; j < g.k; j += RT) m = fmaxf(m, ex[j]);
@@ -654,8 +660,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
 }
 
 // The gradient from the forward's log-sum-exp and rest, for an upstream scalar: a
-// block a row, BWD_U granules in flight a thread (the up to 3
-// classes before the first and after the last go one to a thread). HBM bounds
+// block a row, BWD_U float4s in flight a thread, its classes as in distill_rows_k. HBM bounds
 // it: it reads the logits once and writes the gradient.
 constexpr int BWD_U = 4;
 
@@ -669,7 +674,7 @@ __global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const fl
   const int64_t row = blockIdx.x;
   const float* xr = g.x + row * g.c;
   float* dr = g.dx + row * g.c;
-  const int head = min((int)((0 - (reinterpret_cast<uintptr_t>(xr) >> 2)) & 3u), g.c);
+  const int head = min(row_head(xr, g.c), g.c);
   const int c4 = (g.c - head) >> 2;
   bool some;
   const double psum = load_teacher<N>(g, row, a, red, some);
@@ -700,8 +705,8 @@ __global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const fl
       else d4[c0 + u * N] = d;
     }
   }
-  const int e1 = t < 3 ? t : head + 4 * c4 + t - 3;
-  if (t < 3 ? t < head : t < 6 && e1 < g.c) dr[e1] = out(xr[e1]);
+  const int e1 = t < 32 ? t : head + 4 * c4 + t - 32;
+  if (t < 32 ? t < head : t < 35 && e1 < g.c) dr[e1] = out(xr[e1]);
   write_entries<N>(g, row, a, scale, [&](int id) { return (double)prob(xr[id]); });
 }
 
