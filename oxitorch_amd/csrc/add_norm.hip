@@ -61,9 +61,30 @@ __device__ __forceinline__ float abs_max4(const f4& v) {
 
 typedef uint32_t u32u __attribute__((aligned(1)));
 
+// An odd row's slots where the operand that they were formed from may be this
+// very row: each float by the one slot that owns it. The last slot's repeated
+// floats may have been read after their owner, in another wave, had written
+// them: nothing is formed from them but what the owner writes.
+template <int TPR, int NV>
+__device__ __forceinline__ void store_owned(const RowTile<TPR, NV>& v, float* row, int H, int h4, int t) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = k * TPR + t;
+    if (c < h4 - 1) {
+      *reinterpret_cast<f4u*>(row + 4 * c) = v.v[k];
+    } else if (c == h4 - 1) {
+      const int e0 = H - 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (e0 + j >= 4 * c) row[e0 + j] = v.v[k][j];
+    }
+  }
+}
+
 // The group maxima of a row's slots: a group of 32 to 256 columns is 8 to 64
 // neighbouring lanes (log_lanes), whatever the row's length; log_lanes 0 is the
-// whole row. h may be x or r: a row is read whole before any of it is written.
+// whole row. h may be x or r: every float of it is written by the thread that
+// read it there (an odd row's repeated floats: see store_owned).
 template <int TPR, int NV, int KIND, bool NTS, int NT, int OUT>
 __global__ __launch_bounds__(NT) void add_norm_fwd_k(const float* x, const float* r, const float* __restrict__ w,
                                                      float* h, void* __restrict__ out, float* __restrict__ stat,
@@ -86,7 +107,7 @@ __global__ __launch_bounds__(NT) void add_norm_fwd_k(const float* x, const float
   if (OUT == OUT_F32 || r) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) a.v[k] = a.v[k] + b.v[k];
-    if constexpr (KIND == ROW_ODD) a.store_odd(h + row * H, H, h4, t);
+    if constexpr (KIND == ROW_ODD) store_owned(a, h + row * H, H, h4, t);
     else a.template store<NTS>(h + row * H, h4, t);
   }
   float ss = 0.f;
@@ -112,7 +133,7 @@ __global__ __launch_bounds__(NT) void add_norm_fwd_k(const float* x, const float
   if constexpr (OUT == OUT_F32) {
     if (t == 0 && stat) stat[row] = inv;
     float* y = static_cast<float*>(out);
-    if constexpr (KIND == ROW_ODD) a.store_odd(y + row * H, H, h4, t);
+    if constexpr (KIND == ROW_ODD) store_owned(a, y + row * H, H, h4, t);
     else a.template store<NTS>(y + row * H, h4, t);
   } else {
     uint8_t* q = static_cast<uint8_t*>(out) + row * H;
@@ -165,7 +186,7 @@ __global__ __launch_bounds__(NT) void add_norm_fwd_k(const float* x, const float
 template <int TPR, int NV>
 constexpr int add_bwd_threads() { return TPR == 64 ? (NV <= 2 ? 1024 : 512) : TPR; }
 
-// dx may be gh: a row is read whole before it is written.
+// dx may be gh: every float of it is written by the thread that read it there.
 template <int TPR, int NV, int MODE, int KIND, bool NTS, bool FEW>
 __global__ __launch_bounds__((add_bwd_threads<TPR, NV>())) void add_norm_bwd_k(
     const float* __restrict__ h, const float* __restrict__ w, const float* __restrict__ rstd,
@@ -262,7 +283,7 @@ __global__ __launch_bounds__((add_bwd_threads<TPR, NV>())) void add_norm_bwd_k(
 #pragma unroll
       for (int k = 0; k < NV; ++k) f.g.v[k] = f.a.v[k] + f.g.v[k] * f.inv;
     }
-    if constexpr (ODD) f.g.store_odd(dx + q * H, H, h4, t);
+    if constexpr (ODD) store_owned(f.g, dx + q * H, H, h4, t);
     else f.g.template store<NTS>(dx + q * H, h4, t);
   };
   Rows a, b;

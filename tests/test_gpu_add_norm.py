@@ -108,10 +108,13 @@ def test_no_weight_and_single_outputs(hip):
     assert np.array_equal(h2.numpy(), h.numpy()) and np.array_equal(y2.numpy(), y.numpy())
 
 
-@pytest.mark.parametrize("cols", [3, 768, 1003, 4096, 20003])
-def test_in_place(hip, cols):
+# odd rows whose last float4 begins a wave (1025, 1281, 1795, 2305, 4097, 8193, 12290) share floats with another wave's
+@pytest.mark.parametrize("rows,cols", [(21, 3), (21, 768), (21, 1003), (21, 4096), (21, 20003), (700, 1025), (700, 1281),
+                                       (600, 1795), (600, 2305), (500, 4097), (300, 8193), (300, 12290)])
+@pytest.mark.parametrize("mode", ["ref", "exact"])
+def test_in_place(hip, rows, cols, mode):
     """h over x or over r, and dx over gh: the values of the separate buffers."""
-    d = data(21, cols, cols)
+    d = data(rows, cols, cols)
     D = hip.DeviceArray.from_numpy
     w, gy = D(d["w"]), D(d["gy"])
     h, y, rstd = hip.add_rms_norm_fwd(D(d["x"]), D(d["r"]), w, EPS)
@@ -119,9 +122,10 @@ def test_in_place(hip, cols):
         b = {n: D(d[n]) for n in ("x", "r")}
         h2, y2, _ = hip.add_rms_norm_fwd(b["x"], b["r"], w, EPS, h=b[over])
         assert np.array_equal(b[over].numpy(), h.numpy()) and np.array_equal(y2.numpy(), y.numpy())
-    dx, dw = hip.add_rms_norm_bwd(h, w, rstd, gy, D(d["gh"]), mode="exact")
+    dx, dw = hip.add_rms_norm_bwd(h, w, rstd, gy, D(d["gh"]), mode=mode)
     gh, dw2 = D(d["gh"]), hip.DeviceArray((cols,))
-    hip.call("oxi_add_rms_norm_bwd", h.ptr, w.ptr, rstd.ptr, gy.ptr, gh.ptr, gh.ptr, dw2.ptr, None, 21, cols, 1)
+    hip.call("oxi_add_rms_norm_bwd", h.ptr, w.ptr, rstd.ptr, gy.ptr, gh.ptr, gh.ptr, dw2.ptr, None, rows, cols,
+             hip.NORM_VJP[mode])
     assert np.array_equal(gh.numpy(), dx.numpy()) and np.array_equal(dw2.numpy(), dw.numpy())
 
 
