@@ -164,20 +164,28 @@ __global__ __launch_bounds__(NT) void verify_sums_k(const VerifyArgs g, Sums* __
   if ((threadIdx.x & 63) == 0 && piece < pieces) part[b * pieces + piece] = Sums{left, own};
 }
 
-// The thread at whose weight the running sum, a thread's weight after those
-// before it, passes `limit`, and the sum before it; -1 where it passes none's.
+// The first thread with weight at whose weight the running sum, a thread's weight
+// after those before it, passes `limit`, and the sum before it; -1 where it passes
+// none's. The first, and not the one whose own stretch holds the limit: sums that
+// end one stretch and begin the next are rounded apart, so that a limit there lies
+// in both or in neither.
 struct Crossing {
   int at;
   double before;
 };
 template <int N>
-__device__ __forceinline__ Crossing cross(double w, double before, double limit, Crossing* slot) {
+__device__ __forceinline__ Crossing cross(double w, double before, double limit, Crossing* slots) {
+  const bool over = w > 0.0 && before + w > limit;
+  const uint64_t lanes = __ballot(over);
+  const int lane = threadIdx.x & 63, first = lanes ? __builtin_ctzll(lanes) : 0;
   __syncthreads();
-  if (threadIdx.x == 0) *slot = {-1, 0.0};
+  if (lane == first) slots[threadIdx.x >> 6] = {over ? (int)threadIdx.x : -1, before};
   __syncthreads();
-  if (w > 0.0 && before <= limit && before + w > limit) *slot = {(int)threadIdx.x, before};  // one thread's at most
-  __syncthreads();
-  return *slot;
+  Crossing c = {-1, 0.0};
+#pragma unroll
+  for (int i = N / 64 - 1; i >= 0; --i)
+    if (slots[i].at >= 0) c = slots[i];
+  return c;
 }
 
 // U: as in the first launch, the classes of a piece that each thread has.
@@ -185,7 +193,7 @@ template <int U>
 __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Sums* __restrict__ part, int64_t pieces) {
   static_assert(NT == 256, "a piece is 256 U classes");
   __shared__ double red[NT / 64];
-  __shared__ Crossing slot;
+  __shared__ Crossing slots[NT / 64];
   __shared__ int last;
   const int64_t b = blockIdx.x;
   const int t = threadIdx.x;
@@ -212,7 +220,7 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
     const double w = i0 + t < pieces ? (use_left ? pb[i0 + t].left : pb[i0 + t].own) : 0.0;
     double all;
     const double before = carry + block_before<NT>(w, red, all);
-    const Crossing c = cross<NT>(w, before, limit, &slot);
+    const Crossing c = cross<NT>(w, before, limit, slots);
     if (c.at >= 0) {
       at = i0 + c.at;
       base = c.before;
@@ -271,7 +279,7 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
     }
     double all;
     const double before = base + block_before<NT>(w, red, all);
-    Crossing c = cross<NT>(w, before, limit, &slot);
+    Crossing c = cross<NT>(w, before, limit, slots);
     if (c.at < 0) {  // the last thread with weight, its last class
       if (t == 0) last = -1;
       __syncthreads();

@@ -3,6 +3,8 @@ float64: whole numbers, equal. Random cases where a running sum comes within
 1e-12 of the number drawn (another order of the sum may round to the other side)
 are left out of the comparison; there are none among these seeds."""
 
+import math
+
 import numpy as np
 import pytest
 
@@ -225,3 +227,21 @@ def test_caller_workspace(hip):
         a2, o2 = run(hip, target, draft, tokens, u)
         assert np.array_equal(a, a2) and np.array_equal(o, o2)
         assert (ws.numpy()[n // 8:] == 5).all()
+
+
+@pytest.mark.parametrize("v", [30, 512, 600, 5000, 32000, 131072])
+def test_a_number_where_two_threads_sums_meet(hip, v):
+    """Rows of two halves with the same weights in another order, u = 1/2: the limit is where one half's sum ends and
+    the other's begins, which differ by their roundings. A sum of v terms here passes fewer than 256 roundings a
+    term, so that the token's own stretch [before, before + w) is within 2^8 * 2^-53 of the total."""
+    b = 64
+    r = rng(v)
+    half = np.exp(6 * r.standard_normal((b, v // 2))).astype(np.float32)
+    row = np.concatenate([half, r.permuted(half, axis=1)], 1)[:, None]
+    u = np.full((b, 1), 0.5, np.float32)
+    a, o = run(hip, row, None, np.zeros((b, 0), np.int64), u)
+    for s in range(b):
+        w = row[s, 0].astype(np.float64).tolist()
+        total, x = math.fsum(w), int(o[s, 0])
+        assert math.fsum(w[:x]) <= total * (0.5 + 2.0 ** -45), (s, x)
+        assert math.fsum(w[:x + 1]) >= total * (0.5 - 2.0 ** -45), (s, x)
