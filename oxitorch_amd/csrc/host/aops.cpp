@@ -421,6 +421,7 @@ std::pair<Var, Var> add_rms_norm(const Var& x, const Var& r, const Var& w, float
   const int64_t H = last_dim(x.value(), "add_rms_norm");
   if (r.value().shape != x.value().shape) err_shape(fmt_shape(x.value().shape), fmt_shape(r.value().shape));
   check_param(w.value(), H, "weight");
+  for (const Var* v : {&x, &r, &w}) require_hip(v->value(), "add_rms_norm");
   Tensor xc = t_contiguous(x.value());
   Tensor rc = t_contiguous(r.value());
   Tensor wc = t_contiguous(w.value());
@@ -790,12 +791,14 @@ RotaryFrequencies::RotaryFrequencies(const std::vector<double>& inv_freq, float 
 
 E4m3Rows t_add_rms_norm_e4m3(const Tensor& x, const std::optional<Tensor>& r, const Tensor& w, float eps,
                              int64_t group, Tensor* h) {
-  require_hip(x, "add_rms_norm_e4m3");
   if (x.ndim() == 0) err_invalid("add_rms_norm_e4m3 needs at least one dim");
   const int64_t H = x.shape.back();
   if (r && r->shape != x.shape) err_shape(fmt_shape(x.shape), fmt_shape(r->shape));
   if (w.ndim() != 1 || w.shape[0] != H) err_shape(fmt_shape(w.shape), fmt_shape({H}));
   if (group < 1) err_invalid("add_rms_norm_e4m3: groups of " + std::to_string(group) + " columns");
+  require_hip(x, "add_rms_norm_e4m3");
+  if (r) require_hip(*r, "add_rms_norm_e4m3");
+  require_hip(w, "add_rms_norm_e4m3");
   const Tensor xc = t_contiguous(x), wc = t_contiguous(w);
   Tensor rc;
   if (r) {

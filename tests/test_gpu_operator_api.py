@@ -135,6 +135,16 @@ def test_add_rms_norm_of_other_shapes(ox, F):
     assert xt.grad.shape == [3, 4, 32]
 
 
+@pytest.mark.parametrize("host", range(3))
+def test_a_host_operand_among_the_norms_is_refused(ox, F, host):
+    a = [ox.from_numpy(np.ones(s, np.float32), device="cpu" if i == host else "hip")
+         for i, s in enumerate([(3, 8), (3, 8), (8,)])]
+    with pytest.raises(NotImplementedError, match="add_rms_norm"):
+        F.add_rms_norm(*a)
+    with pytest.raises(NotImplementedError, match="add_rms_norm_e4m3"):
+        F.add_rms_norm_e4m3(*a)
+
+
 def test_e4m3(ox, F):
     r = rng(7)
     x, res = (r.standard_normal((2, 5, 300)).astype(np.float32) for _ in range(2))

@@ -213,3 +213,15 @@ def test_python_refusals():
         F.verify_drafts(ids + 8, None, cpu(3, 3, 8), cpu(3, 3))
     with pytest.raises(NotImplementedError):
         F.verify_drafts(ids, None, cpu(3, 3, 8), cpu(3, 3))
+
+
+def test_host_operands_of_the_norm():
+    import oxitorch_amd as ox
+    from oxitorch_amd.nn import functional as F
+
+    x, r, w = (ox.from_numpy(np.zeros(s, np.float32), device="cpu") for s in ((3, 8), (3, 8), (8,)))
+    with pytest.raises(NotImplementedError, match="add_rms_norm"):
+        F.add_rms_norm(x, r, w)
+    for residual in (r, None):
+        with pytest.raises(NotImplementedError, match="add_rms_norm_e4m3"):
+            F.add_rms_norm_e4m3(x, residual, w)
