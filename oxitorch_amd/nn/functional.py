@@ -74,6 +74,8 @@ def _flat_ints(values, what):
     a = np.asarray(values)
     if a.size and a.dtype.kind not in "iu":
         raise TypeError(f"{what} must be integers, got {a.dtype}")
+    if a.dtype == np.uint64 and a.size and a.max() > np.iinfo(np.int64).max:
+        raise OverflowError(f"{what}: {a.max()} does not fit in 64 signed bits")
     return a.astype(np.int64).ravel()
 
 

@@ -225,3 +225,20 @@ def test_host_operands_of_the_norm():
     for residual in (r, None):
         with pytest.raises(NotImplementedError, match="add_rms_norm_e4m3"):
             F.add_rms_norm_e4m3(x, residual, w)
+
+
+def test_integers_past_int64():
+    """As elsewhere, no wrapping: 2^64 - 1 would become -1, which is padding."""
+    import oxitorch_amd as ox
+    from oxitorch_amd.nn import functional as F
+
+    cpu = lambda *s: ox.from_numpy(np.zeros(s, np.float32), device="cpu")  # noqa: E731
+    ids = np.full((3, 2), 2 ** 64 - 1, np.uint64)
+    with pytest.raises(OverflowError, match="teacher_ids"):
+        F.distillation_loss(cpu(3, 8), ids, cpu(3, 2))
+    with pytest.raises(OverflowError, match="draft_tokens"):
+        F.verify_drafts(ids, None, cpu(3, 3, 8), cpu(3, 3))
+    with pytest.raises(OverflowError, match="lengths"):
+        F.verify_drafts(np.zeros((3, 2), np.uint64), None, cpu(3, 3, 8), cpu(3, 3), ids[:, 0])
+    with pytest.raises(OverflowError, match="positions"):
+        F.rotary_embedding(cpu(2, 3, 4), [1.0], ids[0])
