@@ -737,6 +737,8 @@ int check_distill(const char* what, int64_t n, int64_t c, int64_t k, float tempe
                 OXI_DISTILL_MAX_TOP);
   if (!(temperature > 0.f) || std::isinf(temperature))
     return fail(OXI_INVALID_ARGUMENT, "%s: the temperature must be positive, got %g", what, (double)temperature);
+  if (std::isinf((float)(1.4426950408889634 / temperature)))  // the kernels' factor of the logits
+    return fail(OXI_INVALID_ARGUMENT, "%s: a temperature of %g has no 32-bit reciprocal", what, (double)temperature);
   if (!(divisor > 0.f) || std::isinf(divisor))
     return fail(OXI_INVALID_ARGUMENT, "%s: the divisor must be positive, got %g", what, (double)divisor);
   if (n && c == 0) return fail(OXI_INVALID_ARGUMENT, "%s: zero classes", what);

@@ -101,6 +101,8 @@ def test_distill(capi):
     for k in (0, 1025):
         with pytest.raises(ValueError, match="teacher entries"):
             fwd(k=k)
+    with pytest.raises(ValueError, match="32-bit reciprocal"):
+        fwd(T=1e-40)
     for T in (0.0, -1.0, float("nan"), float("inf")):
         with pytest.raises(ValueError, match="temperature"):
             fwd(T=T)
