@@ -74,12 +74,24 @@ __device__ __forceinline__ Teacher teacher_at(double* lds, int k) {
   return a;
 }
 
-// exp, log and exp(d) - 1 - d in 64 bits, from their series: loops over
-// coefficients in constant memory, so that they take few registers where a
-// row is held in the others.
-__constant__ double RECIP[24] = {0.0,       1.0,       1.0 / 2,  1.0 / 3,  1.0 / 4,  1.0 / 5,  1.0 / 6,  1.0 / 7,
-                                 1.0 / 8,   1.0 / 9,   1.0 / 10, 1.0 / 11, 1.0 / 12, 1.0 / 13, 1.0 / 14, 1.0 / 15,
-                                 1.0 / 16,  1.0 / 17,  1.0 / 18, 1.0 / 19, 1.0 / 20, 1.0 / 21, 1.0 / 22, 1.0 / 23};
+// exp, log and exp(d) - 1 - d in 64 bits, from their series by Horner's rule: the
+// coefficients are literals in scalar registers, so that the code takes few
+// vector registers where a row is held in the others.
+struct Factorials {
+  double inv[16];  // 1/k!
+  constexpr Factorials() : inv{} {
+    double f = 1.0;
+    for (int k = 0; k < 16; ++k) {
+      if (k) f *= k;
+      inv[k] = 1.0 / f;
+    }
+  }
+};
+// A constant in scalar registers (in a vector pair the scheduler loads it early).
+__device__ __forceinline__ double scalar(double c) {
+  asm("" : "+s"(c));
+  return c;
+}
 constexpr double LN2_HI = 0x1.62e42feep-1, LN2_LO = 0x1.a39ef35793c76p-33;  // ln 2, the first part of 32 bits
 
 // e^x = 2^n e^r, |r| <= ln(2)/2: 13 terms leave r^14/14! < 2^-57.
@@ -88,9 +100,10 @@ __device__ __forceinline__ double exp64(double x) {
   if (x > 710.0) return (double)__builtin_huge_valf();
   const double n = rint(x * 1.4426950408889634);
   const double r = fma(-n, LN2_LO, fma(-n, LN2_HI, x));
-  double p = 1.0;
-#pragma unroll 1
-  for (int k = 13; k > 0; --k) p = fma(p * r, RECIP[k], 1.0);
+  constexpr Factorials F;
+  double p = F.inv[13];
+#pragma unroll
+  for (int k = 12; k >= 0; --k) p = fma(p, r, scalar(F.inv[k]));
   return __builtin_ldexp(p, (int)n);
 }
 
@@ -105,19 +118,20 @@ __device__ __forceinline__ double log64(double x) {
     --e;
   }
   const double s = (m - 1.0) / (m + 1.0), z = s * s;
-  double p = RECIP[23];
-#pragma unroll 1
-  for (int k = 21; k > 0; k -= 2) p = fma(p, z, RECIP[k]);
+  double p = 1.0 / 23;
+#pragma unroll
+  for (int k = 21; k > 0; k -= 2) p = fma(p, z, scalar(1.0 / k));
   return fma((double)e, LN2_HI, fma((double)e, LN2_LO, 2.0 * s * p));
 }
 
-// d^2/2 (1 + d/3 (1 + d/4 (...))) for small d.
+// d^2 (1/2! + d/3! + d^2/4! + ...) for small d.
 __device__ __forceinline__ double exp_rest(double d) {
   if (!(fabs(d) < 0.5)) return exp64(d) - 1.0 - d;
-  double p = 1.0;
-#pragma unroll 1
-  for (int k = 15; k > 2; --k) p = fma(p * d, RECIP[k], 1.0);
-  return 0.5 * d * d * p;
+  constexpr Factorials F;
+  double p = F.inv[15];
+#pragma unroll
+  for (int k = 14; k >= 2; --k) p = fma(p, d, scalar(F.inv[k]));
+  return d * d * p;
 }
 
 // Reductions over a wave and over the block in a fixed order, the same bits for
@@ -745,17 +759,21 @@ int check_distill(const char* what, int64_t n, int64_t c, int64_t k, float tempe
   return OXI_OK;
 }
 
-// The row kernel for c classes and k entries: as few float4s a thread as hold the
-// row, streamed past 16 on 1024 threads; false where none takes it.
+// The row kernel for c classes and k entries: as few threads as hold the row,
+// streamed past 16 float4s on 1024 of them; false where none takes it. A wave alone
+// passes no barriers, but works its entries off 64 at a time: 16384 rows of 512
+// classes with 256 and 500 entries take 46 and 94 us on it, 65 and 88 on 256
+// threads; 8192 rows of 2048 with 64 and 150 31 and 43, 33 and 36.
 template <bool GRAD, bool TAIL, bool NTS>
 bool launch_rows(const DistillArgs& g) {
   const int c4 = g.c / 4;  // at most
   if (g.c < 8 || g.c > STREAM_MAX) return false;
+  const bool one_wave = g.c + 12 * g.k <= 3700;
   const dim3 grid((unsigned)g.n);
   const size_t lds = (size_t)g.k * (2 * sizeof(double) + sizeof(int) + sizeof(float)) + sizeof(uint32_t) * (size_t)bitmap_words(g.c);
   const float scale2 = (float)(1.4426950408889634 / g.t);
 #define OXI_DR(RT, NV)                                                                        \
-  if (NV == 0 || c4 <= RT * NV) {                                                             \
+  if ((NV == 0 || c4 <= RT * NV) && (RT > 64 || one_wave)) {                                  \
     distill_rows_k<RT, NV, GRAD, TAIL, NTS><<<grid, dim3(RT), lds, stream()>>>(g, scale2);    \
     return true;                                                                              \
   }
@@ -763,6 +781,8 @@ bool launch_rows(const DistillArgs& g) {
   OXI_DR(64, 4)
   OXI_DR(64, 8)
   OXI_DR(64, 16)
+  OXI_DR(256, 2)
+  OXI_DR(256, 4)
   OXI_DR(256, 6)
   OXI_DR(256, 8)
   OXI_DR(256, 12)
@@ -832,8 +852,10 @@ int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, c
   else distill_bwd_k<N, false><<<grid, dim3(N), lds, stream()>>>(g, gloss, scale2);
   if (c > 16384) {
     OXI_DB(1024)
-  } else {
+  } else if (c + 6 * k > 2400) {
     OXI_DB(256)
+  } else {  // one wave: (16384, 512) with 8 and 500 entries 19 and 104 us against 47 and 70
+    OXI_DB(64)
   }
 #undef OXI_DB
   return check_launch("distill_bwd");
