@@ -402,9 +402,13 @@ __global__ __launch_bounds__(NT) void distill_fwd_k(const DistillArgs g) {
 // block's stores write the row as if nothing were listed; the entries' values go
 // over that after a barrier.
 //
-// The entries are worked out in float64 before the row is loaded and their
-// terms after it is stored, from LDS, so that the registers of that code do
-// not add to the row's: two blocks of 1024 x 8 a CU need 64 (see rows_waves).
+// HBM bounds it. The entries are worked out in float64 before the row is reduced and their
+// terms after it is stored, from LDS, so that the registers of that code do not
+// add to the row's: at most 128 a lane, two blocks of 512 x 16 a CU. The row's loads
+// go out before the entries' work in those (with the rest's term (8192, 32000) 364
+// us, 376 behind it; 1024 x 8 spills), and behind it where a block has the CU to
+// itself ((4096, 50257) 301 us before it, 288 behind) or four share it
+// ((4096, 8192) with the rest's term 56 and 53).
 //
 // NV = 0: longer rows, streamed twice, the first time with a running maximum; the
 // second time they come from the Infinity Cache (a block a row on every CU is
@@ -465,7 +469,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     return reinterpret_cast<const f4*>(reinterpret_cast<const char*>(xr + head) + (uint32_t)c * 16u);
   };
   // the entries' loads go first (a thread's first one; the rest of long lists
-  // later): a wait for them leaves the row's in flight
+  // later): a wait for them leaves the row's in flight, if those are
   const int64_t id0 = t < g.k ? g.ids[row * g.k + t] : -1;
   const float top0 = t < g.k ? g.top[row * g.k + t] : 0.f;
   const float tlse = TAIL ? g.top_lse[row] : 0.f;
@@ -474,12 +478,15 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   const bool has1 = t < 32 ? t < head : t < 35 && e1 < C;
   float v1 = has1 ? xr[e1] : NEG_INF;
   f4 v[NV ? NV : 1];
+  auto load_row = [&]() {
 #pragma unroll
-  for (int q = 0; q < NV; ++q) v[q] = ld_stream(x4(min(q * RT + t, c4 - 1)));
+    for (int q = 0; q < NV; ++q) v[q] = ld_stream(x4(min(q * RT + t, c4 - 1)));
+  };
+  if constexpr (RT == 512) load_row();
   for (int i = t; i < bitmap_words(C); i += RT) bits[i] = 0;
   if (t == 0) twice = 0;
-  // the student's logit at this thread's first entry: last of the loads, waited
-  // for after the entries' arithmetic
+  // the student's logit at this thread's first entry: waited for after the
+  // entries' arithmetic
   const float x0 = id0 >= 0 && id0 < C ? xr[id0] : NEG_INF;
   bool some;
   float psumf = 0.f, prf = 0.f;  // the entries' mass, and what they leave
@@ -555,6 +562,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     psumf = uniform((float)psum);
     prf = uniform((float)rest_of(psum));
   }
+  if constexpr (RT != 512) load_row();
   auto listed = [&](int c) -> uint32_t { return TAIL ? bits[(c >> 3) + 1] >> ((c & 7) * 4) & 15u : 0u; };
   if (TAIL && has1 && (bits[(e1 + 32 - head) >> 5] >> ((e1 + 32 - head) & 31) & 1u)) v1 = NEG_INF;
   float m = NEG_INF, s = 0.f;
@@ -674,11 +682,12 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
 }
 
 // The gradient from the forward's log-sum-exp and rest, for an upstream scalar: a
-// block a row, BWD_U float4s in flight a thread, its classes as in distill_rows_k. HBM bounds
-// it: it reads the logits once and writes the gradient.
-constexpr int BWD_U = 4;
-
-template <int N, bool NTS>
+// block a row, U float4s in flight a thread, as many as hold it up to 32768 classes,
+// its classes as in distill_rows_k. HBM bounds it: it reads the logits once and
+// writes the gradient, (8192, 32000) in 354 us (5.9 TB/s), (16384, 16640) in 359. Four
+// float4s on 1024 threads took 393 and 509, all loads of a row before the
+// entries' work 359-366 and 376.
+template <int N, int U, bool NTS>
 __global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const float* __restrict__ gloss,
                                                    const float scale2) {
   extern __shared__ __align__(16) double dyn[];
@@ -690,6 +699,8 @@ __global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const fl
   float* dr = g.dx + row * g.c;
   const int head = min(row_head(xr, g.c), g.c);
   const int c4 = (g.c - head) >> 2;
+  const f4* x4 = reinterpret_cast<const f4*>(xr + head);
+  f4u* d4 = reinterpret_cast<f4u*>(dr + head);
   bool some;
   const double psum = load_teacher<N>(g, row, a, red, some);
   const float scale = g.gscale * gloss[0];
@@ -705,14 +716,12 @@ __global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const fl
   }
   const float gs = scale * factor;
   auto out = [&](float x) { return some ? prob(x) * gs : 0.f; };
-  const f4* x4 = reinterpret_cast<const f4*>(xr + head);
-  f4u* d4 = reinterpret_cast<f4u*>(dr + head);
-  for (int c0 = t; c0 < c4; c0 += BWD_U * N) {
-    f4 v[BWD_U];
+  for (int c0 = t; c0 < c4; c0 += U * N) {
+    f4 v[U];
 #pragma unroll
-    for (int u = 0; u < BWD_U; ++u) v[u] = ld_stream(x4 + min(c0 + u * N, c4 - 1));
+    for (int u = 0; u < U; ++u) v[u] = ld_stream(x4 + min(c0 + u * N, c4 - 1));
 #pragma unroll
-    for (int u = 0; u < BWD_U; ++u) {
+    for (int u = 0; u < U; ++u) {
       if (c0 + u * N >= c4) continue;
       const f4 d = {out(v[u].x), out(v[u].y), out(v[u].z), out(v[u].w)};
       if constexpr (NTS) __builtin_nontemporal_store(d, d4 + c0 + u * N);
@@ -847,16 +856,23 @@ int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, c
   const dim3 grid((unsigned)n);
   const size_t lds = teacher_bytes(k);
   const bool nt = nt_stream_stores(n * c * 4);
-#define OXI_DB(N)                                                                       \
-  if (nt) distill_bwd_k<N, true><<<grid, dim3(N), lds, stream()>>>(g, gloss, scale2);   \
-  else distill_bwd_k<N, false><<<grid, dim3(N), lds, stream()>>>(g, gloss, scale2);
-  if (c > 16384) {
-    OXI_DB(1024)
-  } else if (c + 6 * k > 2400) {
-    OXI_DB(256)
-  } else {  // one wave: (16384, 512) with 8 and 500 entries 19 and 104 us against 47 and 70
-    OXI_DB(64)
+#define OXI_DB(N, U)                                                                           \
+  {                                                                                            \
+    if (nt) distill_bwd_k<N, U, true><<<grid, dim3(N), lds, stream()>>>(g, gloss, scale2);     \
+    else distill_bwd_k<N, U, false><<<grid, dim3(N), lds, stream()>>>(g, gloss, scale2);       \
   }
+  if (c + 6 * k <= 2400) {  // one wave: (16384, 512) with 8 and 500 entries 19 and 104 us against 47 and 70
+    if (c <= 1024) OXI_DB(64, 4)
+    else OXI_DB(64, 8)
+  } else if (c <= 4096) OXI_DB(256, 4)
+  else if (c <= 6144) OXI_DB(256, 6)
+  else if (c <= 8192) OXI_DB(256, 8)
+  else if (c <= 12288) OXI_DB(256, 12)
+  else if (c <= 16384) OXI_DB(256, 16)
+  else if (c <= 20480) OXI_DB(512, 10)
+  else if (c <= 24576) OXI_DB(512, 12)
+  else if (c <= 28672) OXI_DB(512, 14)
+  else OXI_DB(512, 16)
 #undef OXI_DB
   return check_launch("distill_bwd");
 }

@@ -138,7 +138,8 @@ def check(hip, x, ids, top, T, lse=None, divisor=None, what=""):
     (1, 1, 1), (2, 2, 1), (3, 3, 3), (5, 7, 2), (4, 31, 8), (6, 64, 5), (3, 255, 200), (9, 256, 8), (2, 1000, 64), (5, 1003, 50),
     (3, 4096, 100), (2, 4097, 256), (3, 16385, 8), (2, 32000, 64), (3, 32001, 7), (2, 50257, 50), (2, 65536, 16), (2, 65537, 3),
     (1, 70001, 1024), (2, 131072, 64), (1, 200003, 33), (1, 300001, 5), (1, 310003, 1024), (300, 515, 4), (1100, 96, 6), (40, 9, 8), (7, 600, 300),
-    (3, 2050, 1000), (4, 1500, 150), (3, 3100, 40), (3, 3100, 60), (5, 1020, 223), (5, 1020, 224)])
+    (3, 2050, 1000), (4, 1500, 150), (3, 3100, 40), (3, 3100, 60), (5, 1020, 223), (5, 1020, 224),
+    (2, 5003, 9), (3, 7001, 40), (2, 12001, 8), (2, 13002, 20), (2, 18003, 6), (2, 22001, 5), (3, 26002, 7)])
 @pytest.mark.parametrize("T,tail", [(1.0, False), (2.0, True), (0.7, True), (4.0, False)])
 def test_loss_and_gradient(hip, n, c, k, T, tail):
     print("[case] distill", n, c, k, T, tail, flush=True)
