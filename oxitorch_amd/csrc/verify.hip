@@ -74,6 +74,11 @@ __device__ __forceinline__ Row row_of(const VerifyArgs& g, int64_t b, int64_t ke
   return r;
 }
 
+// A piece's weights: what the draft leaves, and the target's own.
+struct Sums {
+  double left, own;
+};
+
 template <int N>
 __device__ __forceinline__ double block_sum(double v, double* lds) {
   v = wave_sum<double>(v);
@@ -109,6 +114,36 @@ __device__ __forceinline__ double block_before(double v, double* lds, double& al
   return base + (s - v);
 }
 
+// The same of two sums at once.
+template <int N>
+__device__ __forceinline__ Sums block_before(Sums v, Sums* lds, Sums& all) {
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  Sums s = v;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const double l = __shfl_up(s.left, m, 64), o = __shfl_up(s.own, m, 64);
+    if (lane >= m) {
+      s.left += l;
+      s.own += o;
+    }
+  }
+  __syncthreads();
+  if (lane == 63) lds[wid] = s;
+  __syncthreads();
+  Sums base = {0.0, 0.0};
+  all = {0.0, 0.0};
+#pragma unroll
+  for (int i = 0; i < N / 64; ++i) {
+    if (i < wid) {
+      base.left += lds[i].left;
+      base.own += lds[i].own;
+    }
+    all.left += lds[i].left;
+    all.own += lds[i].own;
+  }
+  return {base.left + (s.left - v.left), base.own + (s.own - v.own)};
+}
+
 // ---------------------------------------------------------------------------
 // Two launches: the first cuts each sequence's row into pieces of 64 lanes x U
 // float4s, a wave a piece, which sums its weights; the second, a block a
@@ -116,14 +151,9 @@ __device__ __forceinline__ double block_before(double v, double* lds, double& al
 // one again. Each block of the first finds the row by itself (a gather of two
 // floats a draft). HBM bounds the first, behind the three dependent loads that find the
 // row: 128 sequences of 131072 classes, of which half reject a token, 100 MB in 19.8
-// us, 5.1 TB/s (a block a sequence walking its row: 810); the second takes 6.8 us
-// there, a chain of dependent loads and scans. 4 sequences of 32000: 3.5 and 4.6 us,
+// us, 5.1 TB/s (a block a sequence walking its row: 810); the second takes 5.9 us
+// there, a chain of dependent loads and scans. 4 sequences of 32000: 3.4 and 3.8 us,
 // both such chains.
-
-// A piece's weights: what the draft leaves, and the target's own.
-struct Sums {
-  double left, own;
-};
 
 template <int U>
 __global__ __launch_bounds__(NT) void verify_sums_k(const VerifyArgs g, Sums* __restrict__ part, int64_t pieces) {
@@ -197,6 +227,7 @@ template <int U>
 __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Sums* __restrict__ part, int64_t pieces) {
   static_assert(NT == 256, "a piece is 256 U classes");
   __shared__ double red[NT / 64];
+  __shared__ Sums both[NT / 64];
   __shared__ Crossing slots[NT / 64];
   __shared__ int last;
   const int64_t b = blockIdx.x;
@@ -208,19 +239,27 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
   const Row r = row_of(g, b, kept, rejected);
   const double u = (double)g.uniforms[b * (g.drafts + 1) + g.drafts];
   const Sums* pb = part + b * pieces;
-  double left = 0.0, own = 0.0;
-  for (int64_t i = t; i < pieces; i += NT) {
-    left += pb[i].left;
-    own += pb[i].own;
+  // both kinds' sums over the first NT pieces, which are all of most vocabularies
+  const Sums mine0 = t < pieces ? pb[t] : Sums{0.0, 0.0};
+  Sums total;
+  const Sums before0 = block_before<NT>(mine0, both, total);
+  const Sums first = total;
+  if (pieces > NT) {
+    double left = 0.0, own = 0.0;
+    for (int64_t i = NT + t; i < pieces; i += NT) {
+      left += pb[i].left;
+      own += pb[i].own;
+    }
+    total.left += block_sum<NT>(left, red);
+    total.own += block_sum<NT>(own, red);
   }
-  left = block_sum<NT>(left, red);
-  own = block_sum<NT>(own, red);
-  const bool use_left = rejected && left > 0.0;
-  const double limit = u * (use_left ? left : own);
+  const bool use_left = rejected && total.left > 0.0;
+  const double limit = u * (use_left ? total.left : total.own);
   // the piece
-  int64_t at = -1;
-  double base = 0.0, carry = 0.0;
-  for (int64_t i0 = 0; i0 < pieces; i0 += NT) {
+  const Crossing c0 = cross<NT>(use_left ? mine0.left : mine0.own, use_left ? before0.left : before0.own, limit, slots);
+  int64_t at = c0.at;
+  double base = c0.before, carry = use_left ? first.left : first.own;
+  for (int64_t i0 = NT; at < 0 && i0 < pieces; i0 += NT) {
     const double w = i0 + t < pieces ? (use_left ? pb[i0 + t].left : pb[i0 + t].own) : 0.0;
     double all;
     const double before = carry + block_before<NT>(w, red, all);
