@@ -333,7 +333,7 @@ __device__ __forceinline__ void write_entries(const DistillArgs& g, int64_t row,
     if (a.twice)
       for (int i = j + 1; i < g.k; ++i)
         if (a.dup[i] == j) p += a.p[i];
-    dr[id] = (float)(q(id) - p) * gscale;
+    dr[id] = (float)(q(j, id) - p) * gscale;
   }
 }
 
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(NT) void distill_fwd_k(const DistillArgs g) {
     dr[c] = some ? e * factor : 0.f;
   }
   write_entries<NT>(g, row, a, g.gscale,
-                    [&](int id) { return (double)expf((xr[id] - m) * g.inv_t) / total; });
+                    [&](int, int id) { return (double)expf((xr[id] - m) * g.inv_t) / total; });
 }
 
 // ---------------------------------------------------------------------------
@@ -710,11 +710,15 @@ __global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const fl
   const float scale = g.gscale * gloss[0];
   const float l2 = g.lse[row] * 1.4426950408889634f;
   auto prob = [&](float x) { return __builtin_amdgcn_exp2f(x * scale2 - l2); };
+  // the logit at the thread's first entry, before the row's: it is used again
+  // after its stores
+  const float x0 = t < g.k && a.id[t] >= 0 ? xr[a.id[t]] : 0.f;
+  auto at = [&](int j, int id) { return (double)prob(j == t ? x0 : xr[id]); };
   float factor = 1.f;
   if (g.top_lse && some) {
     double ql = 0.0;
     for (int j = t; j < g.k; j += N)
-      if (a.id[j] >= 0 && a.dup[j] < 0) ql += (double)prob(xr[a.id[j]]);
+      if (a.id[j] >= 0 && a.dup[j] < 0) ql += at(j, a.id[j]);
     ql = block_sum<N>(ql, red);
     factor = rest_factor(psum, ql, exp64((double)g.rest[row]));
   }
@@ -734,7 +738,7 @@ __global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const fl
   }
   const int e1 = t < 32 ? t : head + 4 * c4 + t - 32;
   if (t < 32 ? t < head : t < 35 && e1 < g.c) dr[e1] = out(xr[e1]);
-  write_entries<N>(g, row, a, scale, [&](int id) { return (double)prob(xr[id]); });
+  write_entries<N>(g, row, a, scale, at);
 }
 
 // loss[0] = sum of the rows' losses / divisor, in float64 in a fixed order: one
