@@ -690,7 +690,9 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
 // its classes as in distill_rows_k. HBM bounds it: it reads the logits once and
 // writes the gradient, (8192, 32000) in 354 us (5.9 TB/s), (16384, 16640) in 359. Four
 // float4s on 1024 threads took 393 and 509, all loads of a row before the
-// entries' work 359-366 and 376.
+// entries' work 359-366 and 376. The log-sum-exp between the passes is a float: its
+// rounding moves every q of a row by up to |lse| 2^-24 of itself, what an exponential
+// of a float argument of that size is off by anyway.
 template <int N, int U, bool NTS>
 __global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const float* __restrict__ gloss,
                                                    const float scale2) {
@@ -709,7 +711,7 @@ __global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const fl
   const double psum = load_teacher<N>(g, row, a, red, some);
   const float scale = g.gscale * gloss[0];
   const float l2 = g.lse[row] * 1.4426950408889634f;
-  auto prob = [&](float x) { return __builtin_amdgcn_exp2f(x * scale2 - l2); };
+  auto prob = [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, scale2, -l2)); };
   // the logit at the thread's first entry, before the row's: it is used again
   // after its stores
   const float x0 = t < g.k && a.id[t] >= 0 ? xr[a.id[t]] : 0.f;
