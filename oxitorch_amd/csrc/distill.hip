@@ -41,7 +41,10 @@ struct DistillArgs {
   float inv_t;
   double t;  // temperature
   float gscale;  // T / divisor
+  const float* gloss;  // the upstream gradient, NULL for 1
   int* guard;
+
+  __device__ __forceinline__ float upstream() const { return gloss ? gloss[0] : 1.f; }
 };
 
 // A row's teacher entries in LDS: class ids (-1: padding, or an id that an
@@ -312,7 +315,7 @@ __device__ __forceinline__ float finish_row(const DistillArgs& g, int64_t row, c
     s += rest_term(psum, lr, qr);
     factor = rest_factor(psum, 1.0 - qr, qr);
   }
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && g.row_loss) {
     g.row_loss[row] = some ? (float)(g.t * g.t * s) : 0.f;
     g.lse[row] = (float)((double)m / g.t + lt);
     g.rest[row] = tail ? (float)lr : 0.f;
@@ -352,7 +355,7 @@ __device__ __forceinline__ void mark_listed(const Teacher& a, int k, int c0, uin
 
 // A block a row of any length, which it walks three times: under 8 classes, and past
 // STREAM_MAX of them, where the row comes from HBM each time.
-__global__ __launch_bounds__(NT) void distill_fwd_k(const DistillArgs g) {
+__global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
   extern __shared__ __align__(16) double dyn[];
   __shared__ double red[NT / 64];
   __shared__ uint32_t bits[STRETCH / 32];
@@ -384,13 +387,13 @@ __global__ __launch_bounds__(NT) void distill_fwd_k(const DistillArgs g) {
   }
   const float factor = finish_row<NT>(g, row, a, red, psum, some, m, total, rest);
   if (!g.dx) return;
-  const float scale = (float)(1.0 / total) * g.gscale;
+  const float gscale = g.gscale * g.upstream(), scale = (float)(1.0 / total) * gscale;
   float* dr = g.dx + row * g.c;
   for (int c = t; c < g.c; c += NT) {
     const float e = expf((xr[c] - m) * g.inv_t) * scale;
     dr[c] = some ? e * factor : 0.f;
   }
-  write_entries<NT>(g, row, a, g.gscale,
+  write_entries<NT>(g, row, a, gscale,
                     [&](int, int id) { return (double)expf((xr[id] - m) * g.inv_t) / total; });
 }
 
@@ -412,6 +415,11 @@ __global__ __launch_bounds__(NT) void distill_fwd_k(const DistillArgs g) {
 // it), and behind it where a block has the CU to itself ((4096, 50257) 301 us
 // before it, 288 behind) or four share it ((4096, 8192) with the rest's term 56
 // and 53).
+//
+// The backward for an upstream scalar is the same pass without the loss (no
+// row_loss): (8192, 32000) 359-368 us. From a log-sum-exp rounded to a float every
+// probability of a row would be off by up to |lse| 2^-24 of itself: 6e-4 at logits near
+// 10^4, where these are off by 2e-6.
 //
 // NV = 0: longer rows, streamed twice, the first time with a running maximum; the
 // second time they come from the Infinity Cache (a block a row on every CU is
@@ -472,6 +480,9 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   auto x4 = [&](int c) -> const f4* {
     return reinterpret_cast<const f4*>(reinterpret_cast<const char*>(xr + head) + (uint32_t)c * 16u);
   };
+  // used after the row's sums: nothing waits for it before (a wait here, 366
+  // to 393 us backward at (16384, 16640))
+  const float up = GRAD ? g.upstream() : 1.f;
   // the entries' loads go first (a thread's first one; the rest of long lists
   // later): a wait for them leaves the row's in flight, if those are
   const int64_t id0 = t < g.k ? g.ids[row * g.k + t] : -1;
@@ -629,8 +640,9 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
       if constexpr (NTS) __builtin_nontemporal_store(d, p);
       else *p = d;
     };
+    const float gscale = g.gscale * up;
     if (some) {
-      float gs = g.gscale / total;
+      float gs = gscale / total;
       // (qr - pr) / qr, from the entries' masses where those are the smaller
       if constexpr (TAIL)
         if (rest > 0.f || rest != rest)
@@ -664,8 +676,9 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
         for (int i = j + 1; i < g.k; ++i)
           if (eid[i] == -2 - id) p += ep[i];
       const float eq = __builtin_amdgcn_exp2f((ex[j] - m) * scale2);
-      dr[id] = (float)((double)eq / (double)total - p) * g.gscale;
+      dr[id] = (float)((double)eq / (double)total - p) * gscale;
     }
+    if (!g.row_loss) return;
   }
   const double lt = log64((double)total);
   double terms = 0.0;
@@ -683,64 +696,6 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     g.lse[row] = (float)((double)m / g.t + lt);
     g.rest[row] = (float)lr;
   }
-}
-
-// The gradient from the forward's log-sum-exp and rest, for an upstream scalar: a
-// block a row, U float4s in flight a thread, as many as hold it up to 32768 classes,
-// its classes as in distill_rows_k. HBM bounds it: it reads the logits once and
-// writes the gradient, (8192, 32000) in 354 us (5.9 TB/s), (16384, 16640) in 359. Four
-// float4s on 1024 threads took 393 and 509, all loads of a row before the
-// entries' work 359-366 and 376. The log-sum-exp between the passes is a float: its
-// rounding moves every q of a row by up to |lse| 2^-24 of itself, what an exponential
-// of a float argument of that size is off by anyway.
-template <int N, int U, bool NTS>
-__global__ __launch_bounds__(N) void distill_bwd_k(const DistillArgs g, const float* __restrict__ gloss,
-                                                   const float scale2) {
-  extern __shared__ __align__(16) double dyn[];
-  __shared__ double red[N / 64];
-  Teacher a = teacher_at(dyn, g.k);
-  const int t = threadIdx.x;
-  const int64_t row = blockIdx.x;
-  const float* xr = g.x + row * g.c;
-  float* dr = g.dx + row * g.c;
-  const int head = min(row_head(xr, g.c), g.c);
-  const int c4 = (g.c - head) >> 2;
-  const f4* x4 = reinterpret_cast<const f4*>(xr + head);
-  f4u* d4 = reinterpret_cast<f4u*>(dr + head);
-  bool some;
-  const double psum = load_teacher<N>(g, row, a, red, some);
-  const float scale = g.gscale * gloss[0];
-  const float l2 = g.lse[row] * 1.4426950408889634f;
-  auto prob = [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, scale2, -l2)); };
-  // the logit at the thread's first entry, before the row's: it is used again
-  // after its stores
-  const float x0 = t < g.k && a.id[t] >= 0 ? xr[a.id[t]] : 0.f;
-  auto at = [&](int j, int id) { return (double)prob(j == t ? x0 : xr[id]); };
-  float factor = 1.f;
-  if (g.top_lse && some) {
-    double ql = 0.0;
-    for (int j = t; j < g.k; j += N)
-      if (a.id[j] >= 0 && a.dup[j] < 0) ql += at(j, a.id[j]);
-    ql = block_sum<N>(ql, red);
-    factor = rest_factor(psum, ql, exp64((double)g.rest[row]));
-  }
-  const float gs = scale * factor;
-  auto out = [&](float x) { return some ? prob(x) * gs : 0.f; };
-  for (int c0 = t; c0 < c4; c0 += U * N) {
-    f4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = ld_stream(x4 + min(c0 + u * N, c4 - 1));
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (c0 + u * N >= c4) continue;
-      const f4 d = {out(v[u].x), out(v[u].y), out(v[u].z), out(v[u].w)};
-      if constexpr (NTS) __builtin_nontemporal_store(d, d4 + c0 + u * N);
-      else d4[c0 + u * N] = d;
-    }
-  }
-  const int e1 = t < 32 ? t : head + 4 * c4 + t - 32;
-  if (t < 32 ? t < head : t < 35 && e1 < g.c) dr[e1] = out(xr[e1]);
-  write_entries<N>(g, row, a, scale, at);
 }
 
 // loss[0] = sum of the rows' losses / divisor, in float64 in a fixed order: one
@@ -827,6 +782,12 @@ bool launch_rows_any(const DistillArgs& g) {
   return g.top_lse ? launch_rows<false, true, false>(g) : launch_rows<false, false, false>(g);
 }
 
+void launch_any(const DistillArgs& g) {
+  const bool nt = nt_stream_stores(g.n * g.c * 4);
+  if (!(nt ? launch_rows_any<true>(g) : launch_rows_any<false>(g)))
+    distill_loop_k<<<dim3((unsigned)g.n), dim3(NT), teacher_bytes(g.k), stream()>>>(g);
+}
+
 }  // namespace
 }  // namespace oxi
 
@@ -843,11 +804,11 @@ int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, c
     return fail(OXI_INVALID_ARGUMENT, "distill_fwd: NULL tensor pointer");
   OXI_CHECK_INIT();
   if (n == 0) return oxi_fill(loss, 1, 0.f);
-  const DistillArgs g{logits, ids,    top, top_lse, row_loss,           lse,         rest, dlogits, n, (int)c,
-                      (int)k, 1.0f / temperature, (double)temperature, temperature / divisor, guard_flag()};
-  const bool nt = nt_stream_stores(n * c * 4);
-  if (!(nt ? launch_rows_any<true>(g) : launch_rows_any<false>(g)))
-    distill_fwd_k<<<dim3((unsigned)n), dim3(NT), teacher_bytes(k), stream()>>>(g);
+  const DistillArgs g{logits,  ids,    top,    top_lse,
+                      row_loss, lse,    rest,   dlogits,
+                      n,        (int)c, (int)k, 1.0f / temperature,
+                      (double)temperature, temperature / divisor, nullptr, guard_flag()};
+  launch_any(g);
   if (int rc = check_launch("distill_fwd")) return rc;
   distill_mean_k<<<1, 1024, 0, stream()>>>(row_loss, n, (double)divisor, loss);
   return check_launch("distill_fwd: mean");
@@ -861,30 +822,11 @@ int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, c
   if (!logits || !ids || !top || !lse || !rest || !gloss || !dlogits)
     return fail(OXI_INVALID_ARGUMENT, "distill_bwd: NULL tensor pointer");
   OXI_CHECK_INIT();
-  const DistillArgs g{logits, ids,    top, top_lse, nullptr, const_cast<float*>(lse), const_cast<float*>(rest), dlogits, n,
-                      (int)c, (int)k, 1.0f / temperature, (double)temperature, temperature / divisor, guard_flag()};
-  const float scale2 = (float)(1.4426950408889634 / g.t);
-  const dim3 grid((unsigned)n);
-  const size_t lds = teacher_bytes(k);
-  const bool nt = nt_stream_stores(n * c * 4);
-#define OXI_DB(N, U)                                                                           \
-  {                                                                                            \
-    if (nt) distill_bwd_k<N, U, true><<<grid, dim3(N), lds, stream()>>>(g, gloss, scale2);     \
-    else distill_bwd_k<N, U, false><<<grid, dim3(N), lds, stream()>>>(g, gloss, scale2);       \
-  }
-  if (c + 6 * k <= 2400) {  // one wave: (16384, 512) with 8 and 500 entries 19 and 104 us against 47 and 70
-    if (c <= 1024) OXI_DB(64, 4)
-    else OXI_DB(64, 8)
-  } else if (c <= 4096) OXI_DB(256, 4)
-  else if (c <= 6144) OXI_DB(256, 6)
-  else if (c <= 8192) OXI_DB(256, 8)
-  else if (c <= 12288) OXI_DB(256, 12)
-  else if (c <= 16384) OXI_DB(256, 16)
-  else if (c <= 20480) OXI_DB(512, 10)
-  else if (c <= 24576) OXI_DB(512, 12)
-  else if (c <= 28672) OXI_DB(512, 14)
-  else OXI_DB(512, 16)
-#undef OXI_DB
+  const DistillArgs g{logits,  ids,     top,    top_lse,
+                      nullptr, nullptr, nullptr, dlogits,
+                      n,       (int)c,  (int)k, 1.0f / temperature,
+                      (double)temperature, temperature / divisor, gloss, guard_flag()};
+  launch_any(g);
   return check_launch("distill_bwd");
 }
 
