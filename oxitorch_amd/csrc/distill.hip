@@ -11,8 +11,10 @@
 // row: a student near its teacher has a small loss of terms that cancel. With
 // the rest's term both sides' masses are 1, and the row is summed as
 // q - p + p log(p/q), each of which is >= 0, so that an error of lse enters
-// squared. qr is the sum over the classes that are not listed, never 1 minus
-// the listed.
+// squared. qr is a sum over the classes that are not listed, never 1 minus the
+// listed, and those have a maximum of their own: s = softmax over them and log qr are
+// there where qr itself is below the smallest float, and their gradient is
+// T/divisor s (qr - pr).
 #include <cmath>
 
 #include "internal.h"
@@ -169,6 +171,19 @@ struct AddF32 {
 struct MaxF32 : AddF32 {
   __device__ __forceinline__ static T op(T a, T b) { return fmaxf(a, b); }
 };
+// The same of two values at once.
+struct Two {
+  float a, b;
+};
+template <class R>
+struct Both {
+  typedef Two T;
+  __device__ __forceinline__ static T op(T x, T y) { return {R::op(x.a, y.a), R::op(x.b, y.b)}; }
+  template <int C> __device__ __forceinline__ static T move(T v) {
+    return {R::template move<C>(v.a), R::template move<C>(v.b)};
+  }
+  __device__ __forceinline__ static T lane(T v, int l) { return {R::lane(v.a, l), R::lane(v.b, l)}; }
+};
 template <int N, class R>
 __device__ __forceinline__ typename R::T over_block(typename R::T v, typename R::T* slots) {
   v = R::op(v, R::template move<DPP_QUAD_XOR1>(v));
@@ -279,48 +294,20 @@ __device__ __forceinline__ double entry_term(double p, double lp, double lq, boo
 // What entries of sum psum leave to the other classes.
 __device__ __forceinline__ double rest_of(double psum) { return psum < 1.0 ? 1.0 - psum : psum != psum ? psum : 0.0; }
 
-// The rest's share, lr the logarithm of the student's mass qr there, with what the
-// masses as rounded lack of 1.
-__device__ __forceinline__ double rest_term(double psum, double lr, double qr) {
-  const double pr = rest_of(psum), d = lr - log64(pr);
-  return (pr > 0.0 || pr != pr ? pr * exp_rest(d) : qr) + ((psum + pr) - 1.0);
+// The rest's share, lr the logarithm of the student's mass there, with what the
+// masses as rounded lack of 1. Where no class that is not listed has a finite logit
+// (lr = -inf) a rest of the size that rounding leaves in a log-sum-exp worked out in
+// 32 bits (4 steps of it and of 1) is none: not an infinite loss.
+__device__ __forceinline__ double rest_term(double psum, double lr, float top_lse) {
+  double pr = rest_of(psum);
+  if (lr == (double)NEG_INF && pr <= 0x1p-22 * (1.0 + fabs((double)top_lse))) pr = 0.0;
+  return (pr > 0.0 || pr != pr ? pr * exp_rest(lr - log64(pr)) : exp64(lr)) + ((psum + pr) - 1.0);
 }
 
-// (qr - pr) / qr, the factor of q at the classes not listed: from the masses ql
-// and psum of the listed ones where those are the smaller, 1 where nothing is
-// left to share.
-__device__ __forceinline__ float rest_factor(double psum, double ql, double qr) {
-  if (!(qr > 0.0) && qr == qr) return 1.f;
-  return (float)((psum < 0.5 ? psum - ql : qr - rest_of(psum)) / qr);
-}
-
-// The loss of the row once its maximum, its sum of exp((x - m)/T) and, with
-// the rest's term, the sum over the classes not listed are known; thread 0 writes
-// the row's results. Returns the factor of q at the classes not listed.
-template <int N>
-__device__ __forceinline__ float finish_row(const DistillArgs& g, int64_t row, const Teacher& a, double* red,
-                                            double psum, bool some, float m, double total, double rest) {
-  const bool tail = g.top_lse != nullptr;
-  const double lt = log64(total);
-  const float* xr = g.x + row * g.c;
-  double s = 0.0;
-  for (int j = threadIdx.x; j < g.k; j += N)
-    if (a.id[j] >= 0)
-      s += entry_term(a.p[j], a.lp[j], ((double)xr[a.id[j]] - (double)m) / g.t - lt, tail, a.dup[j] >= 0);
-  s = block_sum<N>(s, red);
-  float factor = 1.f;
-  const double lr = tail ? log64(rest) - lt : 0.0;
-  if (tail && some) {
-    const double qr = rest / total;
-    s += rest_term(psum, lr, qr);
-    factor = rest_factor(psum, 1.0 - qr, qr);
-  }
-  if (threadIdx.x == 0 && g.row_loss) {
-    g.row_loss[row] = some ? (float)(g.t * g.t * s) : 0.f;
-    g.lse[row] = (float)((double)m / g.t + lt);
-    g.rest[row] = tail ? (float)lr : 0.f;
-  }
-  return some ? factor : 0.f;
+// qr - pr, from the masses ql and psum of the listed classes where those are the smaller.
+template <class F>
+__device__ __forceinline__ F rest_excess(F psum, F ql, F qr, F pr) {
+  return psum < (F)0.5 ? psum - ql : qr - pr;
 }
 
 // The gradient at the row's entries, after the block has written the row as if
@@ -353,8 +340,9 @@ __device__ __forceinline__ void mark_listed(const Teacher& a, int k, int c0, uin
   __syncthreads();
 }
 
-// A block a row of any length, which it walks three times: under 8 classes, and past
-// STREAM_MAX of them, where the row comes from HBM each time.
+// A block a row of any length, which it walks twice, the first time with a running
+// maximum: under 8 classes, and past STREAM_MAX of them, where the row comes from
+// HBM each time.
 __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
   extern __shared__ __align__(16) double dyn[];
   __shared__ double red[NT / 64];
@@ -362,37 +350,67 @@ __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
   Teacher a = teacher_at(dyn, g.k);
   const int t = threadIdx.x;
   const int64_t row = blockIdx.x;
+  const bool tail = g.top_lse != nullptr;
   const float* xr = g.x + row * g.c;
   bool some;
   const double psum = load_teacher<NT>(g, row, a, red, some);
-  float m = NEG_INF;
-  for (int c = t; c < g.c; c += NT) m = fmaxf(m, xr[c]);
-  m = group_max<NT>(m, reinterpret_cast<float*>(red));
-  double total = 0.0, listed = 0.0, rest = 0.0;
-  if (g.top_lse) {
-    for (int c0 = 0; c0 < g.c; c0 += STRETCH) {
-      mark_listed<NT>(a, g.k, c0, bits);
-      const int end = min(g.c - c0, STRETCH);
-      for (int c = t; c < end; c += NT) {
-        const double e = expf((xr[c0 + c] - m) * g.inv_t);
-        if (bits[c >> 5] >> (c & 31) & 1) listed += e;
-        else rest += e;
+  // maximum and sum over the classes not listed (without the rest's term over all)
+  float mr = NEG_INF;
+  double sum = 0.0;
+  for (int c0 = 0; c0 < g.c; c0 += STRETCH) {
+    if (tail) mark_listed<NT>(a, g.k, c0, bits);
+    const int end = min(g.c - c0, STRETCH);
+    for (int c = t; c < end; c += NT) {
+      if (tail && (bits[c >> 5] >> (c & 31) & 1)) continue;
+      const float v = xr[c0 + c];
+      if (v > mr) {
+        sum *= expf((mr - v) * g.inv_t);
+        mr = v;
       }
+      sum += expf((v - (mr == NEG_INF ? 0.f : mr)) * g.inv_t);
     }
-    rest = block_sum<NT>(rest, red);
-    total = rest + block_sum<NT>(listed, red);
-  } else {
-    for (int c = t; c < g.c; c += NT) total += expf((xr[c] - m) * g.inv_t);
-    total = block_sum<NT>(total, red);
   }
-  const float factor = finish_row<NT>(g, row, a, red, psum, some, m, total, rest);
+  const float own = mr;
+  mr = group_max<NT>(mr, reinterpret_cast<float*>(red));
+  if (own != NEG_INF) sum *= expf((own - mr) * g.inv_t);
+  sum = block_sum<NT>(sum, red);
+  // and the listed ones
+  float ml = NEG_INF;
+  double listed = 0.0;
+  if (tail) {
+    for (int j = t; j < g.k; j += NT)
+      if (a.id[j] >= 0) ml = fmaxf(ml, xr[a.id[j]]);
+    ml = group_max<NT>(ml, reinterpret_cast<float*>(red));
+  }
+  const float m = fmaxf(mr, ml);
+  if (tail) {
+    for (int j = t; j < g.k; j += NT)
+      if (a.id[j] >= 0 && a.dup[j] < 0) listed += expf((xr[a.id[j]] - m) * g.inv_t);
+    listed = block_sum<NT>(listed, red);
+  }
+  const double below = ((double)mr - (double)m) / g.t;  // the rest's maximum from the row's
+  const double total = tail ? sum * exp64(below) + listed : sum;
+  const double lt = log64(total), lr = log64(sum) + below - lt;
+  if (g.row_loss) {
+    double s = 0.0;
+    for (int j = t; j < g.k; j += NT)
+      if (a.id[j] >= 0)
+        s += entry_term(a.p[j], a.lp[j], ((double)xr[a.id[j]] - (double)m) / g.t - lt, tail, a.dup[j] >= 0);
+    s = block_sum<NT>(s, red);
+    if (tail && some) s += rest_term(psum, lr, g.top_lse[row]);
+    if (t == 0) {
+      g.row_loss[row] = some ? (float)(g.t * g.t * s) : 0.f;
+      g.lse[row] = (float)((double)m / g.t + lt);
+      g.rest[row] = tail ? (float)lr : 0.f;
+    }
+  }
   if (!g.dx) return;
-  const float gscale = g.gscale * g.upstream(), scale = (float)(1.0 / total) * gscale;
+  const float gscale = g.gscale * g.upstream();
+  double share = tail ? rest_excess(psum, listed / total, exp64(lr), rest_of(psum)) : 1.0;
+  share = sum > 0.0 || sum != sum ? share / sum : 0.0;
+  const float scale = (float)share * gscale, shift = tail && mr == NEG_INF ? 0.f : mr;
   float* dr = g.dx + row * g.c;
-  for (int c = t; c < g.c; c += NT) {
-    const float e = expf((xr[c] - m) * g.inv_t) * scale;
-    dr[c] = some ? e * factor : 0.f;
-  }
+  for (int c = t; c < g.c; c += NT) dr[c] = some ? expf((xr[c] - shift) * g.inv_t) * scale : 0.f;
   write_entries<NT>(g, row, a, gscale,
                     [&](int, int id) { return (double)expf((xr[id] - m) * g.inv_t) / total; });
 }
@@ -428,8 +446,11 @@ __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
 constexpr int STREAM_U = 4;         // float4s in flight a thread
 constexpr int STREAM_MAX = 300000;  // classes whose bitmap fits in LDS beside 1024 entries
 
-// Waves a SIMD that the registers must allow: 4 with 128 a lane, 8 with 64.
+// Waves a SIMD that the registers must allow: 4 with 128 a lane, 8 with 64; and at
+// most, so that rows written as they are read do not crowd each other out: a third
+// block of 512 threads or a fifth of 256 a CU took (16384, 16640) from 365 to 393 us.
 constexpr int rows_waves(int nv) { return nv ? 4 : 8; }
+constexpr int rows_waves_most(bool grad, int nv) { return grad && nv >= 10 ? 4 : 8; }
 
 __device__ __forceinline__ f4 exp2_4(const f4& z) {
   return f4{__builtin_amdgcn_exp2f(z.x), __builtin_amdgcn_exp2f(z.y), __builtin_amdgcn_exp2f(z.z),
@@ -455,10 +476,10 @@ __device__ __forceinline__ f4 without(const f4& v, uint32_t bits) {
 }
 
 template <int RT, int NV, bool GRAD, bool TAIL, bool NTS>
-__global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(NV)))) void distill_rows_k(
+__global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(NV), rows_waves_most(GRAD, NV)))) void distill_rows_k(
     const DistillArgs g, const float scale2) {
   __shared__ double red[RT / 64], psum_at;
-  __shared__ float lds[4 * (RT / 64)];
+  __shared__ __align__(8) float lds[4 * (RT / 64)];
   __shared__ int twice;
   // k probabilities, k logarithms of them, k ids (-1: padding, -2 - id: an id
   // that an earlier entry has), the student's logits there, a bit a class
@@ -580,24 +601,38 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   if constexpr (RT != 512) load_row();
   auto listed = [&](int c) -> uint32_t { return TAIL ? bits[(c >> 3) + 1] >> ((c & 7) * 4) & 15u : 0u; };
   if (TAIL && has1 && (bits[(e1 + 32 - head) >> 5] >> ((e1 + 32 - head) & 31) & 1u)) v1 = NEG_INF;
-  float m = NEG_INF, s = 0.f;
+  // The maximum mr and the sum of exponentials of the classes not listed (without
+  // the rest's term: of all), then the row's maximum m and its sum `total`.
+  float mr = NEG_INF, m, s = 0.f;
+  auto maxima = [&]() {
+    mr = fmaxf(mr, v1);
+    if constexpr (TAIL) {
+      float ml = NEG_INF;
 #pragma unroll 1
-  for (int j = t; j < g.k; j += RT) m = fmaxf(m, ex[j]);
+      for (int j = t; j < g.k; j += RT) ml = fmaxf(ml, ex[j]);
+      const Two both = over_block<RT, Both<MaxF32>>(Two{mr, ml}, reinterpret_cast<Two*>(lds));
+      mr = both.a;
+      m = fmaxf(both.a, both.b);
+    } else {
+      m = mr = over_block<RT, MaxF32>(mr, lds + RT / 64);
+    }
+  };
+  // what logits are taken relative to; with nothing finite there, their exponentials are 0
+  auto shift_of = [&](float top) { return TAIL && top == NEG_INF ? 0.f : top; };
   if constexpr (NV > 0) {
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
       const int c = q * RT + t;
       v[q] = without(v[q], c < c4 ? listed(c) : 15u);
-      m = fmaxf(m, max4(v[q]));
+      mr = fmaxf(mr, max4(v[q]));
     }
-    m = over_block<RT, MaxF32>(fmaxf(m, v1), lds + RT / 64);
+    maxima();
+    const float shift = shift_of(mr);
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
-      v[q] = exp2_4((v[q] - m) * scale2);
+      v[q] = exp2_4((v[q] - shift) * scale2);
       s += sum4(v[q]);
     }
-    v1 = __builtin_amdgcn_exp2f((v1 - m) * scale2);
-    s += v1;
   } else {
     for (int c0 = t; c0 < c4; c0 += STREAM_U * RT) {
       f4 r[STREAM_U];
@@ -610,28 +645,33 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
         r[u] = without(r[u], c < c4 ? listed(c) : 15u);
         cm = fmaxf(cm, max4(r[u]));
       }
-      if (cm > m) {
-        s *= __builtin_amdgcn_exp2f((m - cm) * scale2);
-        m = cm;
+      if (cm > mr) {
+        s *= __builtin_amdgcn_exp2f((mr - cm) * scale2);
+        mr = cm;
       }
-      const float ms = m == NEG_INF ? 0.f : m;
+      const float ms = mr == NEG_INF ? 0.f : mr;
 #pragma unroll
       for (int u = 0; u < STREAM_U; ++u) s += sum4(exp2_4((r[u] - ms) * scale2));
     }
-    const float own = m;
-    m = over_block<RT, MaxF32>(fmaxf(m, v1), lds + RT / 64);
-    s *= own == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((own - m) * scale2);
-    v1 = __builtin_amdgcn_exp2f((v1 - m) * scale2);
-    s += v1;
+    const float own = mr;
+    maxima();
+    s *= own == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((own - mr) * scale2);
   }
-  const float rest = over_block<RT, AddF32>(s, lds + 2 * (RT / 64));
-  float total = rest, mine = 0.f;
+  const float shift = shift_of(mr);
+  v1 = __builtin_amdgcn_exp2f((v1 - shift) * scale2);
+  s += v1;
+  float total, mine = 0.f, above = 0.f;  // the row's mass; the listed classes' and the others' parts of it
   if constexpr (TAIL) {
 #pragma unroll 1
     for (int j = t; j < g.k; j += RT)
       if (eid[j] >= 0) mine += __builtin_amdgcn_exp2f((ex[j] - m) * scale2);
-    mine = over_block<RT, AddF32>(mine, lds + 3 * (RT / 64));
-    total += mine;
+    const Two both = over_block<RT, Both<AddF32>>(Two{s, mine}, reinterpret_cast<Two*>(lds + 2 * (RT / 64)));
+    s = both.a;
+    mine = both.b;
+    above = s * __builtin_amdgcn_exp2f((mr - m) * scale2);
+    total = above + mine;
+  } else {
+    total = s = over_block<RT, AddF32>(s, lds + 2 * (RT / 64));
   }
   if constexpr (GRAD) {
     float* const dr = g.dx + row * C;
@@ -642,11 +682,9 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     };
     const float gscale = g.gscale * up;
     if (some) {
-      float gs = gscale / total;
-      // (qr - pr) / qr, from the entries' masses where those are the smaller
-      if constexpr (TAIL)
-        if (rest > 0.f || rest != rest)
-          gs *= (psumf < 0.5f ? psumf - mine / total : rest / total - prf) * (total / rest);
+      float gs = gscale / s;
+      if constexpr (TAIL)  // s is 1 or more where any of its classes has a finite logit
+        gs = s > 0.f || s != s ? gs * rest_excess(psumf, mine / total, above / total, prf) : 0.f;
       if constexpr (NV > 0) {
 #pragma unroll
         for (int q = 0; q < NV; ++q)
@@ -658,7 +696,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
           for (int u = 0; u < STREAM_U; ++u) r[u] = ld_stream(x4(min(c0 + u * RT, c4 - 1)));
 #pragma unroll
           for (int u = 0; u < STREAM_U; ++u)
-            if (c0 + u * RT < c4) put(exp2_4((r[u] - m) * scale2) * gs, c0 + u * RT);
+            if (c0 + u * RT < c4) put(exp2_4((r[u] - shift) * scale2) * gs, c0 + u * RT);
         }
       }
       if (has1) dr[e1] = v1 * gs;
@@ -689,8 +727,8 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   if (t == 0) {
     double lr = 0.0;
     if constexpr (TAIL) {
-      lr = log64((double)rest) - lt;
-      if (some) terms += rest_term(psum_at, lr, (double)rest / (double)total);
+      lr = log64((double)s) + ((double)mr - (double)m) / g.t - lt;
+      if (some) terms += rest_term(psum_at, lr, tlse);
     }
     g.row_loss[row] = some ? (float)(g.t * g.t * terms) : 0.f;
     g.lse[row] = (float)((double)m / g.t + lt);
