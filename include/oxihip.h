@@ -423,8 +423,8 @@ int oxi_cross_entropy_fwd_grad(const float* logits, const int64_t* targets, floa
  * row_loss (n) = T^2 row; loss (1 float) = sum of row_loss / divisor, summed
  * in 64 bits in a fixed order (n for the plain mean, the count of rows that
  * hold entries for padded batches). An id given twice counts with both entries.
- * `lse` (n, log sum exp(logits/T)) and `rest` (n, log qr; 0 without top_lse)
- * go to the backward. With `dlogits` (n, c) set, the same pass also
+ * `lse` (n, log sum exp(logits/T)) and `rest` (n: log qr, or 0 without top_lse,
+ * with what lse lost to its rounding) go to the backward. With `dlogits` (n, c) set, the same pass also
  * writes the gradient for an upstream gradient of 1: T/divisor times q - p
  * at the listed classes and q (1 - pr/qr) at the others (q without top_lse).
  * 1 <= k <= OXI_DISTILL_MAX_TOP. An id >= c raises the device guard flag
@@ -433,8 +433,9 @@ int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, c
                     float* row_loss, float* lse, float* rest, float* dlogits, int64_t n, int64_t c, int64_t k,
                     float temperature, float divisor);
 /* dlogits for the upstream scalar gradient gloss[0] (device): the forward's
- * dlogits times it, of the same accuracy, given the forward's lse and rest. The
- * rows' sums are formed again. */
+ * dlogits times it, of the same accuracy. lse and rest are the forward's, from the
+ * same logits, entries and temperature: rows of up to 65536 classes form their
+ * sums again, longer ones may take them from there. */
 int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, const float* top_lse,
                     const float* lse, const float* rest, const float* gloss, float* dlogits, int64_t n, int64_t c,
                     int64_t k, float temperature, float divisor);

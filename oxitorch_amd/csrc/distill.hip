@@ -304,6 +304,16 @@ __device__ __forceinline__ double rest_term(double psum, double lr, float top_ls
   return (pr > 0.0 || pr != pr ? pr * exp_rest(lr - log64(pr)) : exp64(lr)) + ((psum + pr) - 1.0);
 }
 
+// A row's results: its loss, its log-sum-exp and the logarithm lr of the student's
+// mass at the classes not listed, from the log-sum-exp as stored.
+__device__ __forceinline__ void write_row(const DistillArgs& g, int64_t row, bool some, double terms, double lse,
+                                          double lr) {
+  const float l = (float)lse;
+  g.row_loss[row] = some ? (float)(g.t * g.t * terms) : 0.f;
+  g.lse[row] = l;
+  g.rest[row] = (float)(lr + (lse - (double)l));
+}
+
 // qr - pr, from the masses ql and psum of the listed classes where those are the smaller.
 template <class F>
 __device__ __forceinline__ F rest_excess(F psum, F ql, F qr, F pr) {
@@ -399,9 +409,7 @@ __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
     s = block_sum<NT>(s, red);
     if (tail && some) s += rest_term(psum, lr, g.top_lse[row]);
     if (t == 0) {
-      g.row_loss[row] = some ? (float)(g.t * g.t * s) : 0.f;
-      g.lse[row] = (float)((double)m / g.t + lt);
-      g.rest[row] = tail ? (float)lr : 0.f;
+      write_row(g, row, some, s, (double)m / g.t + lt, tail ? lr : 0.0);
     }
   }
   if (!g.dx) return;
@@ -437,7 +445,8 @@ __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
 // The backward for an upstream scalar is the same pass without the loss (no
 // row_loss): (8192, 32000) 359-368 us. From a log-sum-exp rounded to a float every
 // probability of a row would be off by up to |lse| 2^-24 of itself: 6e-4 at logits near
-// 10^4, where these are off by 2e-6.
+// 10^4, where these are off by 2e-6. Rows that no registers hold take the two floats lse
+// and rest instead of a pass for their sums ((1500, 100001) 229 us, 261 with it).
 //
 // NV = 0: longer rows, streamed twice, the first time with a running maximum; the
 // second time they come from the Infinity Cache (a block a row on every CU is
@@ -604,8 +613,9 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   // The maximum mr and the sum of exponentials of the classes not listed (without
   // the rest's term: of all), then the row's maximum m and its sum `total`.
   float mr = NEG_INF, m, s = 0.f;
+  bool known = false;
   auto maxima = [&]() {
-    mr = fmaxf(mr, v1);
+    if (!known) mr = fmaxf(mr, v1);
     if constexpr (TAIL) {
       float ml = NEG_INF;
 #pragma unroll 1
@@ -634,7 +644,20 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
       s += sum4(v[q]);
     }
   } else {
-    for (int c0 = t; c0 < c4; c0 += STREAM_U * RT) {
+    if (GRAD && !g.row_loss) {
+      // The backward has them from the forward: relative to the float next to
+      // their log-sum-exp. A rest of up to 16 is off by 2^-21; rows with more
+      // below the listed classes (or NaN) are read again.
+      const float off = g.rest[row];
+      const double at = (double)g.lse[row] + (double)off;
+      const float top = (float)(at * g.t);
+      known = fabsf(off) <= 16.f && fabsf(top) < -NEG_INF;
+      if (known) {
+        mr = top;
+        s = t == 0 ? (float)exp64(at - (double)top / g.t) : 0.f;
+      }
+    }
+    for (int c0 = known ? c4 : t; c0 < c4; c0 += STREAM_U * RT) {
       f4 r[STREAM_U];
 #pragma unroll
       for (int u = 0; u < STREAM_U; ++u) r[u] = *x4(min(c0 + u * RT, c4 - 1));  // plain: the row is read again
@@ -659,7 +682,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   }
   const float shift = shift_of(mr);
   v1 = __builtin_amdgcn_exp2f((v1 - shift) * scale2);
-  s += v1;
+  if (!known) s += v1;
   float total, mine = 0.f, above = 0.f;  // the row's mass; the listed classes' and the others' parts of it
   if constexpr (TAIL) {
 #pragma unroll 1
@@ -730,9 +753,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
       lr = log64((double)s) + ((double)mr - (double)m) / g.t - lt;
       if (some) terms += rest_term(psum_at, lr, tlse);
     }
-    g.row_loss[row] = some ? (float)(g.t * g.t * terms) : 0.f;
-    g.lse[row] = (float)((double)m / g.t + lt);
-    g.rest[row] = (float)lr;
+    write_row(g, row, some, terms, (double)m / g.t + lt, lr);
   }
 }
 
@@ -861,7 +882,7 @@ int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, c
     return fail(OXI_INVALID_ARGUMENT, "distill_bwd: NULL tensor pointer");
   OXI_CHECK_INIT();
   const DistillArgs g{logits,  ids,     top,    top_lse,
-                      nullptr, nullptr, nullptr, dlogits,
+                      nullptr, const_cast<float*>(lse), const_cast<float*>(rest), dlogits,
                       n,       (int)c,  (int)k, 1.0f / temperature,
                       (double)temperature, temperature / divisor, gloss, guard_flag()};
   launch_any(g);
