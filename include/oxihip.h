@@ -454,7 +454,8 @@ int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, c
  * uniforms[i] * draft[i][token] < target[i][token]. After the first that is
  * not, position j, one more token is drawn from max(target[j] - draft[j], 0),
  * or, after all of them, from target[j]: the lowest id whose running sum of
- * weights is more than uniforms[drafts] times their total (sums in 64 bits).
+ * weights is more than uniforms[drafts] times their total (sums in 64 bits),
+ * and the highest with weight for a number that is not below 1.
  * Where max(target - draft, 0) has no weight, target[j] is drawn from; a row
  * without weight there gives -1. Probabilities need not sum to 1; a NaN or
  * negative one weighs nothing. Outputs: accepted (batch), the number kept;

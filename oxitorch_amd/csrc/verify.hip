@@ -254,7 +254,8 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
     total.own += block_sum<NT>(own, red);
   }
   const bool use_left = rejected && total.left > 0.0;
-  const double limit = u * (use_left ? total.left : total.own);
+  // a number that is not below 1 draws the last class, whatever the sums' roundings
+  double limit = u < 1.0 ? u * (use_left ? total.left : total.own) : (double)__builtin_huge_valf();
   // the piece
   const Crossing c0 = cross<NT>(use_left ? mine0.left : mine0.own, use_left ? before0.left : before0.own, limit, slots);
   int64_t at = c0.at;
@@ -280,7 +281,7 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
       __syncthreads();
       if (last >= 0) at = i0 + last;
     }
-    base = carry;  // past every limit: the last class with weight is wanted
+    limit = (double)__builtin_huge_valf();  // in it the last class with weight, not the first past the limit
   }
   int64_t token = -1;
   if (at >= 0) {

@@ -291,6 +291,17 @@ def distillation_loss(logits, teacher_ids, teacher_logits, temperature=1.0, teac
 
 # ---- serving: drafted tokens ------------------------------------------------------------
 
+def _uniforms(u):
+    """Numbers in [0, 1) as float32: a tensor as it is; those of an array, checked, and kept below 1 where their
+    rounding reaches it."""
+    if isinstance(u, _native.Tensor):
+        return u
+    a = np.asarray(u)
+    if not ((a >= 0) & (a < 1)).all():
+        raise ValueError("uniforms must lie in [0, 1)")
+    return _native_from_numpy(np.minimum(a.astype(np.float32), np.float32(1 - 2.0 ** -24)))
+
+
 def verify_drafts(draft_tokens, draft_probs, target_probs, uniforms, lengths=None):
     """Which of the tokens that a small model drafted are kept, so that what is
     kept is distributed as the large model's own samples.
@@ -299,7 +310,7 @@ def verify_drafts(draft_tokens, draft_probs, target_probs, uniforms, lengths=Non
     each was drawn from, or None for drafts without probabilities (a lookup, a
     greedy model); `target_probs` (batch, k + 1, classes): the large model's,
     after 0, 1, .. k of them; `uniforms` (batch, k + 1) in [0, 1), a tensor or an
-    array; `lengths` (batch): how many tokens were drafted, None for k.
+    array (in a tensor's, 1 draws the last class with weight); `lengths` (batch): how many tokens were drafted, None for k.
 
     Draft i is kept while uniforms[i] * draft_probs[i][token] <
     target_probs[i][token]; after the first that is not, one token is drawn from
@@ -314,7 +325,7 @@ def verify_drafts(draft_tokens, draft_probs, target_probs, uniforms, lengths=Non
     flat = _flat_ints(tokens, "draft_tokens")
     if lengths is not None:
         lengths = _flat_ints(lengths, "lengths")
-    return _native.verify_drafts(flat, draft_probs, target_probs, _device_values(uniforms), lengths)
+    return _native.verify_drafts(flat, draft_probs, target_probs, _uniforms(uniforms), lengths)
 
 
 def _outside(what):
