@@ -457,9 +457,10 @@ int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, c
  * weights is more than uniforms[drafts] times their total (sums in 64 bits),
  * and the highest with weight for a number that is not below 1.
  * Where max(target - draft, 0) has no weight, target[j] is drawn from; a row
- * without weight there gives -1. Probabilities need not sum to 1; a NaN or
- * negative one weighs nothing. Outputs: accepted (batch), the number kept;
- * out (batch, drafts + 1), the kept tokens, the drawn one, then -1. A drafted
+ * without weight there gives -1. Probabilities need not sum to 1; a negative
+ * one is taken as 0, and a NaN weighs nothing, in a draft's row in what the draft
+ * leaves. Outputs: accepted (batch), the number kept; out (batch, drafts + 1),
+ * the kept tokens, the drawn one, then -1. A drafted
  * token outside [0, vocab) is not kept and, like a length outside [0, drafts],
  * raises the device guard flag (oxi_hip_sync reports it). `workspace`: device
  * memory of oxi_verify_drafts_workspace bytes, 8-byte aligned, that the call

@@ -28,6 +28,9 @@ struct VerifyArgs {
   int* guard;
 };
 
+// A draft's probability: what a negative one stands for is 0 (a NaN stays).
+__device__ __forceinline__ float drafted(float q) { return q < 0.f ? 0.f : q; }
+
 // How many drafts of the sequence are kept, to every thread of the block;
 // `slot`: one int64 of LDS. `rejected`: whether a draft was not.
 template <int N>
@@ -48,7 +51,7 @@ __device__ __forceinline__ int64_t count_kept(const VerifyArgs& g, int64_t b, un
       atomicOr(g.guard, 1);
     } else {
       const double p = g.target[(b * (g.drafts + 1) + i) * g.vocab + x];
-      const double q = g.draft ? (double)g.draft[(b * g.drafts + i) * g.vocab + x] : 1.0;
+      const double q = g.draft ? (double)drafted(g.draft[(b * g.drafts + i) * g.vocab + x]) : 1.0;
       kept = (double)g.uniforms[b * (g.drafts + 1) + i] * q < p;
     }
     if (!kept) atomicMin(slot, (unsigned long long)i);
@@ -188,7 +191,7 @@ __global__ __launch_bounds__(NT) void verify_sums_k(const VerifyArgs g, Sums* __
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double pd = p[u][j] > 0.f ? (double)p[u][j] : 0.0;
-      const double d = (double)p[u][j] - (double)q[u][j];
+      const double d = (double)p[u][j] - (double)drafted(q[u][j]);
       own += pd;
       left += d > 0.0 && v0 + u * 256 + j != r.removed ? d : 0.0;
     }
@@ -310,7 +313,7 @@ __global__ __launch_bounds__(NT) void verify_pick_k(const VerifyArgs g, const Su
       }
     }
     auto weight = [&](int j) {
-      const double d = (double)p[j] - (double)q[j];
+      const double d = (double)p[j] - (double)drafted(q[j]);
       return d > 0.0 && !(use_left && v0 + j == r.removed) ? d : 0.0;
     };
     double w = 0.0;

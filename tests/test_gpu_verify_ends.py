@@ -25,6 +25,25 @@ def test_a_number_that_reaches_one_draws_the_last_class(hip, v, u1):
         assert np.array_equal(a, wa) and np.array_equal(o, wo), (o, wo)
 
 
+@pytest.mark.parametrize("v", [7, 1003, 40000])
+def test_negative_draft_probabilities_weigh_nothing(hip, v):
+    """As the zeros that they stand for: neither does such a token's draft get in by its product, nor the class a
+    greater weight."""
+    target, draft, tokens, u = make(8, 3, v, v)
+    draft[:, :, ::2] -= np.float32(0.3)
+    draft[0] = -draft[0]
+    target[1] = -target[1]  # weighs nothing either, whatever the draft is
+    draft[1] = -1.0
+    tokens[2] = 0
+    draft[3, :, 1] = np.nan
+    assert (draft < 0).any()
+    a, o = run(hip, target, draft, tokens, u)
+    wa, wo, margin = oracle(target, np.where(draft < 0, np.float32(0), draft), tokens, u)
+    assert (margin > 1e-12).all()
+    assert np.array_equal(a, wa) and np.array_equal(o, wo)
+    assert a[1] == 0 and (o[1] == -1).all()
+
+
 def test_numbers_in_64_bits(hip):
     """Numbers below 1 that 32 bits would round to it draw as the largest float below 1 does."""
     import oxitorch_amd as ox
