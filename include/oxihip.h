@@ -424,14 +424,21 @@ int oxi_cross_entropy_fwd_grad(const float* logits, const int64_t* targets, floa
  * in 64 bits in a fixed order (n for the plain mean, the count of rows that
  * hold entries for padded batches). An id given twice counts with both entries.
  * `lse` (n, log sum exp(logits/T)) and `rest` (n: log qr, or 0 without top_lse,
- * with what lse lost to its rounding) go to the backward. With `dlogits` (n, c) set, the same pass also
- * writes the gradient for an upstream gradient of 1: T/divisor times q - p
- * at the listed classes and q (1 - pr/qr) at the others (q without top_lse).
+ * with what lse lost to its rounding) go to the backward. With `dlogits` (n, c)
+ * set, the same pass also writes the gradient for an upstream gradient of 1:
+ * T/divisor times q - p at the listed classes and q (1 - pr/qr) at the others (q
+ * without top_lse).
  * 1 <= k <= OXI_DISTILL_MAX_TOP. An id >= c raises the device guard flag
  * (oxi_hip_sync reports it) and is taken as padding. Takes no workspace. */
 int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, const float* top_lse, float* loss,
                     float* row_loss, float* lse, float* rest, float* dlogits, int64_t n, int64_t c, int64_t k,
                     float temperature, float divisor);
+/* The same with the count of the rows that hold entries, at least 1, as the
+ * divisor. The call forms it on the device from ids and top and writes it to
+ * count[0], so that nobody reads them back (two small launches more). */
+int oxi_distill_fwd_counted(const float* logits, const int64_t* ids, const float* top, const float* top_lse,
+                            float* loss, float* row_loss, float* lse, float* rest, float* dlogits, float* count,
+                            int64_t n, int64_t c, int64_t k, float temperature);
 /* dlogits for the upstream scalar gradient gloss[0] (device): the forward's
  * dlogits times it, of the same accuracy. lse and rest are the forward's, from the
  * same logits, entries and temperature: rows of up to 65536 classes form their
@@ -439,6 +446,9 @@ int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, c
 int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, const float* top_lse,
                     const float* lse, const float* rest, const float* gloss, float* dlogits, int64_t n, int64_t c,
                     int64_t k, float temperature, float divisor);
+int oxi_distill_bwd_counted(const float* logits, const int64_t* ids, const float* top, const float* top_lse,
+                            const float* lse, const float* rest, const float* gloss, float* dlogits,
+                            const float* count, int64_t n, int64_t c, int64_t k, float temperature);
 
 /* ------------------------------------------------------------------------ */
 /* Verification of drafted tokens. No counterpart in the reference.          */

@@ -107,6 +107,8 @@ _SIGS = {
     "oxi_cross_entropy_fwd_grad": [vp, vp, vp, vp, vp, c_i64, c_i64],
     "oxi_distill_fwd": [vp, vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float, c_float],
     "oxi_distill_bwd": [vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float, c_float],
+    "oxi_distill_fwd_counted": [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float],
+    "oxi_distill_bwd_counted": [vp, vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float],
     "oxi_verify_drafts": [vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64],
     "oxi_verify_drafts_workspace": [c_i64, c_i64, P_i64],
     "oxi_index_select": [vp, c_i64, c_i64, c_i64, vp, c_i64, vp],

@@ -42,11 +42,14 @@ struct DistillArgs {
   int c, k;
   float inv_t;
   double t;  // temperature
-  float gscale;  // T / divisor
+  float divisor;
+  const float* count;  // the divisor if it lies on the device, else NULL
   const float* gloss;  // the upstream gradient, NULL for 1
   int* guard;
 
+  __device__ __forceinline__ float divided_by() const { return count ? count[0] : divisor; }
   __device__ __forceinline__ float upstream() const { return gloss ? gloss[0] : 1.f; }
+  __device__ __forceinline__ float grad_scale(float over, float up) const { return (float)t / over * up; }
 };
 
 // A row's teacher entries in LDS: class ids (-1: padding, or an id that an
@@ -413,7 +416,7 @@ __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
     }
   }
   if (!g.dx) return;
-  const float gscale = g.gscale * g.upstream();
+  const float gscale = g.grad_scale(g.divided_by(), g.upstream());
   double share = tail ? rest_excess(psum, listed / total, exp64(lr), rest_of(psum)) : 1.0;
   share = sum > 0.0 || sum != sum ? share / sum : 0.0;
   const float scale = (float)share * gscale, shift = tail && mr == NEG_INF ? 0.f : mr;
@@ -510,9 +513,9 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   auto x4 = [&](int c) -> const f4* {
     return reinterpret_cast<const f4*>(reinterpret_cast<const char*>(xr + head) + (uint32_t)c * 16u);
   };
-  // used after the row's sums: nothing waits for it before (a wait here, 366
+  // used after the row's sums: nothing waits for them before (a wait here, 366
   // to 393 us backward at (16384, 16640))
-  const float up = GRAD ? g.upstream() : 1.f;
+  const float up = GRAD ? g.upstream() : 1.f, over = GRAD ? g.divided_by() : 1.f;
   // the entries' loads go first (a thread's first one; the rest of long lists
   // later): a wait for them leaves the row's in flight, if those are
   const int64_t id0 = t < g.k ? g.ids[row * g.k + t] : -1;
@@ -703,7 +706,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
       if constexpr (NTS) __builtin_nontemporal_store(d, p);
       else *p = d;
     };
-    const float gscale = g.gscale * up;
+    const float gscale = g.grad_scale(over, up);
     if (some) {
       float gs = gscale / s;
       if constexpr (TAIL)  // s is 1 or more where any of its classes has a finite logit
@@ -757,9 +760,26 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
   }
 }
 
-// loss[0] = sum of the rows' losses / divisor, in float64 in a fixed order: one
-// block, one round of loads for up to 8192 rows, 4.5 us.
+// held[row] = 1 where the row holds an entry, else 0: a wave a row. With the launch
+// that adds them up 5 us for 64 entries a row of 8192, 10 for 200 of 16384.
+__global__ __launch_bounds__(NT) void distill_held_k(const int64_t* __restrict__ ids, const float* __restrict__ top,
+                                                     float* __restrict__ held, int64_t n, int c, int k) {
+  const int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+  if (row >= n) return;
+  bool any = false;
+  for (int j = threadIdx.x & 63; j < k; j += 64) {
+    const int64_t id = ids[row * k + j];
+    any |= id >= 0 && id < c && top[row * k + j] != NEG_INF;
+  }
+  const bool some = __ballot(any) != 0;
+  if ((threadIdx.x & 63) == 0) held[row] = some ? 1.f : 0.f;
+}
+
+// loss[0] = sum of the rows' losses / divisor (count[0], if given), in float64 in a
+// fixed order: one block, one round of loads for up to 8192 rows, 4.5 us. Also the
+// count of the rows that hold an entry, `least` 1.
 __global__ __launch_bounds__(1024) void distill_mean_k(const float* __restrict__ row_loss, int64_t n, double divisor,
+                                                       const float* __restrict__ count, float least,
                                                        float* __restrict__ loss) {
   __shared__ double red[1024 / 64];
   constexpr int U = 8;  // loads in flight a thread
@@ -773,7 +793,10 @@ __global__ __launch_bounds__(1024) void distill_mean_k(const float* __restrict__
       if (i0 + u * 1024 < n) acc += (double)v[u];
   }
   acc = block_sum<1024>(acc, red);
-  if (threadIdx.x == 0) loss[0] = (float)(acc / divisor);
+  if (threadIdx.x == 0) {
+    const float v = (float)(acc / (count ? (double)count[0] : divisor));
+    loss[0] = v < least ? least : v;  // a NaN stays
+  }
 }
 
 int check_distill(const char* what, int64_t n, int64_t c, int64_t k, float temperature, float divisor) {
@@ -847,6 +870,49 @@ void launch_any(const DistillArgs& g) {
     distill_loop_k<<<dim3((unsigned)g.n), dim3(NT), teacher_bytes(g.k), stream()>>>(g);
 }
 
+// count: where the divisor lies (formed first), NULL for the one given.
+int distill_fwd(const char* what, const float* logits, const int64_t* ids, const float* top, const float* top_lse,
+                float* loss, float* row_loss, float* lse, float* rest, float* dlogits, float* count, int64_t n,
+                int64_t c, int64_t k, float temperature, float divisor) {
+  if (int rc = check_distill(what, n, c, k, temperature, divisor)) return rc;
+  if (!loss) return fail(OXI_INVALID_ARGUMENT, "%s: loss must not be NULL", what);
+  if (n && (!logits || !ids || !top || !row_loss || !lse || !rest))
+    return fail(OXI_INVALID_ARGUMENT, "%s: NULL tensor pointer", what);
+  OXI_CHECK_INIT();
+  if (n == 0) {
+    if (count)
+      if (int rc = oxi_fill(count, 1, 1.f)) return rc;
+    return oxi_fill(loss, 1, 0.f);
+  }
+  if (count) {  // the rows' flags lie in row_loss meanwhile
+    distill_held_k<<<dim3((unsigned)ceil_div(n, NT / 64)), dim3(NT), 0, stream()>>>(ids, top, row_loss, n, (int)c,
+                                                                                     (int)k);
+    if (int rc = check_launch(what)) return rc;
+    distill_mean_k<<<1, 1024, 0, stream()>>>(row_loss, n, 1.0, nullptr, 1.f, count);
+    if (int rc = check_launch(what)) return rc;
+  }
+  const DistillArgs g{logits, ids,     top, top_lse, row_loss, lse, rest, dlogits, n, (int)c, (int)k,
+                      1.0f / temperature, (double)temperature, divisor, count, nullptr, guard_flag()};
+  launch_any(g);
+  if (int rc = check_launch(what)) return rc;
+  distill_mean_k<<<1, 1024, 0, stream()>>>(row_loss, n, (double)divisor, count, -__builtin_huge_valf(), loss);
+  return check_launch(what);
+}
+
+int distill_bwd(const char* what, const float* logits, const int64_t* ids, const float* top, const float* top_lse,
+                const float* lse, const float* rest, const float* gloss, float* dlogits, const float* count, int64_t n,
+                int64_t c, int64_t k, float temperature, float divisor) {
+  if (int rc = check_distill(what, n, c, k, temperature, divisor)) return rc;
+  if (n == 0) return OXI_OK;
+  if (!logits || !ids || !top || !lse || !rest || !gloss || !dlogits)
+    return fail(OXI_INVALID_ARGUMENT, "%s: NULL tensor pointer", what);
+  OXI_CHECK_INIT();
+  const DistillArgs g{logits, ids, top, top_lse, nullptr, const_cast<float*>(lse), const_cast<float*>(rest), dlogits, n,
+                      (int)c, (int)k, 1.0f / temperature, (double)temperature, divisor, count, gloss, guard_flag()};
+  launch_any(g);
+  return check_launch(what);
+}
+
 }  // namespace
 }  // namespace oxi
 
@@ -857,36 +923,31 @@ extern "C" {
 int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, const float* top_lse, float* loss,
                     float* row_loss, float* lse, float* rest, float* dlogits, int64_t n, int64_t c, int64_t k,
                     float temperature, float divisor) {
-  if (int rc = check_distill("distill_fwd", n, c, k, temperature, divisor)) return rc;
-  if (!loss) return fail(OXI_INVALID_ARGUMENT, "distill_fwd: loss must not be NULL");
-  if (n && (!logits || !ids || !top || !row_loss || !lse || !rest))
-    return fail(OXI_INVALID_ARGUMENT, "distill_fwd: NULL tensor pointer");
-  OXI_CHECK_INIT();
-  if (n == 0) return oxi_fill(loss, 1, 0.f);
-  const DistillArgs g{logits,  ids,    top,    top_lse,
-                      row_loss, lse,    rest,   dlogits,
-                      n,        (int)c, (int)k, 1.0f / temperature,
-                      (double)temperature, temperature / divisor, nullptr, guard_flag()};
-  launch_any(g);
-  if (int rc = check_launch("distill_fwd")) return rc;
-  distill_mean_k<<<1, 1024, 0, stream()>>>(row_loss, n, (double)divisor, loss);
-  return check_launch("distill_fwd: mean");
+  return distill_fwd("distill_fwd", logits, ids, top, top_lse, loss, row_loss, lse, rest, dlogits, nullptr, n, c, k,
+                     temperature, divisor);
+}
+
+int oxi_distill_fwd_counted(const float* logits, const int64_t* ids, const float* top, const float* top_lse,
+                            float* loss, float* row_loss, float* lse, float* rest, float* dlogits, float* count,
+                            int64_t n, int64_t c, int64_t k, float temperature) {
+  if (!count) return fail(OXI_INVALID_ARGUMENT, "distill_fwd_counted: count must not be NULL");
+  return distill_fwd("distill_fwd_counted", logits, ids, top, top_lse, loss, row_loss, lse, rest, dlogits, count, n, c,
+                     k, temperature, 1.f);
 }
 
 int oxi_distill_bwd(const float* logits, const int64_t* ids, const float* top, const float* top_lse,
                     const float* lse, const float* rest, const float* gloss, float* dlogits, int64_t n, int64_t c,
                     int64_t k, float temperature, float divisor) {
-  if (int rc = check_distill("distill_bwd", n, c, k, temperature, divisor)) return rc;
-  if (n == 0) return OXI_OK;
-  if (!logits || !ids || !top || !lse || !rest || !gloss || !dlogits)
-    return fail(OXI_INVALID_ARGUMENT, "distill_bwd: NULL tensor pointer");
-  OXI_CHECK_INIT();
-  const DistillArgs g{logits,  ids,     top,    top_lse,
-                      nullptr, const_cast<float*>(lse), const_cast<float*>(rest), dlogits,
-                      n,       (int)c,  (int)k, 1.0f / temperature,
-                      (double)temperature, temperature / divisor, gloss, guard_flag()};
-  launch_any(g);
-  return check_launch("distill_bwd");
+  return distill_bwd("distill_bwd", logits, ids, top, top_lse, lse, rest, gloss, dlogits, nullptr, n, c, k, temperature,
+                     divisor);
+}
+
+int oxi_distill_bwd_counted(const float* logits, const int64_t* ids, const float* top, const float* top_lse,
+                            const float* lse, const float* rest, const float* gloss, float* dlogits,
+                            const float* count, int64_t n, int64_t c, int64_t k, float temperature) {
+  if (!count) return fail(OXI_INVALID_ARGUMENT, "distill_bwd_counted: count must not be NULL");
+  return distill_bwd("distill_bwd_counted", logits, ids, top, top_lse, lse, rest, gloss, dlogits, count, n, c, k,
+                     temperature, 1.f);
 }
 
 }  // extern "C"

@@ -735,7 +735,7 @@ Var rotary(const Var& x, const RotaryFrequencies& f, const std::optional<std::ve
 // ---- distillation ---------------------------------------------------------------------
 
 Var distillation_loss(const Var& logits, const std::vector<int64_t>& ids, const Tensor& top,
-                      const std::optional<Tensor>& top_lse, float temperature, float divisor) {
+                      const std::optional<Tensor>& top_lse, float temperature) {
   const Tensor& lv = logits.value();
   if (lv.ndim() != 2) err_invalid("distillation_loss expects (batch, classes) logits, got " + fmt_shape(lv.shape));
   const int64_t n = lv.shape[0], c = lv.shape[1];
@@ -755,25 +755,26 @@ Var distillation_loss(const Var& logits, const std::vector<int64_t>& ids, const 
   if (top_lse) ec = t_contiguous(*top_lse);
   auto id = device_i64(ids);
   Tensor loss = Tensor::empty({}, Dev::Hip), row = Tensor::empty({n}, Dev::Hip), lse = Tensor::empty({n}, Dev::Hip),
-         rest = Tensor::empty({n}, Dev::Hip);
+         rest = Tensor::empty({n}, Dev::Hip), count = Tensor::empty({}, Dev::Hip);
   // With a gradient to come, the forward pass also forms the gradient for
   // loss.backward()'s seed, as cross_entropy does (and the same switch turns off).
   std::optional<Tensor> unit;
   if (logits.requires_grad() && is_grad_enabled() && ce_one_pass()) unit = Tensor::empty({n, c}, Dev::Hip);
   const int64_t* ip = static_cast<const int64_t*>(id->ptr);
-  hip_check(oxi_distill_fwd(lc.data(), ip, tc.data(), ec ? ec->data() : nullptr, loss.data(), row.data(), lse.data(),
-                            rest.data(), unit ? unit->data() : nullptr, n, c, k, temperature, divisor));
+  hip_check(oxi_distill_fwd_counted(lc.data(), ip, tc.data(), ec ? ec->data() : nullptr, loss.data(), row.data(),
+                                    lse.data(), rest.data(), unit ? unit->data() : nullptr, count.data(), n, c, k,
+                                    temperature));
   auto fresh = std::make_shared<std::atomic<bool>>(unit.has_value());
   return Var::op(loss, "distillation_loss", {logits},
-                 [lc, tc, ec, id, lse, rest, n, c, k, temperature, divisor, unit, fresh](
+                 [lc, tc, ec, id, lse, rest, count, n, c, k, temperature, unit, fresh](
                      const Tensor& g, const std::vector<bool>& need) -> Grads {
                    if (!need[0]) return {std::nullopt};
                    if (is_implicit_seed(g) && fresh->exchange(false)) return {*unit};
                    Tensor gs = t_contiguous(g);
                    Tensor d = Tensor::empty({n, c}, Dev::Hip);
-                   hip_check(oxi_distill_bwd(lc.data(), static_cast<const int64_t*>(id->ptr), tc.data(),
-                                             ec ? ec->data() : nullptr, lse.data(), rest.data(), gs.data(), d.data(), n, c,
-                                             k, temperature, divisor));
+                   hip_check(oxi_distill_bwd_counted(lc.data(), static_cast<const int64_t*>(id->ptr), tc.data(),
+                                                     ec ? ec->data() : nullptr, lse.data(), rest.data(), gs.data(),
+                                                     d.data(), count.data(), n, c, k, temperature));
                    return {d};
                  });
 }

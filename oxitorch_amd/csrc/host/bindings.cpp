@@ -664,14 +664,14 @@ PYBIND11_MODULE(_native, m) {
 
   m.def(
       "distillation_loss",
-      [](const PyTensor& logits, const py::object& ids, const PyTensor& top, const py::object& lse, float temperature,
-         float divisor) {
+      [](const PyTensor& logits, const py::object& ids, const PyTensor& top, const py::object& lse,
+         float temperature) {
         std::optional<Tensor> l;
         if (!lse.is_none()) l = lse.cast<PyTensor&>().value();
-        return PyTensor(aops::distillation_loss(logits.v, int_ids(ids), top.value(), l, temperature, divisor));
+        return PyTensor(aops::distillation_loss(logits.v, int_ids(ids), top.value(), l, temperature));
       },
       py::arg("logits"), py::arg("teacher_ids"), py::arg("teacher_logits"), py::arg("teacher_lse"),
-      py::arg("temperature"), py::arg("divisor"));
+      py::arg("temperature"));
 
   m.def(
       "verify_drafts",

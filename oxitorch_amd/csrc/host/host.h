@@ -315,9 +315,9 @@ Var embedding(const std::vector<int64_t>& indices, const Var& weight);
 Var rotary(const Var& x, const RotaryFrequencies& f, const std::optional<std::vector<int64_t>>& positions,
            int64_t offset, int layout);
 // The distillation loss of logits (n, c) against the teacher's ids and logits (n,
-// k each), and its log-sum-exp (n) if given; the sum over the rows / divisor.
+// k each), and its log-sum-exp (n) if given; the mean over the rows that hold entries.
 Var distillation_loss(const Var& logits, const std::vector<int64_t>& ids, const Tensor& top,
-                      const std::optional<Tensor>& top_lse, float temperature, float divisor);
+                      const std::optional<Tensor>& top_lse, float temperature);
 }  // namespace aops
 
 // ---- serving: no gradients -----------------------------------------------------------

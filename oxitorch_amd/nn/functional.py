@@ -263,10 +263,11 @@ def distillation_loss(logits, teacher_ids, teacher_logits, temperature=1.0, teac
     teacher's that is known by its k best entries a row: T^2 times the mean over
     the rows of sum p (log p - log q[id]).
 
-    `teacher_ids` (batch, k): the entries' classes as integers; a negative one is
-    padding, and rows of padding alone count neither in the sum nor in the mean
-    (padded tokens). `teacher_logits` (batch, k): the teacher's logits there, a
-    tensor or an array; no gradient goes to them. p is their softmax at
+    `teacher_ids` (batch, k): the entries' classes as integers;
+    `teacher_logits` (batch, k): the teacher's logits there, a tensor or an array; no
+    gradient goes to them. An entry with a negative id or a logit of -inf is padding,
+    and rows of padding alone (padded tokens) count neither in the sum nor in the
+    mean. p is their softmax at
     temperature T over the row's entries; with `teacher_lse` (batch: the
     log-sum-exp of all of the teacher's logits/T) p are the teacher's own
     probabilities, and what they leave to the other classes is compared with
@@ -285,8 +286,7 @@ def distillation_loss(logits, teacher_ids, teacher_logits, temperature=1.0, teac
     if list(top.shape) != list(ids.shape):
         raise ValueError(f"teacher_logits of shape {list(top.shape)} for teacher_ids of shape {list(ids.shape)}")
     lse = None if teacher_lse is None else _device_values(teacher_lse)
-    rows = int((flat.reshape(ids.shape) >= 0).any(axis=1).sum())
-    return _native.distillation_loss(logits, flat, top, lse, float(temperature), float(max(rows, 1)))
+    return _native.distillation_loss(logits, flat, top, lse, float(temperature))
 
 
 # ---- serving: drafted tokens ------------------------------------------------------------
