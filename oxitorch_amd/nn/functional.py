@@ -197,11 +197,15 @@ def rotary_embedding(x, frequencies, positions=None, offset=0, layout="half"):
 
     `frequencies`: what rotary_frequencies returns, an array of angles per
     position, or a _native.RotaryFrequencies that holds them on the device (as
-    nn.RotaryEmbedding keeps one). `positions`: integers, one per token or one
-    per batch and token; None counts from 0. `offset` is added to them. Angles
+    nn.RotaryEmbedding keeps one). `positions`: integers, one per token or (batch,
+    tokens), one per batch and token; None counts from 0. `offset` is added to them. Angles
     are formed in 64 bits. x may be any view (heads before tokens, a slice of a
     fused projection); one call serves query and key heads side by side."""
     if positions is not None:
+        given, each = list(np.shape(positions)), list(x.shape[:-2])
+        long = [d for d in given if d != 1]  # an order other than (batch, tokens) shows in these
+        if len(long) > 1 and long != [d for d in each if d != 1]:
+            raise ValueError(f"positions of shape {given} for tokens of shape {each}")
         positions = _flat_ints(positions, "positions")
     return _native.rotary_embedding(x, _frequencies(frequencies), positions, int(offset), layout)
 
