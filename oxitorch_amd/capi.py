@@ -543,7 +543,7 @@ def distill_fwd(logits: DeviceArray, ids: DeviceArray, top: DeviceArray, tempera
     loss, row_loss, lse, rest = DeviceArray((1,)), DeviceArray((n,)), DeviceArray((n,)), DeviceArray((n,))
     d = DeviceArray((n, c)) if need_grad else None
     call("oxi_distill_fwd", logits.ptr, ids.ptr, top.ptr, top_lse.ptr if top_lse else None, loss.ptr, row_loss.ptr,
-         lse.ptr, rest.ptr, d.ptr if d else None, n, c, ids.shape[1], temperature, divisor if divisor else max(1, n))
+         lse.ptr, rest.ptr, d.ptr if d else None, n, c, ids.shape[1], temperature, max(1, n) if divisor is None else divisor)
     return loss, row_loss, lse, rest, d
 
 
@@ -552,7 +552,7 @@ def distill_bwd(logits: DeviceArray, ids: DeviceArray, top: DeviceArray, lse: De
     n, c = logits.shape
     d = DeviceArray((n, c))
     call("oxi_distill_bwd", logits.ptr, ids.ptr, top.ptr, top_lse.ptr if top_lse else None, lse.ptr, rest.ptr,
-         gloss.ptr, d.ptr, n, c, ids.shape[1], temperature, divisor if divisor else max(1, n))
+         gloss.ptr, d.ptr, n, c, ids.shape[1], temperature, max(1, n) if divisor is None else divisor)
     return d
 
 
