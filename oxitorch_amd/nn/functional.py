@@ -207,6 +207,8 @@ def rotary_embedding(x, frequencies, positions=None, offset=0, layout="half"):
         if len(long) > 1 and long != [d for d in each if d != 1]:
             raise ValueError(f"positions of shape {given} for tokens of shape {each}")
         positions = _flat_ints(positions, "positions")
+    if int(offset) != offset:
+        raise TypeError(f"offset must be an integer, got {offset}")
     return _native.rotary_embedding(x, _frequencies(frequencies), positions, int(offset), layout)
 
 
