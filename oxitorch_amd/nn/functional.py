@@ -184,7 +184,8 @@ def rotary_frequencies(dim, base=10000.0, scaling=None):
 def _frequencies(f):
     if isinstance(f, _native.RotaryFrequencies):
         return f
-    inv, scale = f if isinstance(f, tuple) else (f, 1.0)
+    pair = isinstance(f, tuple) and len(f) == 2 and np.ndim(f[0]) > 0  # what rotary_frequencies returns
+    inv, scale = f if pair else (f, 1.0)
     return _native.RotaryFrequencies([float(v) for v in np.asarray(inv, dtype=np.float64).ravel()], scale)
 
 
