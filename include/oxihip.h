@@ -427,7 +427,9 @@ int oxi_cross_entropy_fwd_grad(const float* logits, const int64_t* targets, floa
  * with what lse lost to its rounding) go to the backward. With `dlogits` (n, c)
  * set, the same pass also writes the gradient for an upstream gradient of 1:
  * T/divisor times q - p at the listed classes and q (1 - pr/qr) at the others (q
- * without top_lse).
+ * without top_lse). That is row's derivative where the teacher's masses sum to 1;
+ * with a top_lse that is too small (sum p > 1, pr = 0) the loss counts p as given,
+ * whose derivative has q sum p for q, and the gradient is q - p all the same.
  * 1 <= k <= OXI_DISTILL_MAX_TOP. An id >= c raises the device guard flag
  * (oxi_hip_sync reports it) and is taken as padding. Takes no workspace. */
 int oxi_distill_fwd(const float* logits, const int64_t* ids, const float* top, const float* top_lse, float* loss,

@@ -6,6 +6,7 @@
 //   k, or given the teacher's log-sum-exp, with pr = 1 - sum p left over)
 //   row = sum p (log p - log q[id]) + pr (log pr - log qr)
 //   dx  = T/divisor (q - p) at the entries, T/divisor q (1 - pr/qr) elsewhere
+//         (sum p + pr = 1: not q (sum p + pr) for q)
 //
 // The k entries of a row are worked out in 64 bits by the block that owns the
 // row: a student near its teacher has a small loss of terms that cancel. With

@@ -278,7 +278,8 @@ def distillation_loss(logits, teacher_ids, teacher_logits, temperature=1.0, teac
     temperature T over the row's entries; with `teacher_lse` (batch: the
     log-sum-exp of all of the teacher's logits/T) p are the teacher's own
     probabilities, and what they leave to the other classes is compared with
-    what the student leaves there.
+    what the student leaves there. The gradient takes them to sum to at most 1, as
+    they do where teacher_lse is the teacher's at T.
 
     Fused as cross_entropy is: one pass over the logits writes the loss and the
     gradient for backward()'s implicit seed."""
