@@ -432,8 +432,8 @@ __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
 // for the loss and its gradient. The float4s begin at a row's first 128-byte line;
 // the classes before and after them go a float to a thread. Exponentials are exp2
 // of (x - m) * (log2(e)/T). With the rest's term the listed classes are taken out
-// of the registers (an exponential of 0) by a bitmap in LDS, and their own few are
-// added by the entries' threads. The block's stores write the row as if nothing
+// of the registers (an exponential of 0) by a bitmap in LDS, m is the maximum of the
+// others, and the entries' threads add the listed ones' own few. The block's stores write the row as if nothing
 // were listed; the entries' values go over that after a barrier.
 //
 // HBM bounds it: (8192, 32000) with 64 entries and the rest 354-364 us, 5.8-6.1 TB/s;
@@ -448,20 +448,24 @@ __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
 //
 // The backward for an upstream scalar is the same pass without the loss (no
 // row_loss): (8192, 32000) 359-368 us. From a log-sum-exp rounded to a float every
-// probability of a row would be off by up to |lse| 2^-24 of itself: 6e-4 at logits near
-// 10^4, where these are off by 2e-6. Rows that no registers hold take the two floats lse
-// and rest instead of a pass for their sums ((1500, 100001) 229 us, 261 with it).
+// probability of a row would be off by up to |lse| 2^-24 of itself, 6e-4 at logits near
+// 10^4; here its error goes by the distance from the maximum. Rows that no registers
+// hold take the two floats lse and rest instead of a pass for their sums ((1500, 100001)
+// 229 us, 261 with it).
 //
-// NV = 0: longer rows, streamed twice, the first time with a running maximum; the
-// second time they come from the Infinity Cache (a block a row on every CU is
-// at most 256 rows in flight, 134 MB of 131072 classes). (1500, 100001) 248 us, 4.8
-// TB/s of the bytes that one pass needs.
+// NV = 0: longer rows, streamed twice, the first time with a running maximum. Two
+// blocks fit a CU, so that up to 512 rows are between their passes: 205 MB of 100001
+// classes, which the Infinity Cache (256 MB) holds, but 268 of 131072 and 614 of 300000.
+// (1500, 100001) 261 us, 4.6 TB/s of the bytes that one pass needs; (2048, 128256)
+// 447 us, 4.7; (1024, 200000) 372, 4.4; (800, 300000) 505, 3.8. With one block a CU 253,
+// 445, 359 and 450, and the loss alone of (1500, 100001) 116 where two take 103.
 constexpr int STREAM_U = 4;         // float4s in flight a thread
 constexpr int STREAM_MAX = 300000;  // classes whose bitmap fits in LDS beside 1024 entries
 
 // Waves a SIMD that the registers must allow: 4 with 128 a lane, 8 with 64; and at
 // most, so that rows written as they are read do not crowd each other out: a third
-// block of 512 threads or a fifth of 256 a CU took (16384, 16640) from 365 to 393 us.
+// block of 512 threads a CU took (16384, 16640) with the rest's term from 366 to 400 us,
+// a fifth of 256 (8192, 12000) from 136 to 144.
 constexpr int rows_waves(int nv) { return nv ? 4 : 8; }
 constexpr int rows_waves_most(bool grad, int nv) { return grad && nv >= 10 ? 4 : 8; }
 

@@ -9,7 +9,7 @@
 // are copied); a thread has one unit, of some of the block's (token, head) rows,
 // ROWS of them in flight. The first of them are loaded before the block forms its
 // tokens' cosines and sines, once for all heads, in LDS. HBM bounds it: (4, 4096,
-// 32, 128) 86 us a call, 6.2 TB/s; (16, 1023, 12, 64) heads first 21 us, 4.7 TB/s,
+// 32, 128) 87 us a call, 6.1 TB/s; (16, 1023, 12, 64) heads first 22 us, 4.6 TB/s,
 // where a launch's beginning and end weigh.
 #include <algorithm>
 

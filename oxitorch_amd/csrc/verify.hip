@@ -153,9 +153,9 @@ __device__ __forceinline__ Sums block_before(Sums v, Sums* lds, Sums& all) {
 // sequence, finds the piece that the drawn number falls into and reads that
 // one again. Each block of the first finds the row by itself (a gather of two
 // floats a draft). HBM bounds the first, behind the three dependent loads that find the
-// row: 128 sequences of 131072 classes, of which half reject a token, 100 MB in 19.8
-// us, 5.1 TB/s (a block a sequence walking its row: 810); the second takes 5.9 us
-// there, a chain of dependent loads and scans. 4 sequences of 32000: 3.4 and 3.8 us,
+// row: 128 sequences of 131072 classes, of which half reject a token, 100 MB in 20.3
+// us, 4.9 TB/s (a block a sequence walking its row: 810); the second takes 5.9 us
+// there, a chain of dependent loads and scans. 4 sequences of 32000: 3.7 and 3.9 us,
 // both such chains.
 
 template <int U>
