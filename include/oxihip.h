@@ -417,9 +417,10 @@ int oxi_cross_entropy_fwd_grad(const float* logits, const int64_t* targets, floa
  * compared with the student's mass qr on the classes not listed:
  *   row = sum p (log p - log q[id]) + pr (log pr - log qr).
  * qr is a logarithm throughout: however far below the listed classes the others
- * lie, the loss is finite. Where none of them has a finite logit, a pr of up to
+ * lie, the loss is finite. Where qr is below 2^-126 (masked logits), a pr of up to
  * 2^-22 (1 + |top_lse|), what a log-sum-exp worked out in 32 bits may lack, counts
- * as 0, and a larger one makes the loss inf (the gradient at those classes is 0).
+ * as 0; where none of those classes has a finite logit a larger one makes the loss
+ * inf (the gradient at them is 0).
  * row_loss (n) = T^2 row; loss (1 float) = sum of row_loss / divisor, summed
  * in 64 bits in a fixed order (n for the plain mean, the count of rows that
  * hold entries for padded batches). An id given twice counts with both entries.

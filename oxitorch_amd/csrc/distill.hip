@@ -298,13 +298,19 @@ __device__ __forceinline__ double entry_term(double p, double lp, double lq, boo
 // What entries of sum psum leave to the other classes.
 __device__ __forceinline__ double rest_of(double psum) { return psum < 1.0 ? 1.0 - psum : psum != psum ? psum : 0.0; }
 
+// That, given whether the student's mass there is below 2^-126, as of masked logits
+// (-inf or the lowest float): a rest of the size that rounding leaves in a log-sum-exp
+// worked out in 32 bits (4 steps of it and of 1) is none then. Its loss would be that
+// rounding times their distance.
+template <class F>
+__device__ __forceinline__ F rest_beside(F pr, bool masked, float top_lse) {
+  return masked && pr <= (F)0x1p-22 * ((F)1 + (F)fabsf(top_lse)) ? (F)0 : pr;
+}
+
 // The rest's share, lr the logarithm of the student's mass there, with what the
-// masses as rounded lack of 1. Where no class that is not listed has a finite logit
-// (lr = -inf) a rest of the size that rounding leaves in a log-sum-exp worked out in
-// 32 bits (4 steps of it and of 1) is none: not an infinite loss.
+// masses as rounded lack of 1.
 __device__ __forceinline__ double rest_term(double psum, double lr, float top_lse) {
-  double pr = rest_of(psum);
-  if (lr == (double)NEG_INF && pr <= 0x1p-22 * (1.0 + fabs((double)top_lse))) pr = 0.0;
+  const double pr = rest_beside(rest_of(psum), lr < -126 * 0.6931471805599453, top_lse);
   return (pr > 0.0 || pr != pr ? pr * exp_rest(lr - log64(pr)) : exp64(lr)) + ((psum + pr) - 1.0);
 }
 
@@ -320,8 +326,8 @@ __device__ __forceinline__ void write_row(const DistillArgs& g, int64_t row, boo
 
 // qr - pr, from the masses ql and psum of the listed classes where those are the smaller.
 template <class F>
-__device__ __forceinline__ F rest_excess(F psum, F ql, F qr, F pr) {
-  return psum < (F)0.5 ? psum - ql : qr - pr;
+__device__ __forceinline__ F rest_excess(F psum, F ql, F qr, F pr, float top_lse) {
+  return psum < (F)0.5 ? psum - ql : qr - rest_beside(pr, qr < (F)0x1p-126, top_lse);
 }
 
 // The gradient at the row's entries, after the block has written the row as if
@@ -412,13 +418,11 @@ __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
         s += entry_term(a.p[j], a.lp[j], ((double)xr[a.id[j]] - (double)m) / g.t - lt, tail, a.dup[j] >= 0);
     s = block_sum<NT>(s, red);
     if (tail && some) s += rest_term(psum, lr, g.top_lse[row]);
-    if (t == 0) {
-      write_row(g, row, some, s, (double)m / g.t + lt, tail ? lr : 0.0);
-    }
+    if (t == 0) write_row(g, row, some, s, (double)m / g.t + lt, tail ? lr : 0.0);
   }
   if (!g.dx) return;
   const float gscale = g.grad_scale(g.divided_by(), g.upstream());
-  double share = tail ? rest_excess(psum, listed / total, exp64(lr), rest_of(psum)) : 1.0;
+  double share = tail ? rest_excess(psum, listed / total, exp64(lr), rest_of(psum), g.top_lse[row]) : 1.0;
   share = sum > 0.0 || sum != sum ? share / sum : 0.0;
   const float scale = (float)share * gscale, shift = tail && mr == NEG_INF ? 0.f : mr;
   float* dr = g.dx + row * g.c;
@@ -433,8 +437,9 @@ __global__ __launch_bounds__(NT) void distill_loop_k(const DistillArgs g) {
 // the classes before and after them go a float to a thread. Exponentials are exp2
 // of (x - m) * (log2(e)/T). With the rest's term the listed classes are taken out
 // of the registers (an exponential of 0) by a bitmap in LDS, m is the maximum of the
-// others, and the entries' threads add the listed ones' own few. The block's stores write the row as if nothing
-// were listed; the entries' values go over that after a barrier.
+// others, and the entries' threads add the listed ones' own few. The block's stores
+// write the row as if nothing were listed; the entries' values go over that after a
+// barrier.
 //
 // HBM bounds it: (8192, 32000) with 64 entries and the rest 354-364 us, 5.8-6.1 TB/s;
 // (4096, 50257) 285 us, 5.8 TB/s; 64 rows of 32000 10 us, a row a CU. The entries
@@ -493,8 +498,9 @@ __device__ __forceinline__ f4 without(const f4& v, uint32_t bits) {
 }
 
 template <int RT, int NV, bool GRAD, bool TAIL, bool NTS>
-__global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(NV), rows_waves_most(GRAD, NV)))) void distill_rows_k(
-    const DistillArgs g, const float scale2) {
+__global__ __launch_bounds__(RT)
+    __attribute__((amdgpu_waves_per_eu(rows_waves(NV), rows_waves_most(GRAD, NV)))) void distill_rows_k(
+        const DistillArgs g, const float scale2) {
   __shared__ double red[RT / 64], psum_at;
   __shared__ __align__(8) float lds[4 * (RT / 64)];
   __shared__ int twice;
@@ -715,7 +721,7 @@ __global__ __launch_bounds__(RT) __attribute__((amdgpu_waves_per_eu(rows_waves(N
     if (some) {
       float gs = gscale / s;
       if constexpr (TAIL)  // s is 1 or more where any of its classes has a finite logit
-        gs = s > 0.f || s != s ? gs * rest_excess(psumf, mine / total, above / total, prf) : 0.f;
+        gs = s > 0.f || s != s ? gs * rest_excess(psumf, mine / total, above / total, prf, tlse) : 0.f;
       if constexpr (NV > 0) {
 #pragma unroll
         for (int q = 0; q < NV; ++q)

@@ -51,8 +51,6 @@ def tail64(x, ids, top, T, lse, divisor):
         empty = not np.isfinite(z[out]).any()
         if empty:
             s, lr, dS = np.zeros(out.sum()), -np.inf, 0.0
-            if pr <= near_one(lse[r]):
-                pr = 0.0
         else:
             mr = z[out].max()
             s = np.exp(z[out] - mr)
@@ -61,6 +59,8 @@ def tail64(x, ids, top, T, lse, divisor):
             with np.errstate(invalid="ignore"):
                 dS = np.where(s > 0, s * eps(z[out] - mr), 0.0).sum() + seq + 2 * U
         qr = np.exp(lr)
+        if qr < 2.0 ** -126 and pr <= near_one(lse[r]):
+            pr = 0.0
         with np.errstate(invalid="ignore"):
             dT = np.where(~out & (q > 0), q * eps(z - m), 0.0).sum() + seq + 4 * U
         if not empty:
@@ -172,6 +172,10 @@ def test_other_classes_masked(hip, c, k):
         assert np.isfinite(g).all() and (g[out] == 0).all()
     # the lowest float is a number: a rest that is finite, and far
     low = np.where(x == -np.inf, np.finfo(np.float32).min, x)
+    masked, _ = check(hip, low, ids, top, T, lse)
+    assert np.allclose(masked, tail64(x, ids, top, T, lse, 6.0)[0], rtol=1e-5, atol=1e-5)
+    for mask in (-1e4, -1e9):
+        check(hip, np.where(x == -np.inf, np.float32(mask), x), ids, top, T, lse)
     rows, rest = check(hip, low, ids, top, T, (lse + np.float32(0.5)))
     assert np.isfinite(rows).all() and (rest < -1e37).all()
 
