@@ -454,6 +454,81 @@ int oxi_distill_bwd_counted(const float* logits, const int64_t* ids, const float
                             const float* count, int64_t n, int64_t c, int64_t k, float temperature);
 
 /* ------------------------------------------------------------------------ */
+/* Post-training losses over rows of logits. No counterpart in the reference; */
+/* they stand next to oxi_cross_entropy_* and oxi_distill_*.                  */
+
+/* Log-probabilities of chosen classes at temperature T, and the entropies of their
+ * rows' distributions: for row i of logits (n, c) with q = softmax(x/T) and a = ids[i]
+ *   logp = log q_a,   entropy = -sum q log q.
+ * A negative id is padding: such a row's logits are not read and its results are 0 (an
+ * id >= c raises the device guard flag, which oxi_hip_sync reports, and is padding
+ * too). A row with no finite logit gives NaN, as in cross_entropy. `entropy` and
+ * `saved` may be NULL; saved (n, 4) is what the backward needs of each row. The
+ * workspace: oxi_token_logp_workspace bytes, 16-byte aligned, that this call alone
+ * uses until the stream has passed it, or NULL to take it from the caching allocator
+ * (a call under graph capture passes its own). */
+int oxi_token_logp_fwd(const float* logits, const int64_t* ids, float* logp, float* entropy, float* saved,
+                       void* workspace, int64_t n, int64_t c, float temperature);
+/* dlogits (n, c) = gloss[0] times the sum of glogp d logp and gentropy d entropy (n
+ * floats each; one of them may be NULL, for none; gloss NULL: 1), from the saved floats
+ * of oxi_token_logp_fwd, oxi_policy_loss_fwd or oxi_preference_loss_fwd over the same
+ * logits, ids and temperature. Padded rows get zeros, and so do rows whose gradients
+ * are 0, whose logits are not read. Takes no workspace. */
+int oxi_token_logp_bwd(const float* logits, const int64_t* ids, const float* saved, const float* glogp,
+                       const float* gentropy, const float* gloss, float* dlogits, int64_t n, int64_t c,
+                       float temperature);
+int oxi_token_logp_workspace(int64_t n, int64_t c, int64_t* bytes);
+
+/* The clipped policy loss. For the row's chosen class, with r = exp(logp - old_logp)
+ * and the advantage A:
+ *   s = min(r A, clip(r, 1 - clip_low, 1 + clip_high) A); with clip_max, where A < 0,
+ *       at least clip_max A
+ *   k = exp(d) - 1 - d, d = ref_logp - logp
+ *   row = -s + kl_coef k - entropy_coef entropy
+ *   loss = sum of w row / divisor
+ * All per-row operands are n floats. old_logp NULL: r = 1 (the policy that sampled).
+ * ref_logp NULL: no k. weights NULL: w = 1; a row of weight 0 counts as padding.
+ * clip_high may be inf; clip_max 0: none. kl_coef 0 (entropy_coef 0) leaves its term
+ * out of the loss, not out of `rows`. The divisor is the number of counted rows for
+ * their mean.
+ * out (4 floats): sums of w/divisor times the rows' loss, k, entropy, and whether s is
+ * bounded (the clipped share), in 64 bits in a fixed order; rows (4, n): the same for
+ * each row, without w; logp (n, may be NULL). Padded rows are 0 in all of them.
+ * coef (2, n): the loss's derivatives by each row's logp and entropy, and saved (n, 4),
+ * go to the backward: for an upstream gradient gloss[0] it is
+ *   oxi_token_logp_bwd(logits, ids, saved, coef, entropy_coef ? coef + n : NULL, gloss, ..)
+ * With `dlogits` (n, c) set, the call also writes that for an upstream of 1. The
+ * workspace as above, oxi_policy_loss_workspace bytes. */
+int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* advantages, const float* old_logp,
+                        const float* ref_logp, const float* weights, float* out, float* rows, float* logp, float* coef,
+                        float* saved, float* dlogits, void* workspace, int64_t n, int64_t c, float temperature,
+                        float clip_low, float clip_high, float clip_max, float kl_coef, float entropy_coef,
+                        float divisor);
+int oxi_policy_loss_workspace(int64_t n, int64_t c, int64_t* bytes);
+
+/* The preference loss of pairs of sequences. `starts` (2 pairs + 1, int64 on the
+ * device, from 0 to at most n, not decreasing): sequence s is rows starts[s] ..
+ * starts[s + 1] - 1; sequence 2p is pair p's chosen one, 2p + 1 its rejected one. Rows
+ * outside of them and rows with a negative id (the prompt's tokens) are padding, as
+ * above. With S the sum of logp (T = 1) over a sequence's counted rows, R that of
+ * ref_logp (n; NULL: 0), both divided by their count where `average` is set:
+ *   u = beta ((S_c - R_c) - (S_r - R_r)) - margin
+ *   SIGMOID: (1 - smoothing) log(1 + exp(-u)) + smoothing log(1 + exp(u))
+ *   HINGE: max(0, 1 - u);  IPO: (u/beta - 1/(2 beta))^2
+ * pair_loss (pairs); loss (1 float): their mean, 0 without pairs; seq_logp (2 pairs):
+ * S. A sequence without counted rows has S = 0. coef (n: the loss's derivative by each
+ * row's logp) and saved (n, 4) go to oxi_token_logp_bwd; with `dlogits` (n, c) set the
+ * call also writes the gradient for an upstream of 1. A sequence whose bounds lie
+ * outside [0, n] or decrease raises the device guard flag and is empty. The workspace
+ * as above, oxi_preference_loss_workspace bytes. */
+enum { OXI_PREFERENCE_SIGMOID = 0, OXI_PREFERENCE_HINGE = 1, OXI_PREFERENCE_IPO = 2 };
+int oxi_preference_loss_fwd(const float* logits, const int64_t* ids, const int64_t* starts, const float* ref_logp,
+                            float* loss, float* pair_loss, float* seq_logp, float* coef, float* saved, float* dlogits,
+                            void* workspace, int64_t n, int64_t c, int64_t pairs, int kind, int average, float beta,
+                            float margin, float smoothing);
+int oxi_preference_loss_workspace(int64_t n, int64_t c, int64_t* bytes);
+
+/* ------------------------------------------------------------------------ */
 /* Verification of drafted tokens. No counterpart in the reference.          */
 
 /* Checks the tokens that a small model drafted against the probabilities of
@@ -657,6 +732,30 @@ int oxi_sgd_step_multi(const oxi_sgd_slice* slices, int count,
 int oxi_adamw_step_multi(const oxi_adamw_slice* slices, int count,
                          float lr, float beta1, float beta2, float eps,
                          float weight_decay, int decoupled);
+
+/* ------------------------------------------------------------------------ */
+/* Gradient clipping over a whole parameter list.                            */
+
+/* One gradient tensor: n contiguous floats, and where its clipped values go. */
+typedef struct oxi_grad_slice {
+  const float* g;
+  float* out; /* may be g; unused by oxi_grad_norm */
+  int64_t n;
+} oxi_grad_slice;
+
+/* total[0] (a double on the device): the joint norm of all slices' elements,
+ * (sum |g|^p)^(1/p) for norm_type p = 1 or 2, max |g| for an infinite one (which
+ * passes NaN over, as OXI_REDUCE_MAX does; -inf where there is no number). Summed in
+ * 64 bits in a fixed order. The workspace: oxi_grad_norm_workspace bytes, 8-byte
+ * aligned, or NULL as above. The norms of clip_grad_norm_
+ * (python/oxitorch/optim.py:248-299), one tensor at a time there. */
+int oxi_grad_norm(const oxi_grad_slice* slices, int count, double norm_type, double* total, void* workspace);
+int oxi_grad_norm_workspace(const oxi_grad_slice* slices, int count, int64_t* bytes);
+/* Clips by that norm, which is read on the device: out = g * (float)(max_norm / (total +
+ * 1e-6)) where that factor is below 1, else out = g (nothing is done in place). Slices
+ * must not overlap one another (`out` may be the slice's own g). The scaling of
+ * clip_grad_norm_. */
+int oxi_grad_clip(const oxi_grad_slice* slices, int count, const double* total, double max_norm);
 
 #ifdef __cplusplus
 }

@@ -34,6 +34,7 @@ lib = ctypes.CDLL(str(LIB_PATH))
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 c_float = ctypes.c_float
+c_double = ctypes.c_double
 c_size = ctypes.c_size_t
 vp = ctypes.c_void_p
 P_i64 = ctypes.POINTER(ctypes.c_int64)
@@ -48,6 +49,7 @@ REDUCE = ["sum", "mean", "max", "min", "argmax", "argmin", "norm"]
 NORM_VJP = {"ref": 0, "exact": 1}
 GELU = {"tanh": 0, "none": 1, "erf": 1}
 ROTARY = {"half": 0, "interleaved": 1}
+PREFERENCE = {"sigmoid": 0, "hinge": 1, "ipo": 2}  # OXI_PREFERENCE_*
 DISTILL_MAX_TOP = 1024  # OXI_DISTILL_MAX_TOP
 ACT = {"none": -1, "gelu_tanh": 0, "gelu_erf": 1, "silu": 2, "softmax": 3, "log_softmax": 4}
 
@@ -109,6 +111,13 @@ _SIGS = {
     "oxi_distill_bwd": [vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float, c_float],
     "oxi_distill_fwd_counted": [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float],
     "oxi_distill_bwd_counted": [vp, vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_float],
+    "oxi_token_logp_fwd": [vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_float],
+    "oxi_token_logp_bwd": [vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_float],
+    "oxi_token_logp_workspace": [c_i64, c_i64, P_i64],
+    "oxi_policy_loss_fwd": [vp] * 13 + [c_i64, c_i64] + [c_float] * 7,
+    "oxi_policy_loss_workspace": [c_i64, c_i64, P_i64],
+    "oxi_preference_loss_fwd": [vp] * 11 + [c_i64, c_i64, c_i64, c_int, c_int] + [c_float] * 3,
+    "oxi_preference_loss_workspace": [c_i64, c_i64, P_i64],
     "oxi_verify_drafts": [vp, vp, vp, vp, vp, vp, vp, vp, c_i64, c_i64, c_i64],
     "oxi_verify_drafts_workspace": [c_i64, c_i64, P_i64],
     "oxi_index_select": [vp, c_i64, c_i64, c_i64, vp, c_i64, vp],
@@ -125,6 +134,9 @@ _SIGS = {
     "oxi_masked_select": [vp, P_i64, vp, P_i64, P_i64, c_int, ctypes.POINTER(vp), ctypes.POINTER(c_i64), vp],
     "oxi_masked_select_record_bytes": [P_i64, c_int, ctypes.POINTER(c_i64)],
     "oxi_masked_select_bwd": [vp, P_i64, c_int, vp, c_i64, vp, P_i64, c_i64],
+    "oxi_grad_norm": [vp, c_int, c_double, vp, vp],
+    "oxi_grad_norm_workspace": [vp, c_int, P_i64],
+    "oxi_grad_clip": [vp, c_int, vp, c_double],
     "oxi_sgd_step": [vp, vp, vp, vp, c_i64, c_float, c_float, c_int],
     "oxi_adamw_step": [vp, vp, vp, vp, vp, c_i64, c_float, c_float, c_float, c_float, c_float, c_int, c_i64],
     "oxi_sgd_step_multi": [vp, c_int, c_float, c_float, c_int],
@@ -556,6 +568,74 @@ def distill_bwd(logits: DeviceArray, ids: DeviceArray, top: DeviceArray, lse: De
     return d
 
 
+def token_logp_fwd(logits: DeviceArray, ids: DeviceArray, temperature=1.0, need_entropy=False, workspace=None):
+    """(logp, entropy or None, saved): log-probabilities of the chosen classes
+    (ids int64, negative: padding), the rows' entropies, and what the backward needs."""
+    n, c = logits.shape
+    logp, saved = DeviceArray((n,)), DeviceArray((n, 4))
+    entropy = DeviceArray((n,)) if need_entropy else None
+    call("oxi_token_logp_fwd", logits.ptr, ids.ptr, logp.ptr, entropy.ptr if entropy else None, saved.ptr,
+         workspace.ptr if workspace else None, n, c, temperature)
+    return logp, entropy, saved
+
+
+def token_logp_bwd(logits: DeviceArray, ids: DeviceArray, saved: DeviceArray, glogp: DeviceArray | None,
+                   gentropy: DeviceArray | None = None, gloss: DeviceArray | None = None, temperature=1.0) -> DeviceArray:
+    n, c = logits.shape
+    d = DeviceArray((n, c))
+    call("oxi_token_logp_bwd", logits.ptr, ids.ptr, saved.ptr, glogp.ptr if glogp else None,
+         gentropy.ptr if gentropy else None, gloss.ptr if gloss else None, d.ptr, n, c, temperature)
+    return d
+
+
+def _workspace_bytes(name, *args) -> int:
+    n = c_i64(0)
+    call(name, *args, ctypes.byref(n))
+    return n.value
+
+
+def token_logp_workspace(n: int, c: int) -> int:
+    return _workspace_bytes("oxi_token_logp_workspace", n, c)
+
+
+def policy_loss_workspace(n: int, c: int) -> int:
+    return _workspace_bytes("oxi_policy_loss_workspace", n, c)
+
+
+def preference_loss_workspace(n: int, c: int) -> int:
+    return _workspace_bytes("oxi_preference_loss_workspace", n, c)
+
+
+def policy_loss_fwd(logits: DeviceArray, ids: DeviceArray, advantages: DeviceArray, old_logp=None, ref_logp=None,
+                    weights=None, temperature=1.0, clip=(0.2, 0.2), clip_max=0.0, kl_coef=0.0, entropy_coef=0.0,
+                    divisor=1.0, need_grad=False, workspace=None):
+    """(out, rows, logp, coef, saved, dlogits or None) of oxi_policy_loss_fwd."""
+    n, c = logits.shape
+    out, rows, logp = DeviceArray((4,)), DeviceArray((4, n)), DeviceArray((n,))
+    coef, saved = DeviceArray((2, n)), DeviceArray((n, 4))
+    d = DeviceArray((n, c)) if need_grad else None
+    call("oxi_policy_loss_fwd", logits.ptr, ids.ptr, advantages.ptr, *(a.ptr if a else None for a in
+         (old_logp, ref_logp, weights)), out.ptr, rows.ptr, logp.ptr, coef.ptr, saved.ptr, d.ptr if d else None,
+         workspace.ptr if workspace else None, n, c, temperature, clip[0], clip[1], clip_max, kl_coef, entropy_coef,
+         divisor)
+    return out, rows, logp, coef, saved, d
+
+
+def preference_loss_fwd(logits: DeviceArray, ids: DeviceArray, starts: DeviceArray, ref_logp=None, kind="sigmoid",
+                        average=False, beta=0.1, margin=0.0, smoothing=0.0, need_grad=False, workspace=None):
+    """(loss, pair_loss, seq_logp, coef, saved, dlogits or None) of
+    oxi_preference_loss_fwd; starts (2 * pairs + 1) int64."""
+    n, c = logits.shape
+    pairs = (starts.size - 1) // 2
+    loss, pair_loss, seq_logp = DeviceArray((1,)), DeviceArray((pairs,)), DeviceArray((2 * pairs,))
+    coef, saved = DeviceArray((n,)), DeviceArray((n, 4))
+    d = DeviceArray((n, c)) if need_grad else None
+    call("oxi_preference_loss_fwd", logits.ptr, ids.ptr, starts.ptr, ref_logp.ptr if ref_logp else None, loss.ptr,
+         pair_loss.ptr, seq_logp.ptr, coef.ptr, saved.ptr, d.ptr if d else None, workspace.ptr if workspace else None,
+         n, c, pairs, PREFERENCE[kind], int(bool(average)), beta, margin, smoothing)
+    return loss, pair_loss, seq_logp, coef, saved, d
+
+
 def verify_drafts_workspace(batch: int, vocab: int) -> int:
     n = c_i64(0)
     call("oxi_verify_drafts_workspace", batch, vocab, ctypes.byref(n))
@@ -736,6 +816,33 @@ class SgdSlice(ctypes.Structure):
 class AdamWSlice(ctypes.Structure):
     """oxi_adamw_slice"""
     _fields_ = [("p", vp), ("g", vp), ("m", vp), ("v", vp), ("p_out", vp), ("n", c_i64), ("t", c_i64)]
+
+
+class GradSlice(ctypes.Structure):
+    """oxi_grad_slice"""
+    _fields_ = [("g", vp), ("out", vp), ("n", c_i64)]
+
+
+def _grad_slices(grads, outs=None):
+    return slice_array(GradSlice, [(g.ptr, o.ptr if o else None, g.size) for g, o in zip(grads, outs or [None] * len(grads))])
+
+
+def grad_norm_workspace(grads) -> int:
+    return _workspace_bytes("oxi_grad_norm_workspace", _grad_slices(grads), len(grads))
+
+
+def grad_norm(grads, norm_type=2.0, workspace=None, total: DeviceArray | None = None) -> DeviceArray:
+    """The joint norm of a list of gradients, one float64 on the device."""
+    total = total if total is not None else DeviceArray((1,), np.float64)
+    call("oxi_grad_norm", _grad_slices(grads), len(grads), norm_type, total.ptr, workspace.ptr if workspace else None)
+    return total
+
+
+def grad_clip(grads, total: DeviceArray, max_norm, outs=None):
+    """The gradients clipped by their joint norm, in `outs` (fresh ones; pass `grads` for in place)."""
+    outs = outs if outs is not None else [DeviceArray(g.shape) for g in grads]
+    call("oxi_grad_clip", _grad_slices(grads, outs), len(grads), total.ptr, max_norm)
+    return outs
 
 
 def slice_array(cls, rows):

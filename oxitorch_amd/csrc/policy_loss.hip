@@ -1,0 +1,144 @@
+// The clipped policy loss over rows of logits with a KL term and an entropy bonus,
+// and its gradient. For a row's chosen token, with r = exp(logp - old) and the
+// advantage A:
+//
+//   s = min(r A, clip(r, 1 - low, 1 + high) A), for A < 0 at least most A
+//   k = e^d - 1 - d, d = ref - logp
+//   row = -s + kl k - ent H,   loss = sum w row / divisor
+//   d row/d logp = -[s is r A] r A - kl (e^d - 1),   d row/d H = -ent
+//
+// (the mathematics of logp, H and their gradients is in token_rows.h). All of a row's
+// own arithmetic is in 64 bits: k of a policy near its reference is the small rest of
+// terms that cancel, and a ratio next to an edge of the clipping must fall on the side
+// that the definition has it on.
+#include <cmath>
+
+#include "token_rows.h"
+
+namespace oxi {
+namespace {
+
+struct PolicyOp {
+  const float *adv, *old, *ref, *weights;
+  float *rows, *logp, *coef, *saved;
+  int64_t n;
+  double low, high, most;  // the ratio's bounds, and the factor of a negative advantage that bounds s (0: none)
+  double kl, ent, inv_div;
+
+  __device__ __forceinline__ void finish(int64_t row, const RowStats& r, bool lead) const {
+    const double A = (double)adv[row];
+    const double ratio = old ? exp64(r.logp - (double)old[row]) : 1.0;
+    const double free = A == 0.0 ? 0.0 : ratio * A;
+    const double bounded = (ratio < low ? low : ratio > high ? high : ratio) * A;
+    bool clipped = free > bounded;
+    double s = clipped ? bounded : free;
+    if (most > 0.0 && A < 0.0 && s < most * A) {
+      s = most * A;
+      clipped = true;
+    }
+    double g = clipped ? 0.0 : -free, k = 0.0;
+    double loss = -s;
+    if (ref) {
+      const double d = (double)ref[row] - r.logp;
+      k = d == (double)__builtin_huge_valf() ? d : exp_rest(d);
+      if (kl != 0.0) {
+        g -= kl * (fabs(d) < 0.5 ? k + d : exp64(d) - 1.0);
+        loss += kl * k;
+      }
+    }
+    if (ent != 0.0) loss -= ent * r.entropy;
+    const double w = (weights ? (double)weights[row] : 1.0) * inv_div;
+    if (!lead) return;
+    rows[row] = (float)loss;
+    rows[n + row] = (float)k;
+    rows[2 * n + row] = (float)r.entropy;
+    rows[3 * n + row] = clipped ? 1.f : 0.f;
+    if (logp) logp[row] = (float)r.logp;
+    coef[row] = (float)(g * w);
+    coef[n + row] = (float)(-ent * w);
+    save_row(saved, row, r);
+  }
+  __device__ __forceinline__ void skip(int64_t row) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rows[i * n + row] = 0.f;
+    if (logp) logp[row] = 0.f;
+    coef[row] = coef[n + row] = 0.f;
+    save_nothing(saved, row);
+  }
+};
+
+// out[i] = sum over the rows of w rows[i] / divisor in float64, in a fixed order: one block.
+__global__ __launch_bounds__(1024) void policy_mean_k(const TokenRows in, const float* __restrict__ rows, double inv_div,
+                                                      float* __restrict__ out) {
+  __shared__ double red[1024 / 64];
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  for (int64_t i = threadIdx.x; i < in.n; i += 1024) {
+    const int64_t id = in.ids[i];
+    const float w = in.weights ? in.weights[i] : 1.f;
+    if (id < 0 || id >= in.c || w == 0.f) continue;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] += (double)w * (double)rows[k * in.n + i];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const double v = block_sum<1024>(acc[k], red);
+    if (threadIdx.x == 0) out[k] = (float)(v * inv_div);
+  }
+}
+
+}  // namespace
+}  // namespace oxi
+
+using namespace oxi;
+
+extern "C" {
+
+int oxi_policy_loss_workspace(int64_t n, int64_t c, int64_t* bytes) {
+  if (!bytes) return fail(OXI_INVALID_ARGUMENT, "policy_loss_workspace: NULL result");
+  if (int rc = check_token_rows("policy_loss_workspace", n, c, 1.f)) return rc;
+  *bytes = token_parts_bytes(n, c);
+  return OXI_OK;
+}
+
+int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* advantages, const float* old_logp,
+                        const float* ref_logp, const float* weights, float* out, float* rows, float* logp, float* coef,
+                        float* saved, float* dlogits, void* workspace, int64_t n, int64_t c, float temperature,
+                        float clip_low, float clip_high, float clip_max, float kl_coef, float entropy_coef,
+                        float divisor) {
+  const char* what = "policy_loss_fwd";
+  if (int rc = check_token_rows(what, n, c, temperature)) return rc;
+  if (!(clip_low >= 0.f) || !(clip_high >= 0.f))
+    return fail(OXI_INVALID_ARGUMENT, "%s: the clipping must not be negative, got %g and %g", what, (double)clip_low,
+                (double)clip_high);
+  if (clip_max != 0.f && !(clip_max >= 1.f))
+    return fail(OXI_INVALID_ARGUMENT, "%s: clip_max must be 0 (none) or at least 1, got %g", what, (double)clip_max);
+  if (!std::isfinite(kl_coef) || !std::isfinite(entropy_coef))
+    return fail(OXI_INVALID_ARGUMENT, "%s: the coefficients must be finite", what);
+  if (kl_coef != 0.f && !ref_logp)
+    return fail(OXI_INVALID_ARGUMENT, "%s: a KL term needs the reference's log-probabilities", what);
+  if (!(divisor > 0.f) || std::isinf(divisor))
+    return fail(OXI_INVALID_ARGUMENT, "%s: the divisor must be positive, got %g", what, (double)divisor);
+  if (!out) return fail(OXI_INVALID_ARGUMENT, "%s: out must not be NULL", what);
+  if (n && (!logits || !ids || !advantages || !rows || !coef || !saved))
+    return fail(OXI_INVALID_ARGUMENT, "%s: NULL tensor pointer", what);
+  if (reinterpret_cast<uintptr_t>(workspace) & 15)
+    return fail(OXI_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
+  OXI_CHECK_INIT();
+  if (n == 0) return oxi_fill(out, 4, 0.f);
+  Workspace own(workspace ? 0 : (size_t)token_parts_bytes(n, c));
+  if (!workspace && !own.p) return fail_alloc(what);
+  TokenRows in = token_rows(logits, ids, n, c, temperature);
+  in.weights = weights;
+  const double inv_div = 1.0 / (double)divisor;
+  const PolicyOp op{advantages, old_logp, ref_logp, weights, rows, logp, coef, saved, n, 1.0 - (double)clip_low,
+                    1.0 + (double)clip_high, (double)clip_max, (double)kl_coef, (double)entropy_coef, inv_div};
+  if (int rc = token_rows_joined(in, static_cast<f4*>(workspace ? workspace : own.p), op, what)) return rc;
+  if (dlogits)
+    if (int rc = launch_token_bwd(logits, ids, saved, coef, entropy_coef != 0.f ? coef + n : nullptr, nullptr, dlogits,
+                                  n, c, temperature, what))
+      return rc;
+  policy_mean_k<<<1, 1024, 0, stream()>>>(in, rows, inv_div, out);
+  return check_launch(what);
+}
+
+}  // extern "C"

@@ -1,0 +1,175 @@
+// Rows of logits with one chosen class each, as the losses of post-training take
+// them (token log-probabilities, policy and preference losses):
+//
+//   z = x/T, m = max x, t = (x - m) log2(e)/T, s = sum 2^t
+//   logp = ln 2 t_a - ln s for the chosen class a,  H = ln s - ln 2 (sum 2^t t)/s
+//   dx_j = (gl (d_ja - q_j) - gh q_j (ln q_j + H))/T,  q = 2^t/s
+//
+// for the gradients gl of logp and gh of H. The sums leave the chosen class out, so
+// that 1 - q_a = rest/s and, where a has the largest logit, logp = -log1p(rest) keep
+// their digits for a token that is all but certain; in 32 bits 1 - q_a would be 0
+// or a multiple of 2^-24. Exponentials and a thread's sums of them are in 32 bits,
+// relative to the maximum; what is formed of a row's sums is in 64.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "internal.h"
+#include "launch_limits.h"
+#include "row64.h"
+#include "rowtile.h"
+
+namespace oxi {
+
+// Exponents below this count as this in the products 2^t t, where 2^t is 0: a class
+// at -inf adds 0, not NaN.
+constexpr float LEAST_T = -200.f;
+constexpr double LOG_2 = 0.6931471805599453;
+
+// log(1 + x) for x >= 0 (and NaN).
+__device__ __forceinline__ double log1p64(double x) {
+  if (!(x < 0.4)) return log64(1.0 + x);
+  const double s = x / (2.0 + x), z = s * s;  // |s| < 0.167
+  double p = 1.0 / 23;
+#pragma unroll
+  for (int k = 21; k > 0; k -= 2) p = fma(p, z, scalar(1.0 / k));
+  return 2.0 * s * p;
+}
+
+// The rows of a call, and which of them count.
+struct TokenRows {
+  const float* x;
+  const int64_t* ids;
+  const float* weights;   // a row of weight 0 does not count; NULL: all do
+  const int64_t* starts;  // rows outside [starts[0], starts[sequences]) do not; NULL: all do
+  int64_t sequences;
+  int64_t n;
+  int c;
+  float scale2;  // log2(e)/T
+  double inv_t;
+  int* guard;
+
+  // An id past the classes raises the guard and is padding.
+  __device__ __forceinline__ bool counts(int64_t row, int64_t id) const {
+    if (id >= c && threadIdx.x == 0) atomicOr(guard, 1);
+    return id >= 0 && id < c && (!weights || weights[row] != 0.f) &&
+           (!starts || (row >= starts[0] && row < starts[sequences]));
+  }
+};
+
+struct RowStats {
+  double logp, entropy;
+  float m, rest, total, off;  // off = entropy - ln total
+};
+
+// From the maximum m, the chosen logit xa and the sums over the other classes of 2^t
+// and 2^t t.
+__device__ __forceinline__ RowStats row_stats(float m, float xa, double rest, double et, float scale2, double inv_t) {
+  const float ta = (xa - m) * scale2;
+  const double ea = (double)__builtin_amdgcn_exp2f(ta);
+  const double total = rest + ea;
+  const double d = ((double)xa - (double)m) * inv_t;  // NaN where no class is left
+  const double lt = d == 0.0 ? log1p64(rest) : log64(total);
+  const double mean = (et + ea * (double)fmaxf(ta, LEAST_T)) / total;
+  RowStats r;
+  r.logp = d - lt;
+  r.entropy = lt - LOG_2 * mean;
+  r.m = m;
+  r.rest = (float)rest;
+  r.total = (float)total;
+  r.off = (float)(-LOG_2 * mean);
+  return r;
+}
+
+// What the backward needs of a row: its 4 floats of `saved`.
+__device__ __forceinline__ void save_row(float* saved, int64_t row, const RowStats& r) {
+  *reinterpret_cast<f4u*>(saved + 4 * row) = f4{r.m, r.rest, r.total, r.off};
+}
+__device__ __forceinline__ void save_nothing(float* saved, int64_t row) {
+  *reinterpret_cast<f4u*>(saved + 4 * row) = f4{0.f, 0.f, 1.f, 0.f};
+}
+
+// v with component i at -inf.
+__device__ __forceinline__ f4 drop(const f4& v, int i) {
+  return f4{i == 0 ? NEG_INF : v.x, i == 1 ? NEG_INF : v.y, i == 2 ? NEG_INF : v.z, i == 3 ? NEG_INF : v.w};
+}
+__device__ __forceinline__ f4 put_at(const f4& v, int i, float a) {
+  return f4{i == 0 ? a : v.x, i == 1 ? a : v.y, i == 2 ? a : v.z, i == 3 ? a : v.w};
+}
+
+// How a row of C classes lies: `head` classes, float4s, up to 3 classes more.
+struct RowLay {
+  int head, c4;
+  __device__ __forceinline__ RowLay(const float* row, int C) : head(min(row_head(row, C), C)), c4((C - head) >> 2) {}
+  // The class outside the float4s that thread t takes, or -1.
+  __device__ __forceinline__ int edge(int t, int C) const {
+    const int e = t < 32 ? t : head + 4 * c4 + t - 32;
+    return (t < 32 ? t < head : t < 35 && e < C) ? e : -1;
+  }
+  // The float4 of class a, or -1 outside of them; its component.
+  __device__ __forceinline__ int slot(int a) const { return a >= head && a < head + 4 * c4 ? (a - head) >> 2 : -1; }
+  __device__ __forceinline__ int component(int a) const { return (a - head) & 3; }
+};
+
+// Rows cut into parts of PART_NT * PART_U float4s, a block each.
+constexpr int PART_NT = 256, PART_U = 8;
+inline int64_t row_parts(int64_t c) { return c > 0 ? ceil_div(c, (int64_t)PART_NT * PART_U * 4) : 1; }
+
+// Maximum, sum and sum of 2^t t of each part, the chosen class left out; relative to
+// the part's own maximum.
+int launch_token_parts(const TokenRows& in, f4* parts, const char* what);
+
+// A wave a row: joins its parts; `op` writes what the row gives.
+template <class Op>
+__global__ __launch_bounds__(256) void token_join_k(const TokenRows in, const f4* __restrict__ parts, int np,
+                                                    const Op op) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= in.n) return;
+  const int64_t id = in.ids[row];
+  if (!in.counts(row, id)) {
+    if (lane == 0) op.skip(row);
+    return;
+  }
+  const float xa = in.x[row * in.c + id];
+  const f4* mine = parts + row * np;
+  float m = xa;
+  for (int p = lane; p < np; p += 64) m = fmaxf(m, mine[p].x);
+  m = wave_max(m);
+  double s = 0.0, et = 0.0;
+  for (int p = lane; p < np; p += 64) {
+    const f4 v = mine[p];
+    if (v.y == 0.f) continue;  // nothing finite there
+    const float d = (v.x - m) * in.scale2;
+    const double f = (double)__builtin_amdgcn_exp2f(d);
+    s += f * (double)v.y;
+    et += f * ((double)v.z + (double)fmaxf(d, LEAST_T) * (double)v.y);
+  }
+  s = over_block<64, AddF64>(s, (double*)nullptr);
+  et = over_block<64, AddF64>(et, (double*)nullptr);
+  const RowStats r = row_stats(m, xa, s, et, in.scale2, in.inv_t);
+  op.finish(row, r, lane == 0);
+}
+
+// dx of the rows from their saved floats, for the gradients gl and gh (NULL: none) of
+// their log-probabilities and entropies times gloss[0] (NULL: 1).
+int launch_token_bwd(const float* x, const int64_t* ids, const float* saved, const float* gl, const float* gh,
+                     const float* gloss, float* dx, int64_t n, int64_t c, float temperature, const char* what);
+
+// Whether sizes and temperature can be taken; 0 or an error's code.
+int check_token_rows(const char* what, int64_t n, int64_t c, float temperature);
+TokenRows token_rows(const float* x, const int64_t* ids, int64_t n, int64_t c, float temperature);
+
+// Bytes of the parts of n rows.
+inline int64_t token_parts_bytes(int64_t n, int64_t c) { return n * row_parts(c) * (int64_t)sizeof(f4); }
+
+template <class Op>
+int token_rows_joined(const TokenRows& in, f4* parts, const Op& op, const char* what) {
+  if (int rc = launch_token_parts(in, parts, what)) return rc;
+  token_join_k<Op><<<dim3((unsigned)ceil_div(in.n, 4)), dim3(256), 0, stream()>>>(in, parts, (int)row_parts(in.c), op);
+  return check_launch(what);
+}
+
+}  // namespace oxi
