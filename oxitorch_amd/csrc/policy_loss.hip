@@ -19,13 +19,15 @@ namespace oxi {
 namespace {
 
 struct PolicyOp {
+  static constexpr int READ_MAX = ROWS_MAX;  // the same bits with a gradient and without
   const float *adv, *old, *ref, *weights;
   float *rows, *logp, *coef, *saved;
   int64_t n;
   double low, high, most;  // the ratio's bounds, and the factor of a negative advantage that bounds s (0: none)
   double kl, ent, inv_div;
 
-  __device__ __forceinline__ void finish(int64_t row, const RowStats& r, bool lead) const {
+  // Writes the row's results; the loss's derivatives by its logp and entropy.
+  __device__ __forceinline__ Two finish(int64_t row, const RowStats& r, bool lead) const {
     const double A = (double)adv[row];
     const double ratio = old ? exp64(r.logp - (double)old[row]) : 1.0;
     const double free = A == 0.0 ? 0.0 : ratio * A;
@@ -48,15 +50,17 @@ struct PolicyOp {
     }
     if (ent != 0.0) loss -= ent * r.entropy;
     const double w = (weights ? (double)weights[row] : 1.0) * inv_div;
-    if (!lead) return;
+    const Two by{(float)(g * w), (float)(-ent * w)};
+    if (!lead) return by;
     rows[row] = (float)loss;
     rows[n + row] = (float)k;
     rows[2 * n + row] = (float)r.entropy;
     rows[3 * n + row] = clipped ? 1.f : 0.f;
     if (logp) logp[row] = (float)r.logp;
-    coef[row] = (float)(g * w);
-    coef[n + row] = (float)(-ent * w);
+    coef[row] = by.a;
+    coef[n + row] = by.b;
     save_row(saved, row, r);
+    return by;
   }
   __device__ __forceinline__ void skip(int64_t row) const {
 #pragma unroll
@@ -66,6 +70,12 @@ struct PolicyOp {
     save_nothing(saved, row);
   }
 };
+
+bool launch_rows(const TokenRows& in, const PolicyOp& op, float* dx, bool ent) {
+  const bool nt = nt_stream_stores(in.n * in.c * 4);
+  if (ent) return nt ? launch_token_rows_as<true, true, true>(in, op, dx) : launch_token_rows_as<true, true, false>(in, op, dx);
+  return nt ? launch_token_rows_as<true, false, true>(in, op, dx) : launch_token_rows_as<true, false, false>(in, op, dx);
+}
 
 // out[i] = sum over the rows of w rows[i] / divisor in float64, in a fixed order: one block.
 __global__ __launch_bounds__(1024) void policy_mean_k(const TokenRows in, const float* __restrict__ rows, double inv_div,
@@ -132,11 +142,15 @@ int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* ad
   const double inv_div = 1.0 / (double)divisor;
   const PolicyOp op{advantages, old_logp, ref_logp, weights, rows, logp, coef, saved, n, 1.0 - (double)clip_low,
                     1.0 + (double)clip_high, (double)clip_max, (double)kl_coef, (double)entropy_coef, inv_div};
-  if (int rc = token_rows_joined(in, static_cast<f4*>(workspace ? workspace : own.p), op, what)) return rc;
-  if (dlogits)
-    if (int rc = launch_token_bwd(logits, ids, saved, coef, entropy_coef != 0.f ? coef + n : nullptr, nullptr, dlogits,
-                                  n, c, temperature, what))
-      return rc;
+  if (dlogits && launch_rows(in, op, dlogits, entropy_coef != 0.f)) {
+    if (int rc = check_launch(what)) return rc;
+  } else {
+    if (int rc = token_rows_read(in, static_cast<f4*>(workspace ? workspace : own.p), op, what)) return rc;
+    if (dlogits)
+      if (int rc = launch_token_bwd(logits, ids, saved, coef, entropy_coef != 0.f ? coef + n : nullptr, nullptr,
+                                    dlogits, n, c, temperature, what))
+        return rc;
+  }
   policy_mean_k<<<1, 1024, 0, stream()>>>(in, rows, inv_div, out);
   return check_launch(what);
 }

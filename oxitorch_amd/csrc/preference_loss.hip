@@ -19,13 +19,15 @@ namespace oxi {
 namespace {
 
 struct PreferenceOp {
+  static constexpr int READ_MAX = ROWS_MAX_READ;
   double* logp;
   float *coef, *saved;
-  __device__ __forceinline__ void finish(int64_t row, const RowStats& r, bool lead) const {
-    if (!lead) return;
+  __device__ __forceinline__ Two finish(int64_t row, const RowStats& r, bool lead) const {
+    if (!lead) return {0.f, 0.f};
     logp[row] = r.logp;
     coef[row] = 0.f;  // a counted row's own comes with its pair
     save_row(saved, row, r);
+    return {0.f, 0.f};
   }
   __device__ __forceinline__ void skip(int64_t row) const {
     logp[row] = 0.0;
@@ -174,7 +176,7 @@ int oxi_preference_loss_fwd(const float* logits, const int64_t* ids, const int64
     TokenRows in = token_rows(logits, ids, n, c, 1.f);
     in.starts = starts;
     in.sequences = 2 * pairs;
-    if (int rc = token_rows_joined(in, parts, PreferenceOp{logp, coef, saved}, what)) return rc;
+    if (int rc = token_rows_read(in, parts, PreferenceOp{logp, coef, saved}, what)) return rc;
   }
   if (pairs) {
     const PairArgs g{starts, ids, logp, ref_logp, pair_loss, seq_logp, coef, n, pairs, (int)c, kind, average ? 1 : 0,

@@ -121,12 +121,14 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
 }
 
 struct LogpOp {
+  static constexpr int READ_MAX = ROWS_MAX_READ;
   float *logp, *entropy, *saved;
-  __device__ __forceinline__ void finish(int64_t row, const RowStats& r, bool lead) const {
-    if (!lead) return;
+  __device__ __forceinline__ Two finish(int64_t row, const RowStats& r, bool lead) const {
+    if (!lead) return {0.f, 0.f};
     logp[row] = (float)r.logp;
     if (entropy) entropy[row] = (float)r.entropy;
     if (saved) save_row(saved, row, r);
+    return {0.f, 0.f};
   }
   __device__ __forceinline__ void skip(int64_t row) const {
     logp[row] = 0.f;
@@ -218,7 +220,7 @@ int oxi_token_logp_fwd(const float* logits, const int64_t* ids, float* logp, flo
   Workspace own(workspace ? 0 : (size_t)token_parts_bytes(n, c));
   if (!workspace && !own.p) return fail_alloc(what);
   f4* parts = static_cast<f4*>(workspace ? workspace : own.p);
-  return token_rows_joined(token_rows(logits, ids, n, c, temperature), parts, LogpOp{logp, entropy, saved}, what);
+  return token_rows_read(token_rows(logits, ids, n, c, temperature), parts, LogpOp{logp, entropy, saved}, what);
 }
 
 int oxi_token_logp_bwd(const float* logits, const int64_t* ids, const float* saved, const float* glogp,

@@ -53,7 +53,7 @@ struct TokenRows {
 
   // An id past the classes raises the guard and is padding.
   __device__ __forceinline__ bool counts(int64_t row, int64_t id) const {
-    if (id >= c && threadIdx.x == 0) atomicOr(guard, 1);
+    if (id >= c && (threadIdx.x & 63) == 0) atomicOr(guard, 1);
     return id >= 0 && id < c && (!weights || weights[row] != 0.f) &&
            (!starts || (row >= starts[0] && row < starts[sequences]));
   }
@@ -158,6 +158,142 @@ __global__ __launch_bounds__(256) void token_join_k(const TokenRows in, const f4
 int launch_token_bwd(const float* x, const int64_t* ids, const float* saved, const float* gl, const float* gh,
                      const float* gloss, float* dx, int64_t n, int64_t c, float temperature, const char* what);
 
+// ---------------------------------------------------------------------------
+// A row a group of RT threads (a wave, four to a block, or a block), held in
+// registers as NV float4s a thread: the logits cross HBM once for the loss and its
+// gradient. Every thread works the row's few 64-bit formulas out by itself.
+
+// What a gradient at a class takes besides 2^t and t.
+struct RowGrad {
+  float alpha, beta, chosen;
+  // For the gradients gl of logp and gh of the entropy.
+  __device__ __forceinline__ RowGrad(const RowStats& r, float xa, float scale2, float inv_t, float gl, float gh) {
+    const float a = gl * inv_t, b = gh * inv_t;
+    alpha = -(a + b * r.off) / r.total;
+    beta = -b * (float)LOG_2 / r.total;
+    const float z = (xa - r.m) * scale2;
+    const float q = __builtin_amdgcn_exp2f(z) / r.total;
+    chosen = a * (r.rest / r.total) - (gh != 0.f ? b * q * fmaf((float)LOG_2, fmaxf(z, LEAST_T), r.off) : 0.f);
+  }
+};
+
+constexpr int rows_block(int rt) { return rt == 64 ? 256 : rt; }
+// Waves a SIMD that the registers must allow.
+constexpr int rows_waves(int nv) { return nv >= 10 ? 4 : 8; }
+
+template <int RT, int NV, bool GRAD, bool ENT, bool NTS, class Op>
+__global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(4))) void token_rows_k(
+    const TokenRows in, const Op op, float* __restrict__ dx) {
+  __shared__ __align__(8) float lds[3 * (RT / 64)];
+  const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
+  const int64_t row = RT == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  if (RT == 64 && row >= in.n) return;
+  const int C = in.c;
+  const float* xr = in.x + row * C;
+  float* dr = dx + row * C;
+  const int64_t id64 = in.ids[row];
+  const RowLay lay(xr, C);
+  auto put = [&](const f4& d, int c) {
+    f4u* const p = reinterpret_cast<f4u*>(reinterpret_cast<char*>(dr + lay.head) + (uint32_t)c * 16u);
+    if constexpr (NTS) __builtin_nontemporal_store(d, p);
+    else *p = d;
+  };
+  const int e = lay.edge(t, C);
+  if (!in.counts(row, id64)) {
+    if (t == 0) op.skip(row);
+    if constexpr (GRAD) {
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+        if (q * RT + t < lay.c4) put(f4{0.f, 0.f, 0.f, 0.f}, q * RT + t);
+      if (e >= 0) dr[e] = 0.f;
+    }
+    return;
+  }
+  const int id = (int)id64;
+  const int at = lay.slot(id), comp = lay.component(id);
+  const int at_q = at >= 0 ? at / RT : -1, at_t = at >= 0 ? at % RT : -1;
+  const float xa = xr[id];
+  f4 v[NV];
+#pragma unroll
+  for (int q = 0; q < NV; ++q)
+    v[q] = ld_stream(reinterpret_cast<const f4*>(reinterpret_cast<const char*>(xr + lay.head) +
+                                                 (uint32_t)min(q * RT + t, lay.c4 - 1) * 16u));
+  float v1 = e >= 0 && e != id ? xr[e] : NEG_INF;
+  float m = fmaxf(v1, xa);
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    if (q * RT + t >= lay.c4) v[q] = f4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+    if (q == at_q && t == at_t) v[q] = drop(v[q], comp);
+    m = fmaxf(m, max4(v[q]));
+  }
+  m = over_block<RT, MaxF32>(m, lds);
+  // With an entropy's gradient the registers keep t, else 2^t.
+  float s = 0.f, et = 0.f;
+  auto add = [&](float x) {
+    const float z = (x - m) * in.scale2;
+    const float p = __builtin_amdgcn_exp2f(z);
+    s += p;
+    et = fmaf(p, fmaxf(z, LEAST_T), et);
+    return ENT ? z : p;
+  };
+#pragma unroll
+  for (int q = 0; q < NV; ++q) v[q] = f4{add(v[q].x), add(v[q].y), add(v[q].z), add(v[q].w)};
+  v1 = add(v1);
+  const Two both = over_block<RT, Both<AddF32>>(Two{s, et}, reinterpret_cast<Two*>(lds + RT / 64));
+  const RowStats r = row_stats(m, xa, (double)both.a, (double)both.b, in.scale2, in.inv_t);
+  const Two k = op.finish(row, r, t == 0);
+  if constexpr (GRAD) {
+    const RowGrad g(r, xa, in.scale2, (float)in.inv_t, k.a, ENT ? k.b : 0.f);
+    auto grad = [&](float z) {
+      // its exponential is formed again: held from the sums on, it would take the registers twice
+      if constexpr (ENT) asm("" : "+v"(z));
+      if constexpr (ENT) return __builtin_amdgcn_exp2f(z) * fmaf(g.beta, fmaxf(z, LEAST_T), g.alpha);
+      else return z * g.alpha;
+    };
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      if (q * RT + t >= lay.c4) continue;
+      f4 d = f4{grad(v[q].x), grad(v[q].y), grad(v[q].z), grad(v[q].w)};
+      if (q == at_q && t == at_t) d = put_at(d, comp, g.chosen);
+      put(d, q * RT + t);
+    }
+    if (e >= 0) dr[e] = e == id ? g.chosen : grad(v1);
+  }
+}
+
+// The row kernel for c classes: as few threads as hold the row; false past ROWS_MAX of
+// them (without a gradient past Op::READ_MAX) and under 8, where none does.
+constexpr int ROWS_MAX = 65536, ROWS_MAX_READ = PART_NT * PART_U * 4;
+template <bool GRAD, bool ENT, bool NTS, class Op>
+bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx) {
+  const int c4 = in.c / 4;  // at most
+  if (in.c < 8 || in.c > (GRAD ? ROWS_MAX : Op::READ_MAX)) return false;
+#define OXI_TR(RT, NV)                                                                                        \
+  if constexpr (GRAD || RT * NV * 4 <= Op::READ_MAX) if (c4 <= RT * NV) {                                    \
+    token_rows_k<RT, NV, GRAD, ENT, NTS, Op>                                                                  \
+        <<<dim3((unsigned)(RT == 64 ? ceil_div(in.n, 4) : in.n)), dim3(rows_block(RT)), 0, stream()>>>(in, op, dx); \
+    return true;                                                                                              \
+  }
+  OXI_TR(64, 2)
+  OXI_TR(64, 4)
+  OXI_TR(64, 8)
+  OXI_TR(256, 4)
+  OXI_TR(256, 8)
+  OXI_TR(256, 12)
+  OXI_TR(256, 16)
+  OXI_TR(512, 10)
+  OXI_TR(512, 12)
+  OXI_TR(512, 14)
+  OXI_TR(512, 16)
+  OXI_TR(1024, 10)
+  OXI_TR(1024, 12)
+  OXI_TR(1024, 13)
+  OXI_TR(1024, 14)
+  OXI_TR(1024, 16)
+#undef OXI_TR
+  return false;
+}
+
 // Whether sizes and temperature can be taken; 0 or an error's code.
 int check_token_rows(const char* what, int64_t n, int64_t c, float temperature);
 TokenRows token_rows(const float* x, const int64_t* ids, int64_t n, int64_t c, float temperature);
@@ -165,8 +301,10 @@ TokenRows token_rows(const float* x, const int64_t* ids, int64_t n, int64_t c, f
 // Bytes of the parts of n rows.
 inline int64_t token_parts_bytes(int64_t n, int64_t c) { return n * row_parts(c) * (int64_t)sizeof(f4); }
 
+// The rows' results without a gradient.
 template <class Op>
-int token_rows_joined(const TokenRows& in, f4* parts, const Op& op, const char* what) {
+int token_rows_read(const TokenRows& in, f4* parts, const Op& op, const char* what) {
+  if (launch_token_rows_as<false, false, false>(in, op, nullptr)) return check_launch(what);
   if (int rc = launch_token_parts(in, parts, what)) return rc;
   token_join_k<Op><<<dim3((unsigned)ceil_div(in.n, 4)), dim3(256), 0, stream()>>>(in, parts, (int)row_parts(in.c), op);
   return check_launch(what);
