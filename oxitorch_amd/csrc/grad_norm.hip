@@ -3,7 +3,7 @@
 //   total = (sum |g|^p)^(1/p), p = 1 or 2, or max |g|
 //   out = g * min(1, max_norm / (total + 1e-6))
 //
-// Every tensor is cut into chunks of CHUNK floats, a block each; the tensors' places
+// Every tensor is cut into chunks, a block each; the tensors' places
 // travel in the kernel arguments, up to MOST_SLICES a launch. The terms are squared and
 // summed in 64 bits (no overflow, and a sum over 10^9 terms keeps its digits), a sum a
 // chunk, then one block adds the chunks' in a fixed order. The clipping reads total on
@@ -20,7 +20,14 @@ namespace {
 
 constexpr int NT = 256;
 constexpr int UNROLL = 4;               // float4s in flight a thread
-constexpr int CHUNK = NT * UNROLL * 4;  // floats
+constexpr int STEP = NT * UNROLL * 4;   // floats that a block has in flight
+// Floats a block of the norm's: STEP, or many of them where that still fills the chip
+// many times over, so that the chunks' sums are few.
+constexpr int LONG_STEPS = 8;
+constexpr int64_t MANY = (int64_t)1 << 25;
+inline int64_t chunk_of(int64_t total) { return total >= MANY ? (int64_t)STEP * LONG_STEPS : STEP; }
+// Of the clipping's: loads in a loop would wait behind the stores before them.
+constexpr int CLIP_UNROLL = 2, CLIP_CHUNK = NT * CLIP_UNROLL * 4;
 constexpr int MOST_SLICES = 96;
 
 struct Slices {
@@ -29,6 +36,7 @@ struct Slices {
   int64_t n[MOST_SLICES];
   uint32_t end[MOST_SLICES];  // blocks up to and with slice s
   int count;
+  int64_t chunk;
 };
 
 __device__ __forceinline__ int slice_of(const Slices& a, uint32_t b) {
@@ -42,12 +50,13 @@ __device__ __forceinline__ int slice_of(const Slices& a, uint32_t b) {
 }
 
 // KIND 0: max, 1: sum, 2: sum of squares. parts[first + block] = the chunk's.
-template <int KIND>
+// AGAIN: plain loads, for what the clipping then finds in the Infinity Cache.
+template <int KIND, bool AGAIN>
 __global__ __launch_bounds__(NT) void norm_part_k(const Slices a, double* __restrict__ parts, int64_t first) {
   __shared__ double red[NT / 64];
   const int s = slice_of(a, blockIdx.x);
-  const int64_t n = a.n[s];
-  const int64_t e0 = (int64_t)(blockIdx.x - (s ? a.end[s - 1] : 0u)) * CHUNK;
+  int64_t e0 = (int64_t)(blockIdx.x - (s ? a.end[s - 1] : 0u)) * a.chunk;
+  const int64_t n = min(a.n[s], e0 + a.chunk);
   const float* g = a.g[s];
   double acc = KIND == 0 ? (double)NEG_INF : 0.0;
   auto add = [&](float v) {
@@ -55,19 +64,23 @@ __global__ __launch_bounds__(NT) void norm_part_k(const Slices a, double* __rest
     else if constexpr (KIND == 1) acc += (double)fabsf(v);
     else acc = fma((double)v, (double)v, acc);
   };
+  for (; e0 + STEP <= n; e0 += STEP) {
+    f4 v[UNROLL];
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const int64_t e = e0 + (int64_t)(u * NT + threadIdx.x) * 4;
-    if (e + 4 <= n) {
-      const f4 v = *reinterpret_cast<const f4u*>(g + e);
-      add(v.x);
-      add(v.y);
-      add(v.z);
-      add(v.w);
-    } else {
-      for (int64_t i = e; i < n; ++i) add(g[i]);
+    for (int u = 0; u < UNROLL; ++u) {
+      const f4u* p = reinterpret_cast<const f4u*>(g + e0) + u * NT + threadIdx.x;
+      if constexpr (AGAIN) v[u] = *p;
+      else v[u] = __builtin_nontemporal_load(p);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      add(v[u].x);
+      add(v[u].y);
+      add(v[u].z);
+      add(v[u].w);
     }
   }
+  for (int64_t e = e0 + threadIdx.x; e < n; e += NT) add(g[e]);
   if constexpr (KIND == 0) {
     acc = (double)over_block<NT, MaxF32>((float)acc, reinterpret_cast<float*>(red));
   } else {
@@ -87,48 +100,63 @@ __global__ __launch_bounds__(1024) void norm_total_k(const double* __restrict__ 
   if (threadIdx.x == 0) total[0] = KIND == 2 ? sqrt(acc) : acc;
 }
 
+// From the end, where the norm's pass has just been.
+template <bool NTS>
 __global__ __launch_bounds__(NT) void clip_k(const Slices a, const double* __restrict__ total, double max_norm) {
-  const int s = slice_of(a, blockIdx.x);
-  const int64_t n = a.n[s];
-  const int64_t e0 = (int64_t)(blockIdx.x - (s ? a.end[s - 1] : 0u)) * CHUNK;
+  const uint32_t b = gridDim.x - 1 - blockIdx.x;
+  const int s = slice_of(a, b);
+  const int64_t e0 = (int64_t)(b - (s ? a.end[s - 1] : 0u)) * CLIP_CHUNK;
+  const int64_t n = min(a.n[s], e0 + CLIP_CHUNK);
   const float* g = a.g[s];
   float* out = a.out[s];
   const double ratio = max_norm / (total[0] + 1e-6);
   const bool clip = ratio < 1.0;  // not for a NaN
   if (!clip && out == g) return;
   const float k = clip ? (float)ratio : 1.f;
+  if (n - e0 < CLIP_CHUNK) {
+    for (int64_t e = e0 + threadIdx.x; e < n; e += NT) out[e] = g[e] * k;
+    return;
+  }
+  f4 v[CLIP_UNROLL];
 #pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const int64_t e = e0 + (int64_t)(u * NT + threadIdx.x) * 4;
-    if (e + 4 <= n) {
-      const f4 v = *reinterpret_cast<const f4u*>(g + e);
-      *reinterpret_cast<f4u*>(out + e) = v * k;
-    } else {
-      for (int64_t i = e; i < n; ++i) out[i] = g[i] * k;
-    }
+  for (int u = 0; u < CLIP_UNROLL; ++u)
+    v[u] = __builtin_nontemporal_load(reinterpret_cast<const f4u*>(g + e0) + u * NT + threadIdx.x);
+#pragma unroll
+  for (int u = 0; u < CLIP_UNROLL; ++u) {
+    f4u* p = reinterpret_cast<f4u*>(out + e0) + u * NT + threadIdx.x;
+    if constexpr (NTS) __builtin_nontemporal_store(v[u] * k, p);
+    else *p = v[u] * k;
   }
 }
 
-int check_slices(const char* what, const oxi_grad_slice* slices, int count, bool outs, int64_t* chunks) {
+int check_slices(const char* what, const oxi_grad_slice* slices, int count, bool outs, int64_t* total) {
   if (count < 0) return fail(OXI_INVALID_ARGUMENT, "%s: negative slice count", what);
   if (count > 0 && !slices) return fail(OXI_INVALID_ARGUMENT, "%s: NULL slice array", what);
-  *chunks = 0;
+  *total = 0;
   for (int i = 0; i < count; ++i) {
     if (slices[i].n < 0) return fail(OXI_INVALID_ARGUMENT, "%s: slice %d has a negative size", what, i);
     if (slices[i].n == 0) continue;
     if (!slices[i].g || (outs && !slices[i].out))
       return fail(OXI_INVALID_ARGUMENT, "%s: slice %d has a NULL pointer", what, i);
-    if (slices[i].n > INT64_MAX - CHUNK || !grid_fits(ceil_div(slices[i].n, CHUNK), NT))
-      return fail(OXI_INVALID_ARGUMENT, "%s: slice %d is too large", what, i);
-    *chunks += ceil_div(slices[i].n, CHUNK);
+    if (slices[i].n > ((int64_t)1 << 40)) return fail(OXI_INVALID_ARGUMENT, "%s: slice %d is too large", what, i);
+    *total += slices[i].n;
   }
   return OXI_OK;
 }
 
-// Calls launch(slices, blocks, blocks before) for as many slices at once as fit.
+// Chunks of all slices, which hold `total` floats.
+int64_t chunks_of(const oxi_grad_slice* slices, int count, int64_t total) {
+  int64_t chunks = 0;
+  for (int i = 0; i < count; ++i) chunks += ceil_div(slices[i].n, chunk_of(total));
+  return chunks;
+}
+
+// Calls launch(slices, blocks, blocks before) for as many slices at once as fit, in
+// order or from the last on.
 template <class F>
-int for_slices(const oxi_grad_slice* slices, int count, const char* what, F launch) {
+int for_slices(const oxi_grad_slice* slices, int count, int64_t chunk, bool back, const char* what, F launch) {
   Slices a{};
+  a.chunk = chunk;
   int64_t blocks = 0, before = 0;
   int rc = OXI_OK;
   auto flush = [&]() {
@@ -139,13 +167,14 @@ int for_slices(const oxi_grad_slice* slices, int count, const char* what, F laun
     blocks = 0;
     a.count = 0;
   };
-  for (int i = 0; i < count; ++i) {
-    if (slices[i].n == 0) continue;
-    const int64_t nb = ceil_div(slices[i].n, CHUNK);
+  for (int j = 0; j < count; ++j) {
+    const oxi_grad_slice& q = slices[back ? count - 1 - j : j];
+    if (q.n == 0) continue;
+    const int64_t nb = ceil_div(q.n, a.chunk);
     if (a.count == MOST_SLICES || !grid_fits(blocks + nb, NT)) flush();
-    a.g[a.count] = slices[i].g;
-    a.out[a.count] = slices[i].out;
-    a.n[a.count] = slices[i].n;
+    a.g[a.count] = q.g;
+    a.out[a.count] = q.out;
+    a.n[a.count] = q.n;
     blocks += nb;
     a.end[a.count++] = (uint32_t)blocks;
   }
@@ -162,29 +191,41 @@ extern "C" {
 
 int oxi_grad_norm_workspace(const oxi_grad_slice* slices, int count, int64_t* bytes) {
   if (!bytes) return fail(OXI_INVALID_ARGUMENT, "grad_norm_workspace: NULL result");
-  int64_t chunks = 0;
-  if (int rc = check_slices("grad_norm_workspace", slices, count, false, &chunks)) return rc;
-  *bytes = chunks * (int64_t)sizeof(double);
+  int64_t n = 0;
+  if (int rc = check_slices("grad_norm_workspace", slices, count, false, &n)) return rc;
+  *bytes = chunks_of(slices, count, n) * (int64_t)sizeof(double);
   return OXI_OK;
 }
 
 int oxi_grad_norm(const oxi_grad_slice* slices, int count, double norm_type, double* total, void* workspace) {
   const char* what = "grad_norm";
-  int64_t chunks = 0;
-  if (int rc = check_slices(what, slices, count, false, &chunks)) return rc;
+  int64_t n = 0;
+  if (int rc = check_slices(what, slices, count, false, &n)) return rc;
   const int kind = norm_type == 2.0 ? 2 : norm_type == 1.0 ? 1 : std::isinf(norm_type) && norm_type > 0 ? 0 : -1;
   if (kind < 0) return fail(OXI_INVALID_ARGUMENT, "%s: the norm must be 1, 2 or infinite, got %g", what, norm_type);
   if (!total) return fail(OXI_INVALID_ARGUMENT, "%s: total must not be NULL", what);
   if ((reinterpret_cast<uintptr_t>(total) | reinterpret_cast<uintptr_t>(workspace)) & 7)
     return fail(OXI_INVALID_ARGUMENT, "%s: total and the workspace must be 8-byte aligned", what);
   OXI_CHECK_INIT();
+  const int64_t chunks = chunks_of(slices, count, n);
   Workspace own(workspace ? 0 : (size_t)chunks * sizeof(double));
   if (chunks && !workspace && !own.p) return fail_alloc(what);
   double* parts = static_cast<double*>(workspace ? workspace : own.p);
-  const int rc = for_slices(slices, count, what, [&](const Slices& a, unsigned blocks, int64_t before) {
-    if (kind == 0) norm_part_k<0><<<blocks, NT, 0, stream()>>>(a, parts, before);
-    else if (kind == 1) norm_part_k<1><<<blocks, NT, 0, stream()>>>(a, parts, before);
-    else norm_part_k<2><<<blocks, NT, 0, stream()>>>(a, parts, before);
+  // the last chunks, with which the clipping begins, are read with plain loads
+  const int64_t hot = chunks - REREAD_BYTES / (4 * chunk_of(n));
+  const int rc = for_slices(slices, count, chunk_of(n), false, what, [&](const Slices& a, unsigned blocks, int64_t before) {
+    const bool again = before + blocks > hot;
+#define OXI_NP(KIND)                                                                        \
+  if (again) norm_part_k<KIND, true><<<blocks, NT, 0, stream()>>>(a, parts, before);        \
+  else norm_part_k<KIND, false><<<blocks, NT, 0, stream()>>>(a, parts, before)
+    if (kind == 0) {
+      OXI_NP(0);
+    } else if (kind == 1) {
+      OXI_NP(1);
+    } else {
+      OXI_NP(2);
+    }
+#undef OXI_NP
   });
   if (rc) return rc;
   if (kind == 0) norm_total_k<0><<<1, 1024, 0, stream()>>>(parts, chunks, total);
@@ -195,15 +236,17 @@ int oxi_grad_norm(const oxi_grad_slice* slices, int count, double norm_type, dou
 
 int oxi_grad_clip(const oxi_grad_slice* slices, int count, const double* total, double max_norm) {
   const char* what = "grad_clip";
-  int64_t chunks = 0;
-  if (int rc = check_slices(what, slices, count, true, &chunks)) return rc;
+  int64_t n = 0;
+  if (int rc = check_slices(what, slices, count, true, &n)) return rc;
   if (!total) return fail(OXI_INVALID_ARGUMENT, "%s: total must not be NULL", what);
   if (reinterpret_cast<uintptr_t>(total) & 7)
     return fail(OXI_INVALID_ARGUMENT, "%s: total must be 8-byte aligned", what);
   if (std::isnan(max_norm)) return fail(OXI_INVALID_ARGUMENT, "%s: max_norm is NaN", what);
   OXI_CHECK_INIT();
-  return for_slices(slices, count, what, [&](const Slices& a, unsigned blocks, int64_t) {
-    clip_k<<<blocks, NT, 0, stream()>>>(a, total, max_norm);
+  const bool nt = nt_stream_stores(n * 4);
+  return for_slices(slices, count, CLIP_CHUNK, true, what, [&](const Slices& a, unsigned blocks, int64_t) {
+    if (nt) clip_k<true><<<blocks, NT, 0, stream()>>>(a, total, max_norm);
+    else clip_k<false><<<blocks, NT, 0, stream()>>>(a, total, max_norm);
   });
 }
 

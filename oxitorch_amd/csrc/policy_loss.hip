@@ -82,12 +82,24 @@ __global__ __launch_bounds__(1024) void policy_mean_k(const TokenRows in, const 
                                                       float* __restrict__ out) {
   __shared__ double red[1024 / 64];
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
-  for (int64_t i = threadIdx.x; i < in.n; i += 1024) {
-    const int64_t id = in.ids[i];
-    const float w = in.weights ? in.weights[i] : 1.f;
-    if (id < 0 || id >= in.c || w == 0.f) continue;
+  constexpr int U = 4;  // rows in flight a thread
+  for (int64_t i0 = threadIdx.x; i0 < in.n; i0 += U * 1024) {
+    int64_t id[U];
+    float w[U], v[4][U];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] += (double)w * (double)rows[k * in.n + i];
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = min(i0 + u * 1024, in.n - 1);
+      id[u] = in.ids[i];
+      w[u] = in.weights ? in.weights[i] : 1.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k][u] = rows[k * in.n + i];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * 1024 >= in.n || id[u] < 0 || id[u] >= in.c || w[u] == 0.f) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += (double)w[u] * (double)v[k][u];
+    }
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -139,6 +151,7 @@ int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* ad
   if (!workspace && !own.p) return fail_alloc(what);
   TokenRows in = token_rows(logits, ids, n, c, temperature);
   in.weights = weights;
+  in.again = true;
   const double inv_div = 1.0 / (double)divisor;
   const PolicyOp op{advantages, old_logp, ref_logp, weights, rows, logp, coef, saved, n, 1.0 - (double)clip_low,
                     1.0 + (double)clip_high, (double)clip_max, (double)kl_coef, (double)entropy_coef, inv_div};

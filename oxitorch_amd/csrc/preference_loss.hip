@@ -176,6 +176,7 @@ int oxi_preference_loss_fwd(const float* logits, const int64_t* ids, const int64
     TokenRows in = token_rows(logits, ids, n, c, 1.f);
     in.starts = starts;
     in.sequences = 2 * pairs;
+    in.again = true;
     if (int rc = token_rows_read(in, parts, PreferenceOp{logp, coef, saved}, what)) return rc;
   }
   if (pairs) {

@@ -8,6 +8,8 @@
 namespace oxi {
 namespace {
 
+// AGAIN: plain loads, for rows that a backward then finds in the Infinity Cache.
+template <bool AGAIN>
 __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* __restrict__ parts, int np,
                                                         int64_t row0) {
   __shared__ float lds[3 * (PART_NT / 64)];
@@ -26,9 +28,12 @@ __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* 
 #pragma unroll
   for (int u = 0; u < PART_U; ++u) {
     const int q = c0 + u * PART_NT;
-    v[u] = q < lay.c4 ? ld_stream(x4 + q) : f4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-    if (q == at) v[u] = drop(v[u], comp);
+    v[u] = f4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+    if (q < lay.c4) v[u] = AGAIN ? x4[q] : ld_stream(x4 + q);
   }
+#pragma unroll
+  for (int u = 0; u < PART_U; ++u)
+    if (c0 + u * PART_NT == at) v[u] = drop(v[u], comp);
   const int e = part == 0 ? lay.edge(t, in.c) : -1;
   const float v1 = e >= 0 && e != (int)id ? xr[e] : NEG_INF;
 #pragma unroll
@@ -54,7 +59,7 @@ __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* 
   if (t == 0) parts[row * np + part] = f4{m, both.a, both.b, 0.f};
 }
 
-constexpr int BWD_NT = 256, BWD_U = 4;
+constexpr int BWD_NT = 256, BWD_U = 2;
 
 template <bool ENT, bool NTS>
 __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ x, const int64_t* __restrict__ ids,
@@ -62,8 +67,9 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
                                                       const float* __restrict__ gh, const float* __restrict__ gloss,
                                                       float* __restrict__ dx, int c, int chunks, int64_t row0,
                                                       float scale2, float inv_t, int* guard) {
-  const int64_t row = row0 + blockIdx.x / (unsigned)chunks;
-  const int chunk = (int)(blockIdx.x % (unsigned)chunks);
+  const unsigned back = gridDim.x - 1 - blockIdx.x;
+  const int64_t row = row0 + back / (unsigned)chunks;
+  const int chunk = (int)(back % (unsigned)chunks);
   const int t = threadIdx.x;
   const int64_t id = ids[row];
   const f4 sv = *reinterpret_cast<const f4u*>(saved + 4 * row);
@@ -168,9 +174,15 @@ static int64_t rows_a_launch(int64_t blocks, int threads) { return 0xffffffffll 
 
 int launch_token_parts(const TokenRows& in, f4* parts, const char* what) {
   const int64_t np = row_parts(in.c), most = rows_a_launch(np, PART_NT);
-  for (int64_t r0 = 0; r0 < in.n; r0 += most) {
-    const int64_t rows = in.n - r0 < most ? in.n - r0 : most;
-    token_part_k<<<dim3((unsigned)(rows * np)), dim3(PART_NT), 0, stream()>>>(in, parts, (int)np, r0);
+  // the last rows, with which the backward begins, are read with plain loads
+  const int64_t cold = in.again ? in.n - REREAD_BYTES / (4 * (int64_t)in.c) : in.n;
+  for (int64_t r0 = 0; r0 < in.n;) {
+    const int64_t end = r0 < cold && cold < in.n ? cold : in.n;
+    const int64_t rows = end - r0 < most ? end - r0 : most;
+    const dim3 grid((unsigned)(rows * np));
+    if (r0 < cold) token_part_k<false><<<grid, dim3(PART_NT), 0, stream()>>>(in, parts, (int)np, r0);
+    else token_part_k<true><<<grid, dim3(PART_NT), 0, stream()>>>(in, parts, (int)np, r0);
+    r0 += rows;
   }
   return check_launch(what);
 }
@@ -220,7 +232,9 @@ int oxi_token_logp_fwd(const float* logits, const int64_t* ids, float* logp, flo
   Workspace own(workspace ? 0 : (size_t)token_parts_bytes(n, c));
   if (!workspace && !own.p) return fail_alloc(what);
   f4* parts = static_cast<f4*>(workspace ? workspace : own.p);
-  return token_rows_read(token_rows(logits, ids, n, c, temperature), parts, LogpOp{logp, entropy, saved}, what);
+  TokenRows in = token_rows(logits, ids, n, c, temperature);
+  in.again = saved != nullptr;
+  return token_rows_read(in, parts, LogpOp{logp, entropy, saved}, what);
 }
 
 int oxi_token_logp_bwd(const float* logits, const int64_t* ids, const float* saved, const float* glogp,

@@ -50,6 +50,7 @@ struct TokenRows {
   float scale2;  // log2(e)/T
   double inv_t;
   int* guard;
+  bool again;  // whether the logits are read again by a backward
 
   // An id past the classes raises the guard and is padding.
   __device__ __forceinline__ bool counts(int64_t row, int64_t id) const {
@@ -177,16 +178,23 @@ struct RowGrad {
   }
 };
 
+// The row of block b: 16 neighbours go to one XCD (blocks go round the 8 of them), so that
+// the lines of ids and of the rows' other numbers are read and written by one L2.
+__device__ __forceinline__ int64_t row_of_block(uint32_t b, int64_t n) {
+  const uint32_t g = b & ~127u;
+  return (int64_t)g + 128 <= n ? (int64_t)(g + (b & 7) * 16 + ((b >> 3) & 15)) : (int64_t)b;
+}
+
 constexpr int rows_block(int rt) { return rt == 64 ? 256 : rt; }
 // Waves a SIMD that the registers must allow.
 constexpr int rows_waves(int nv) { return nv >= 10 ? 4 : 8; }
 
 template <int RT, int NV, bool GRAD, bool ENT, bool NTS, class Op>
-__global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(4))) void token_rows_k(
+__global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(RT == 1024 && NV <= 8 ? 8 : 4))) void token_rows_k(
     const TokenRows in, const Op op, float* __restrict__ dx) {
   __shared__ __align__(8) float lds[3 * (RT / 64)];
   const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
-  const int64_t row = RT == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  const int64_t row = RT == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : row_of_block(blockIdx.x, in.n);
   if (RT == 64 && row >= in.n) return;
   const int C = in.c;
   const float* xr = in.x + row * C;
@@ -281,6 +289,7 @@ bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx) {
   OXI_TR(256, 8)
   OXI_TR(256, 12)
   OXI_TR(256, 16)
+  OXI_TR(1024, 8)
   OXI_TR(512, 10)
   OXI_TR(512, 12)
   OXI_TR(512, 14)
