@@ -779,6 +779,134 @@ Var distillation_loss(const Var& logits, const std::vector<int64_t>& ids, const 
                  });
 }
 
+// ---- post-training losses ------------------------------------------------------------
+
+namespace {
+
+// (batch, classes) logits and one id a row; ids below 0 are padding.
+void check_tokens(const Tensor& lv, const std::vector<int64_t>& ids, const char* what) {
+  if (lv.ndim() != 2) err_invalid(std::string(what) + " expects (batch, classes) logits, got " + fmt_shape(lv.shape));
+  if ((int64_t)ids.size() != lv.shape[0])
+    err_invalid(std::to_string(ids.size()) + " tokens for batch of " + std::to_string(lv.shape[0]));
+  for (int64_t i : ids)
+    if (i >= lv.shape[1])
+      err_oob("index " + std::to_string(i) + " is out of bounds for axis 1 with size " + std::to_string(lv.shape[1]));
+  require_hip(lv, what);
+}
+
+// A row's number each, contiguous on the device; unset stays unset.
+std::optional<Tensor> per_row(const std::optional<Tensor>& t, int64_t n, const char* what) {
+  if (!t) return std::nullopt;
+  if (t->shape != Shape{n}) err_shape(fmt_shape({n}), fmt_shape(t->shape));
+  require_hip(*t, what);
+  return t_contiguous(*t);
+}
+
+float* ptr(const std::optional<Tensor>& t) { return t ? t->data() : nullptr; }
+
+// The node of a loss whose gradient goes by each row's logp and, with `gh`, its entropy:
+// `unit`, what the forward wrote for backward()'s seed, or a pass from coef and saved.
+Var token_loss(const Tensor& loss, const char* op, const Var& logits, const Tensor& lc,
+               const std::shared_ptr<Storage>& id, const Tensor& saved, const Tensor& coef, bool gh, float temperature,
+               const std::optional<Tensor>& unit) {
+  const int64_t n = lc.shape[0], c = lc.shape[1];
+  auto fresh = std::make_shared<std::atomic<bool>>(unit.has_value());
+  return Var::op(loss, op, {logits},
+                 [lc, id, saved, coef, gh, temperature, n, c, unit, fresh](const Tensor& g,
+                                                                          const std::vector<bool>& need) -> Grads {
+                   if (!need[0]) return {std::nullopt};
+                   if (is_implicit_seed(g) && fresh->exchange(false)) return {*unit};
+                   Tensor gs = t_contiguous(g);
+                   Tensor d = Tensor::empty({n, c}, Dev::Hip);
+                   hip_check(oxi_token_logp_bwd(lc.data(), static_cast<const int64_t*>(id->ptr), saved.data(),
+                                                coef.data(), gh ? coef.data() + n : nullptr, gs.data(), d.data(), n, c,
+                                                temperature));
+                   return {d};
+                 });
+}
+
+bool wants_gradient(const Var& logits) { return logits.requires_grad() && is_grad_enabled(); }
+
+}  // namespace
+
+Var token_log_probs(const Var& logits, const std::vector<int64_t>& ids, float temperature, bool entropy) {
+  const Tensor& lv = logits.value();
+  check_tokens(lv, ids, "token_log_probs");
+  const int64_t n = lv.shape[0], c = lv.shape[1];
+  Tensor lc = t_contiguous(lv);
+  auto id = device_i64(ids);
+  Tensor out = Tensor::empty(entropy ? Shape{2, n} : Shape{n}, Dev::Hip);
+  std::optional<Tensor> saved;
+  if (wants_gradient(logits)) saved = Tensor::empty({n, 4}, Dev::Hip);
+  hip_check(oxi_token_logp_fwd(lc.data(), static_cast<const int64_t*>(id->ptr), out.data(),
+                               entropy ? out.data() + n : nullptr, saved ? saved->data() : nullptr, nullptr, n, c,
+                               temperature));
+  return Var::op(out, "token_log_probs", {logits},
+                 [lc, id, saved, entropy, n, c, temperature](const Tensor& g, const std::vector<bool>& need) -> Grads {
+                   if (!need[0]) return {std::nullopt};
+                   Tensor gs = t_contiguous(g);
+                   Tensor d = Tensor::empty({n, c}, Dev::Hip);
+                   hip_check(oxi_token_logp_bwd(lc.data(), static_cast<const int64_t*>(id->ptr), saved->data(),
+                                                gs.data(), entropy ? gs.data() + n : nullptr, nullptr, d.data(), n, c,
+                                                temperature));
+                   return {d};
+                 });
+}
+
+std::pair<Var, Tensor> policy_loss(const Var& logits, const std::vector<int64_t>& ids, const Tensor& advantages,
+                                   const std::optional<Tensor>& old_logp, const std::optional<Tensor>& ref_logp,
+                                   const std::optional<Tensor>& weights, const PolicyOptions& o) {
+  const Tensor& lv = logits.value();
+  check_tokens(lv, ids, "policy_loss");
+  const int64_t n = lv.shape[0], c = lv.shape[1];
+  const auto adv = per_row(advantages, n, "policy_loss"), old = per_row(old_logp, n, "policy_loss"),
+             ref = per_row(ref_logp, n, "policy_loss"), w = per_row(weights, n, "policy_loss");
+  Tensor lc = t_contiguous(lv);
+  auto id = device_i64(ids);
+  Tensor out = Tensor::empty({4}, Dev::Hip), rows = Tensor::empty({4, n}, Dev::Hip), coef = Tensor::empty({2, n}, Dev::Hip),
+         saved = Tensor::empty({n, 4}, Dev::Hip);
+  // With a gradient to come, the forward pass also forms the gradient for
+  // loss.backward()'s seed, as cross_entropy does (and the same switch turns off).
+  std::optional<Tensor> unit;
+  if (wants_gradient(logits) && ce_one_pass()) unit = Tensor::empty({n, c}, Dev::Hip);
+  hip_check(oxi_policy_loss_fwd(lc.data(), static_cast<const int64_t*>(id->ptr), ptr(adv), ptr(old), ptr(ref), ptr(w),
+                                out.data(), rows.data(), nullptr, coef.data(), saved.data(), ptr(unit), nullptr, n, c,
+                                o.temperature, o.clip_low, o.clip_high, o.clip_max, o.kl, o.entropy, o.divisor));
+  const Tensor loss = t_select(out, 0, 0);
+  return {token_loss(loss, "policy_loss", logits, lc, id, saved, coef, o.entropy != 0.0f, o.temperature, unit),
+          t_narrow(out, 0, 1, 4, 1)};
+}
+
+std::pair<Var, std::pair<Tensor, Tensor>> preference_loss(const Var& logits, const std::vector<int64_t>& ids,
+                                                          const std::vector<int64_t>& lengths,
+                                                          const std::optional<Tensor>& ref_logp,
+                                                          const PreferenceOptions& o) {
+  const Tensor& lv = logits.value();
+  check_tokens(lv, ids, "preference_loss");
+  const int64_t n = lv.shape[0], c = lv.shape[1], pairs = (int64_t)lengths.size() / 2;
+  if (lengths.size() % 2) err_invalid("preference_loss: an odd number of sequences: " + std::to_string(lengths.size()));
+  std::vector<int64_t> starts{0};
+  for (int64_t l : lengths) {
+    if (l < 0 || l > n - starts.back())
+      err_invalid("preference_loss: a sequence of " + std::to_string(l) + " rows after " +
+                  std::to_string(starts.back()) + " of " + std::to_string(n));
+    starts.push_back(starts.back() + l);
+  }
+  const auto ref = per_row(ref_logp, n, "preference_loss");
+  Tensor lc = t_contiguous(lv);
+  auto id = device_i64(ids), at = device_i64(starts);
+  Tensor loss = Tensor::empty({}, Dev::Hip), pair = Tensor::empty({pairs}, Dev::Hip),
+         seq = Tensor::empty({pairs, 2}, Dev::Hip), coef = Tensor::empty({n}, Dev::Hip),
+         saved = Tensor::empty({n, 4}, Dev::Hip);
+  std::optional<Tensor> unit;
+  if (wants_gradient(logits) && ce_one_pass()) unit = Tensor::empty({n, c}, Dev::Hip);
+  hip_check(oxi_preference_loss_fwd(lc.data(), static_cast<const int64_t*>(id->ptr),
+                                    static_cast<const int64_t*>(at->ptr), ptr(ref), loss.data(), pair.data(), seq.data(),
+                                    coef.data(), saved.data(), ptr(unit), nullptr, n, c, pairs, o.kind, o.average ? 1 : 0,
+                                    o.beta, o.margin, o.smoothing));
+  return {token_loss(loss, "preference_loss", logits, lc, id, saved, coef, false, 1.0f, unit), {pair, seq}};
+}
+
 }  // namespace aops
 
 RotaryFrequencies::RotaryFrequencies(const std::vector<double>& inv_freq, float s)

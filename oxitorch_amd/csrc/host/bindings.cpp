@@ -674,6 +674,60 @@ PYBIND11_MODULE(_native, m) {
       py::arg("temperature"));
 
   m.def(
+      "token_log_probs",
+      [](const PyTensor& logits, const py::object& tokens, float temperature, bool entropy) {
+        return PyTensor(aops::token_log_probs(logits.v, int_ids(tokens), temperature, entropy));
+      },
+      py::arg("logits"), py::arg("tokens"), py::arg("temperature"), py::arg("entropy"));
+  m.def(
+      "policy_loss",
+      [](const PyTensor& logits, const py::object& tokens, const PyTensor& advantages, const py::object& old_logp,
+         const py::object& ref_logp, const py::object& weights, float temperature, float clip_low, float clip_high,
+         float clip_max, float kl, float entropy, float divisor) {
+        auto given = [](const py::object& o) -> std::optional<Tensor> {
+          if (o.is_none()) return std::nullopt;
+          return o.cast<PyTensor&>().value();
+        };
+        auto [loss, stats] = aops::policy_loss(logits.v, int_ids(tokens), advantages.value(), given(old_logp),
+                                               given(ref_logp), given(weights),
+                                               {temperature, clip_low, clip_high, clip_max, kl, entropy, divisor});
+        return py::make_tuple(PyTensor(loss), leaf(stats));
+      },
+      py::arg("logits"), py::arg("tokens"), py::arg("advantages"), py::arg("old_logp"), py::arg("ref_logp"),
+      py::arg("weights"), py::arg("temperature"), py::arg("clip_low"), py::arg("clip_high"), py::arg("clip_max"),
+      py::arg("kl"), py::arg("entropy"), py::arg("divisor"));
+  m.def(
+      "preference_loss",
+      [](const PyTensor& logits, const py::object& tokens, const py::object& lengths, const py::object& ref_logp,
+         const std::string& kind, bool average, float beta, float margin, float smoothing) {
+        aops::PreferenceOptions o;
+        if (kind == "sigmoid") o.kind = OXI_PREFERENCE_SIGMOID;
+        else if (kind == "hinge") o.kind = OXI_PREFERENCE_HINGE;
+        else if (kind == "ipo") o.kind = OXI_PREFERENCE_IPO;
+        else err_invalid("preference_loss kind must be \"sigmoid\", \"hinge\" or \"ipo\", got \"" + kind + "\"");
+        o.average = average;
+        o.beta = beta;
+        o.margin = margin;
+        o.smoothing = smoothing;
+        std::optional<Tensor> ref;
+        if (!ref_logp.is_none()) ref = ref_logp.cast<PyTensor&>().value();
+        auto [loss, more] = aops::preference_loss(logits.v, int_ids(tokens), int_ids(lengths), ref, o);
+        return py::make_tuple(PyTensor(loss), leaf(more.first), leaf(more.second));
+      },
+      py::arg("logits"), py::arg("tokens"), py::arg("lengths"), py::arg("ref_logp"), py::arg("kind"),
+      py::arg("average"), py::arg("beta"), py::arg("margin"), py::arg("smoothing"));
+  // (norm, clipped gradients or None where none is to be clipped)
+  m.def("clip_grad_norm", [](const std::vector<PyTensor>& grads, double max_norm, double norm_type) -> py::tuple {
+    std::vector<Tensor> g;
+    for (const PyTensor& t : grads) g.push_back(t.value());
+    auto [norm, outs] = t_clip_grad_norm(g, max_norm, norm_type);
+    if (!outs) return py::make_tuple(norm, py::none());
+    py::list l;
+    for (Tensor& t : *outs) l.append(leaf(std::move(t)));
+    return py::make_tuple(norm, l);
+  });
+
+  m.def(
       "verify_drafts",
       [](const py::object& tokens, const py::object& draft, const PyTensor& target, const PyTensor& uniforms,
          const py::object& lengths) {

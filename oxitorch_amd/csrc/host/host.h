@@ -318,6 +318,27 @@ Var rotary(const Var& x, const RotaryFrequencies& f, const std::optional<std::ve
 // k each), and its log-sum-exp (n) if given; the mean over the rows that hold entries.
 Var distillation_loss(const Var& logits, const std::vector<int64_t>& ids, const Tensor& top,
                       const std::optional<Tensor>& top_lse, float temperature);
+// Log-probabilities (n) of one id a row of logits (n, c), ids below 0 being padding;
+// with `entropy` (2, n), the second row the entropies.
+Var token_log_probs(const Var& logits, const std::vector<int64_t>& ids, float temperature, bool entropy);
+struct PolicyOptions {
+  float temperature = 1.0f, clip_low = 0.2f, clip_high = 0.2f, clip_max = 0.0f, kl = 0.0f, entropy = 0.0f, divisor = 1.0f;
+};
+// The clipped policy loss, and (3) the means of the KL term, the entropy and the clipped share.
+std::pair<Var, Tensor> policy_loss(const Var& logits, const std::vector<int64_t>& ids, const Tensor& advantages,
+                                   const std::optional<Tensor>& old_logp, const std::optional<Tensor>& ref_logp,
+                                   const std::optional<Tensor>& weights, const PolicyOptions& o);
+struct PreferenceOptions {
+  int kind = 0;  // OXI_PREFERENCE_*
+  bool average = false;
+  float beta = 0.1f, margin = 0.0f, smoothing = 0.0f;
+};
+// The preference loss of sequences of the given lengths, (chosen, rejected) by turns;
+// the pairs' losses and (pairs, 2) the sequences' log-probabilities.
+std::pair<Var, std::pair<Tensor, Tensor>> preference_loss(const Var& logits, const std::vector<int64_t>& ids,
+                                                          const std::vector<int64_t>& lengths,
+                                                          const std::optional<Tensor>& ref_logp,
+                                                          const PreferenceOptions& o);
 }  // namespace aops
 
 // ---- serving: no gradients -----------------------------------------------------------
@@ -337,6 +358,11 @@ Tensor t_dequantize(const E4m3Rows& q);
 std::pair<std::vector<int64_t>, std::vector<int64_t>> t_verify_drafts(
     const Tensor& target, const std::optional<Tensor>& draft, const std::vector<int64_t>& tokens,
     const std::optional<std::vector<int64_t>>& lengths, const Tensor& uniforms);
+
+// The gradients' joint norm (p = 1, 2 or infinite; waits for the device), and the
+// gradients times max_norm/(norm + 1e-6) where that is below 1, in fresh tensors.
+std::pair<double, std::optional<std::vector<Tensor>>> t_clip_grad_norm(const std::vector<Tensor>& grads, double max_norm,
+                                                                       double norm_type);
 
 // ---- optimizers (crates/oxi-autograd/src/optim.rs) ------------------------------
 // All state (velocities, moments, per-parameter step counters) lives here as

@@ -44,6 +44,37 @@ Operands operands(const Var& param, const Tensor& grad, const char* what) {
 
 }  // namespace
 
+// clip_grad_norm_ (python/oxitorch/optim.py:248-273) on the device: one wait, for the norm.
+std::pair<double, std::optional<std::vector<Tensor>>> t_clip_grad_norm(const std::vector<Tensor>& grads, double max_norm,
+                                                                       double norm_type) {
+  std::vector<Tensor> ins, outs;
+  std::vector<oxi_grad_slice> slices;
+  int64_t n = 0;
+  for (const Tensor& g : grads) {
+    require_hip(g, "clip_grad_norm_");
+    // a dense tensor's elements in their own order, whatever the order of its dims
+    Tensor like = g;
+    like.strides = result_strides(g.shape, {&g});
+    ins.push_back(like.strides == g.strides ? g : t_contiguous(g));
+    slices.push_back({ins.back().data(), nullptr, ins.back().numel()});
+    n += ins.back().numel();
+  }
+  if (n == 0) return {0.0, std::nullopt};
+  Storage total(Dev::Hip, sizeof(double));
+  double* tp = static_cast<double*>(total.ptr);
+  hip_check(oxi_grad_norm(slices.data(), (int)slices.size(), norm_type, tp, nullptr));
+  double norm = 0.0;
+  hip_check(oxi_hip_memcpy_d2h(&norm, tp, sizeof(double)));
+  if (!(max_norm / (norm + 1e-6) < 1.0)) return {norm, std::nullopt};
+  for (size_t i = 0; i < ins.size(); ++i) {
+    outs.push_back(Tensor::empty(ins[i].shape, Dev::Hip));
+    outs.back().strides = ins[i].strides;
+    slices[i].out = outs.back().data();
+  }
+  hip_check(oxi_grad_clip(slices.data(), (int)slices.size(), tp, max_norm));
+  return {norm, std::move(outs)};
+}
+
 // Sgd::step_param (optim.rs:104-137).
 void Sgd::step_param(size_t index, Var& param) {
   const std::optional<Tensor> grad = param.grad();

@@ -2,7 +2,8 @@
 (python/oxitorch/nn/__init__.py): functional norms, activations, softmax
 family, cross-entropy and embedding, plus their Module wrappers; and the
 operators of language models around them that the reference does not have
-(residual RMS norm, rotary positions, distillation, draft verification)."""
+(residual RMS norm, rotary positions, distillation, draft verification, token
+log-probabilities, policy and preference losses)."""
 
 from .module import Module, Parameter, Sequential
 from . import functional
@@ -17,6 +18,8 @@ from .functional import (
     leaky_relu,
     log_softmax,
     mse_loss,
+    policy_loss,
+    preference_loss,
     relu,
     rms_norm,
     rotary_embedding,
@@ -25,6 +28,7 @@ from .functional import (
     silu,
     softmax,
     tanh,
+    token_log_probs,
     verify_drafts,
 )
 from .layers import (
@@ -50,6 +54,7 @@ __all__ = [
     "leaky_relu", "log_softmax", "mse_loss", "relu", "rms_norm", "sigmoid", "silu", "softmax", "tanh",
     "GELU", "Embedding", "LayerNorm", "LeakyReLU", "ReLU", "RMSNorm", "SiLU", "Sigmoid", "Softmax", "Tanh",
     "add_rms_norm", "add_rms_norm_e4m3", "distillation_loss", "rotary_embedding", "rotary_frequencies", "verify_drafts",
+    "policy_loss", "preference_loss", "token_log_probs",
     "AddRMSNorm", "RotaryEmbedding",
     "bmm", "conv2d", "dropout", "linear", "max_pool2d", "Conv2d", "Dropout", "Linear", "MaxPool2d",
 ]

@@ -297,6 +297,98 @@ def distillation_loss(logits, teacher_ids, teacher_logits, temperature=1.0, teac
     return _native.distillation_loss(logits, flat, top, lse, float(temperature))
 
 
+# ---- post-training losses ---------------------------------------------------------------
+
+def _tokens(tokens, n, classes):
+    """One class a row as a flat int64 array; negative ones are padding."""
+    t = _flat_ints(tokens, "tokens")
+    if len(t) != n:
+        raise ValueError(f"{len(t)} tokens for batch of {n}")
+    if t.size and t.max() >= classes:
+        raise IndexError(f"index {int(t.max())} is out of bounds for axis 1 with size {classes}")
+    return t
+
+
+def _optional_values(v):
+    return None if v is None else _device_values(v)
+
+
+def token_log_probs(logits, tokens, temperature=1.0, entropy=False):
+    """Log-probabilities (batch,) of one token a row under softmax(logits/T); with
+    `entropy` (log-probabilities, entropies of the rows' distributions).
+
+    `tokens`: flat integers; a negative one is padding, whose row is not read and
+    gives 0. Under no_grad what policy_loss and preference_loss take as the old
+    policy's or the reference's; with gradients the base of losses of one's own: both
+    results' gradients go back in one pass. The log-probability of a token that is all
+    but certain keeps its digits, and so does the gradient at it."""
+    n, classes = logits.shape
+    both = _native.token_log_probs(logits, _tokens(tokens, n, classes), float(temperature), bool(entropy))
+    return (both.select(0, 0), both.select(0, 1)) if entropy else both
+
+
+def policy_loss(logits, tokens, advantages, old_log_probs=None, reference_log_probs=None, weights=None, clip=0.2,
+                clip_max=None, kl=0.0, entropy=0.0, temperature=1.0, stats=False):
+    """The clipped policy loss of sampled tokens, with a KL term against a reference
+    policy and an entropy bonus: the mean over the rows of
+
+        -min(r A, clip(r, 1 - clip, 1 + clip) A) + kl (exp(d) - 1 - d) - entropy H
+
+    with r = exp(logp - old_log_probs), d = reference_log_probs - logp, H the entropy of
+    the row's distribution, logp as in token_log_probs, A = `advantages`.
+
+    `tokens`: flat integers, a negative one is padding. `advantages`,
+    `old_log_probs`, `reference_log_probs`, `weights`: tensors or arrays, one number a row,
+    that no gradient goes to. Without old_log_probs r is 1 (the first step after
+    sampling). `clip`: a number or (below, above); `clip_max` bounds the loss of a negative
+    advantage at clip_max |A|. With `weights` the loss is the sum of weight * row
+    instead of the mean, and rows of weight 0 are padding (a mean by sequences: 1 / (its
+    tokens * sequences)). With `stats`, (loss, (3,) tensor of the same means of the KL
+    term's exp(d) - 1 - d, H and whether r was clipped).
+
+    Fused as cross_entropy is: one pass over the logits writes the loss and the
+    gradient for backward()'s implicit seed."""
+    n, classes = logits.shape
+    t = _tokens(tokens, n, classes)
+    low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+    divisor = 1.0 if weights is not None else float(max(1, int((t >= 0).sum())))
+    loss, more = _native.policy_loss(logits, t, _device_values(advantages), _optional_values(old_log_probs),
+                                     _optional_values(reference_log_probs), _optional_values(weights),
+                                     float(temperature), float(low), float(high),
+                                     0.0 if clip_max is None else float(clip_max), float(kl), float(entropy), divisor)
+    return (loss, more) if stats else loss
+
+
+def preference_loss(logits, tokens, lengths, reference_log_probs=None, beta=0.1, kind="sigmoid", margin=0.0,
+                    smoothing=0.0, average=False, details=False):
+    """The preference loss of pairs of sequences: the mean over the pairs of
+
+        "sigmoid": (1 - smoothing) softplus(-u) + smoothing softplus(u)
+        "hinge":   max(0, 1 - u)
+        "ipo":     (u/beta - 1/(2 beta))^2
+
+    with u = beta ((S_c - R_c) - (S_r - R_r)) - margin, S the sum of the sequence's tokens'
+    log-probabilities and R that of `reference_log_probs` (one number a row; None: 0), or
+    with `average` their means.
+
+    `lengths` (pairs, 2): the rows of each pair's chosen and rejected sequence, which lie
+    one after the other in `logits` (rows, classes). `tokens`: flat integers, a negative
+    one (the prompt's) does not count; rows behind the last sequence are padding. With
+    `details`, (loss, the pairs' losses, (pairs, 2) S).
+
+    The logits are read twice, the second time for the gradient of backward()'s
+    implicit seed, which the forward writes as cross_entropy does."""
+    n, classes = logits.shape
+    t = _tokens(tokens, n, classes)
+    given = np.asarray(lengths)
+    if given.size and (given.ndim != 2 or given.shape[1] != 2):
+        raise ValueError(f"lengths of shape {list(given.shape)}: (pairs, 2) is expected")
+    loss, pair, seq = _native.preference_loss(logits, t, _flat_ints(given, "lengths"),
+                                              _optional_values(reference_log_probs), kind, bool(average), float(beta),
+                                              float(margin), float(smoothing))
+    return (loss, pair, seq) if details else loss
+
+
 # ---- serving: drafted tokens ------------------------------------------------------------
 
 def _uniforms(u):

@@ -145,15 +145,18 @@ def _with_grads(params):
 def clip_grad_norm_(params, max_norm, norm_type=2.0):
     """Scale all gradients by max_norm/(total+1e-6) when their joint p-norm
     `total` exceeds max_norm; returns the pre-clip total as a float. Norms
-    and scaling run on the device; `norm_type` is any p >= 1 or inf."""
+    and scaling run on the device, over all tensors at once and with one wait
+    for 1, 2 and inf; `norm_type` is any p >= 1 or inf."""
     pairs = list(_with_grads(list(params)))
-    if norm_type == float("inf"):
-        total = max((float(g.apply("abs").max().item()) for _, g in pairs), default=0.0)
-    else:
-        acc = 0.0
-        for _, g in pairs:
-            acc += float((g.apply("abs") ** float(norm_type)).sum().item())
-        total = acc ** (1.0 / norm_type)
+    if norm_type in (1, 2, float("inf")):
+        total, clipped = _native.clip_grad_norm([g for _, g in pairs], float(max_norm), float(norm_type))
+        for (t, _), g in zip(pairs, clipped or ()):
+            t.grad = g
+        return total
+    acc = 0.0
+    for _, g in pairs:
+        acc += float((g.apply("abs") ** float(norm_type)).sum().item())
+    total = acc ** (1.0 / norm_type)
     scale = max_norm / (total + 1e-6)
     if scale < 1.0:
         for t, g in pairs:
