@@ -71,11 +71,21 @@ struct PolicyOp {
   }
 };
 
-bool launch_rows(const TokenRows& in, const PolicyOp& op, float* dx, bool ent) {
-  const bool nt = nt_stream_stores(in.n * in.c * 4);
-  if (ent) return nt ? launch_token_rows_as<true, true, true>(in, op, dx) : launch_token_rows_as<true, true, false>(in, op, dx);
-  return nt ? launch_token_rows_as<true, false, true>(in, op, dx) : launch_token_rows_as<true, false, false>(in, op, dx);
+template <bool GRAD, bool ENT, bool NTS>
+bool launch_as(const TokenRows& in, const PolicyOp& op, float* dx, void* workspace) {
+  return launch_token_cluster<GRAD, ENT, NTS>(in, op, dx, workspace) || launch_token_rows_as<GRAD, ENT, NTS>(in, op, dx);
 }
+
+// One pass over the logits, the same with a gradient and without; false where no kernel holds such rows.
+bool launch_rows(const TokenRows& in, const PolicyOp& op, float* dx, bool ent, void* workspace) {
+  if (!dx) return launch_as<false, false, false>(in, op, dx, workspace);
+  const bool nt = nt_stream_stores(in.n * in.c * 4);
+  if (ent) return nt ? launch_as<true, true, true>(in, op, dx, workspace) : launch_as<true, true, false>(in, op, dx, workspace);
+  return nt ? launch_as<true, false, true>(in, op, dx, workspace) : launch_as<true, false, false>(in, op, dx, workspace);
+}
+
+// The parts' sums, or a cluster's words, which are no more than the parts.
+int64_t workspace_bytes(int64_t n, int64_t c) { return 64 + n * row_parts(c) * 3 * (int64_t)sizeof(uint64_t); }
 
 // out[i] = sum over the rows of w rows[i] / divisor in float64, in a fixed order: one block.
 __global__ __launch_bounds__(1024) void policy_mean_k(const TokenRows in, const float* __restrict__ rows, double inv_div,
@@ -118,7 +128,7 @@ extern "C" {
 int oxi_policy_loss_workspace(int64_t n, int64_t c, int64_t* bytes) {
   if (!bytes) return fail(OXI_INVALID_ARGUMENT, "policy_loss_workspace: NULL result");
   if (int rc = check_token_rows("policy_loss_workspace", n, c, 1.f)) return rc;
-  *bytes = token_parts_bytes(n, c);
+  *bytes = n ? workspace_bytes(n, c) : 0;
   return OXI_OK;
 }
 
@@ -147,7 +157,7 @@ int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* ad
     return fail(OXI_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
   OXI_CHECK_INIT();
   if (n == 0) return oxi_fill(out, 4, 0.f);
-  Workspace own(workspace ? 0 : (size_t)token_parts_bytes(n, c));
+  Workspace own(workspace ? 0 : (size_t)workspace_bytes(n, c));
   if (!workspace && !own.p) return fail_alloc(what);
   TokenRows in = token_rows(logits, ids, n, c, temperature);
   in.weights = weights;
@@ -155,10 +165,11 @@ int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* ad
   const double inv_div = 1.0 / (double)divisor;
   const PolicyOp op{advantages, old_logp, ref_logp, weights, rows, logp, coef, saved, n, 1.0 - (double)clip_low,
                     1.0 + (double)clip_high, (double)clip_max, (double)kl_coef, (double)entropy_coef, inv_div};
-  if (dlogits && launch_rows(in, op, dlogits, entropy_coef != 0.f)) {
+  void* const at = workspace ? workspace : own.p;
+  if (launch_rows(in, op, dlogits, entropy_coef != 0.f, at)) {
     if (int rc = check_launch(what)) return rc;
   } else {
-    if (int rc = token_rows_read(in, static_cast<f4*>(workspace ? workspace : own.p), op, what)) return rc;
+    if (int rc = token_rows_read(in, static_cast<f4*>(at), op, what)) return rc;
     if (dlogits)
       if (int rc = launch_token_bwd(logits, ids, saved, coef, entropy_coef != 0.f ? coef + n : nullptr, nullptr,
                                     dlogits, n, c, temperature, what))

@@ -145,6 +145,19 @@ struct LogpOp {
 
 }  // namespace
 
+namespace {
+__global__ __launch_bounds__(256) void zero_words_k(uint64_t* __restrict__ p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+}  // namespace
+
+Cluster start_cluster(void* at, int64_t n, int blocks) {
+  const int64_t words = cluster_bytes(n, blocks) / (int64_t)sizeof(uint64_t);
+  zero_words_k<<<dim3((unsigned)ceil_div(words, 256)), dim3(256), 0, stream()>>>(static_cast<uint64_t*>(at), words);
+  return {static_cast<uint64_t*>(at) + 8, static_cast<uint32_t*>(at), blocks};
+}
+
 int check_token_rows(const char* what, int64_t n, int64_t c, float temperature) {
   if (n < 0 || c < 0) return fail(OXI_INVALID_ARGUMENT, "%s: negative size", what);
   if (c > ((int64_t)1 << 30) || !grid_fits(n, 1024))

@@ -162,7 +162,8 @@ int launch_token_bwd(const float* x, const int64_t* ids, const float* saved, con
 // ---------------------------------------------------------------------------
 // A row a group of RT threads (a wave, four to a block, or a block), held in
 // registers as NV float4s a thread: the logits cross HBM once for the loss and its
-// gradient. Every thread works the row's few 64-bit formulas out by itself.
+// gradient. Every thread works the row's few 64-bit formulas out by itself: from the
+// first wave through LDS (8192, 32000) took 324 us against 316.
 
 // What a gradient at a class takes besides 2^t and t.
 struct RowGrad {
@@ -301,6 +302,163 @@ bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx) {
   OXI_TR(1024, 16)
 #undef OXI_TR
   return false;
+}
+
+// ---------------------------------------------------------------------------
+// A row a cluster of blocks, each with a piece of it in registers (RT * NV float4s):
+// rows that one block's registers do not hold. The blocks give each other their piece's maximum and sums by words of
+// a value and a flag each, so that no order of memory accesses matters; the words are
+// zeroed by a launch before. A block's row and piece go by a ticket that it takes as
+// it starts: a block waits only for those of its own row, which have started or take
+// the next tickets, and the rows before finish without it, so every wait ends.
+// (1024, 131072) with an entropy term 187 us, 5.4 TB/s; parts, their join and the
+// backward's pass 238. For few shorter rows, (64, 32000) on 4 blocks each, the ticket
+// and the words cost what the other CUs gain: 11.0 us against 10.2 on one block.
+constexpr int CLUSTER_RT = 512, CLUSTER_MOST = 16;
+struct Cluster {
+  uint64_t* words;  // 3 a block
+  uint32_t* ticket;
+  int blocks;  // a row
+};
+inline int64_t cluster_bytes(int64_t n, int blocks) { return 64 + n * blocks * 3 * (int64_t)sizeof(uint64_t); }
+// words and ticket zeroed, in `at`
+Cluster start_cluster(void* at, int64_t n, int blocks);
+
+constexpr uint64_t WORD_SET = (uint64_t)1 << 32;
+__device__ __forceinline__ void give_word(uint64_t* p, float v) {
+  __hip_atomic_store(p, WORD_SET | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The word once it is set.
+__device__ __forceinline__ float take_word(const uint64_t* p) {
+  uint64_t v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  while (!(v & WORD_SET)) {
+    __builtin_amdgcn_s_sleep(1);
+    v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  return __uint_as_float((uint32_t)v);
+}
+
+template <int NV, bool GRAD, bool ENT, bool NTS, class Op>
+__global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4))) void token_cluster_k(
+    const TokenRows in, const Op op, float* __restrict__ dx, const Cluster cl) {
+  constexpr int RT = CLUSTER_RT;
+  __shared__ __align__(8) float lds[3 * (RT / 64)];
+  __shared__ float from[3 * CLUSTER_MOST];
+  __shared__ uint32_t ticket;
+  const int t = threadIdx.x;
+  if (t == 0) ticket = atomicAdd(cl.ticket, 1u);
+  __syncthreads();
+  const uint32_t b = ticket;
+  const int64_t row = b / (unsigned)cl.blocks;
+  const int piece = (int)(b % (unsigned)cl.blocks);
+  const int C = in.c;
+  const float* xr = in.x + row * C;
+  float* dr = dx + row * C;
+  const int64_t id64 = in.ids[row];
+  const RowLay lay(xr, C);
+  const int c0 = piece * (RT * NV) + t;
+  auto put = [&](const f4& d, int c) {
+    f4u* const p = reinterpret_cast<f4u*>(dr + lay.head) + c;
+    if constexpr (NTS) __builtin_nontemporal_store(d, p);
+    else *p = d;
+  };
+  const int e = piece == 0 ? lay.edge(t, C) : -1;
+  const bool lead = piece == 0 && t == 0;
+  if (!in.counts(row, id64)) {
+    if (lead) op.skip(row);
+    if constexpr (GRAD) {
+#pragma unroll
+      for (int q = 0; q < NV; ++q)
+        if (c0 + q * RT < lay.c4) put(f4{0.f, 0.f, 0.f, 0.f}, c0 + q * RT);
+      if (e >= 0) dr[e] = 0.f;
+    }
+    return;
+  }
+  const int id = (int)id64;
+  const int at = lay.slot(id), comp = lay.component(id);
+  const float xa = xr[id];
+  f4 v[NV];
+#pragma unroll
+  for (int q = 0; q < NV; ++q) v[q] = ld_stream(reinterpret_cast<const f4*>(xr + lay.head) + min(c0 + q * RT, lay.c4 - 1));
+  float v1 = e >= 0 && e != id ? xr[e] : NEG_INF;
+  float own = v1;
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    if (c0 + q * RT >= lay.c4) v[q] = f4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+    if (c0 + q * RT == at) v[q] = drop(v[q], comp);
+    own = fmaxf(own, max4(v[q]));
+  }
+  own = over_block<RT, MaxF32>(own, lds);
+  const float shift = own == NEG_INF ? 0.f : own;
+  // With an entropy's gradient the registers keep t relative to the piece's maximum, else 2^t.
+  float s = 0.f, et = 0.f;
+  auto add = [&](float x) {
+    const float z = (x - shift) * in.scale2;
+    const float p = __builtin_amdgcn_exp2f(z);
+    s += p;
+    et = fmaf(p, fmaxf(z, LEAST_T), et);
+    return ENT ? z : p;
+  };
+#pragma unroll
+  for (int q = 0; q < NV; ++q) v[q] = f4{add(v[q].x), add(v[q].y), add(v[q].z), add(v[q].w)};
+  v1 = add(v1);
+  const Two both = over_block<RT, Both<AddF32>>(Two{s, et}, reinterpret_cast<Two*>(lds + RT / 64));
+  uint64_t* const words = cl.words + 3 * cl.blocks * row;
+  if (t < 3) give_word(words + 3 * piece + t, t == 0 ? own : t == 1 ? both.a : both.b);
+  if (t < 3 * cl.blocks) from[t] = take_word(words + t);
+  __syncthreads();
+  float m = xa;
+  for (int k = 0; k < cl.blocks; ++k) m = fmaxf(m, from[3 * k]);
+  double rest = 0.0, mean = 0.0;
+  for (int k = 0; k < cl.blocks; ++k) {
+    if (from[3 * k + 1] == 0.f) continue;  // nothing finite there
+    const float d = (from[3 * k] - m) * in.scale2;
+    const double f = (double)__builtin_amdgcn_exp2f(d);
+    rest += f * (double)from[3 * k + 1];
+    mean += f * ((double)from[3 * k + 2] + (double)fmaxf(d, LEAST_T) * (double)from[3 * k + 1]);
+  }
+  const RowStats r = row_stats(m, xa, rest, mean, in.scale2, in.inv_t);
+  const Two k = op.finish(row, r, lead);
+  if constexpr (GRAD) {
+    const RowGrad g(r, xa, in.scale2, (float)in.inv_t, k.a, ENT ? k.b : 0.f);
+    const float up = (shift - m) * in.scale2;  // the piece's t from the row's
+    const float alpha = ENT ? g.alpha : g.alpha * __builtin_amdgcn_exp2f(up);
+    auto grad = [&](float z) {
+      if constexpr (ENT) {
+        asm("" : "+v"(z));  // its exponential is formed again, not held
+        z += up;
+        return __builtin_amdgcn_exp2f(z) * fmaf(g.beta, fmaxf(z, LEAST_T), alpha);
+      } else {
+        return z * alpha;
+      }
+    };
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      if (c0 + q * RT >= lay.c4) continue;
+      f4 d = f4{grad(v[q].x), grad(v[q].y), grad(v[q].z), grad(v[q].w)};
+      if (c0 + q * RT == at) d = put_at(d, comp, g.chosen);
+      put(d, c0 + q * RT);
+    }
+    if (e >= 0) dr[e] = e == id ? g.chosen : grad(v1);
+  }
+}
+
+// The blocks a row of c classes: as few as hold it; 0 where one block does, or more
+// than CLUSTER_MOST would be needed.
+constexpr int CLUSTER_NV = 16;
+inline int cluster_blocks(int64_t c) {
+  const int64_t blocks = ceil_div(c, (int64_t)CLUSTER_RT * CLUSTER_NV * 4);
+  return c > ROWS_MAX && blocks <= CLUSTER_MOST ? (int)blocks : 0;
+}
+
+template <bool GRAD, bool ENT, bool NTS, class Op>
+bool launch_token_cluster(const TokenRows& in, const Op& op, float* dx, void* workspace) {
+  const int blocks = cluster_blocks(in.c);
+  if (!blocks || !grid_fits(in.n * blocks, CLUSTER_RT)) return false;
+  const Cluster cl = start_cluster(workspace, in.n, blocks);
+  token_cluster_k<CLUSTER_NV, GRAD, ENT, NTS, Op>
+      <<<dim3((unsigned)(in.n * blocks)), dim3(CLUSTER_RT), 0, stream()>>>(in, op, dx, cl);
+  return true;
 }
 
 // Whether sizes and temperature can be taken; 0 or an error's code.
