@@ -26,10 +26,17 @@ struct PolicyOp {
   double low, high, most;  // the ratio's bounds, and the factor of a negative advantage that bounds s (0: none)
   double kl, ent, inv_div;
 
+  // The row's own numbers, loaded before its logits.
+  struct Given {
+    float adv, old, ref, weight;
+  };
+  __device__ __forceinline__ Given load(int64_t row) const {
+    return {adv[row], old ? old[row] : 0.f, ref ? ref[row] : 0.f, weights ? weights[row] : 1.f};
+  }
   // Writes the row's results; the loss's derivatives by its logp and entropy.
-  __device__ __forceinline__ Two finish(int64_t row, const RowStats& r, bool lead) const {
-    const double A = (double)adv[row];
-    const double ratio = old ? exp64(r.logp - (double)old[row]) : 1.0;
+  __device__ __forceinline__ Two finish(int64_t row, const Given& in, const RowStats& r, bool lead) const {
+    const double A = (double)in.adv;
+    const double ratio = old ? exp64(r.logp - (double)in.old) : 1.0;
     const double free = A == 0.0 ? 0.0 : ratio * A;
     const double bounded = (ratio < low ? low : ratio > high ? high : ratio) * A;
     bool clipped = free > bounded;
@@ -41,7 +48,7 @@ struct PolicyOp {
     double g = clipped ? 0.0 : -free, k = 0.0;
     double loss = -s;
     if (ref) {
-      const double d = (double)ref[row] - r.logp;
+      const double d = (double)in.ref - r.logp;
       k = d == (double)__builtin_huge_valf() ? d : exp_rest(d);
       if (kl != 0.0) {
         g -= kl * (fabs(d) < 0.5 ? k + d : exp64(d) - 1.0);
@@ -49,7 +56,7 @@ struct PolicyOp {
       }
     }
     if (ent != 0.0) loss -= ent * r.entropy;
-    const double w = (weights ? (double)weights[row] : 1.0) * inv_div;
+    const double w = (double)in.weight * inv_div;
     const Two by{(float)(g * w), (float)(-ent * w)};
     if (!lead) return by;
     rows[row] = (float)loss;

@@ -22,7 +22,9 @@ struct PreferenceOp {
   static constexpr int READ_MAX = ROWS_MAX_READ;
   double* logp;
   float *coef, *saved;
-  __device__ __forceinline__ Two finish(int64_t row, const RowStats& r, bool lead) const {
+  struct Given {};
+  __device__ __forceinline__ Given load(int64_t) const { return {}; }
+  __device__ __forceinline__ Two finish(int64_t row, const Given&, const RowStats& r, bool lead) const {
     if (!lead) return {0.f, 0.f};
     logp[row] = r.logp;
     coef[row] = 0.f;  // a counted row's own comes with its pair

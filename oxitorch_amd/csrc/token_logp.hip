@@ -129,7 +129,9 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
 struct LogpOp {
   static constexpr int READ_MAX = ROWS_MAX_READ;
   float *logp, *entropy, *saved;
-  __device__ __forceinline__ Two finish(int64_t row, const RowStats& r, bool lead) const {
+  struct Given {};
+  __device__ __forceinline__ Given load(int64_t) const { return {}; }
+  __device__ __forceinline__ Two finish(int64_t row, const Given&, const RowStats& r, bool lead) const {
     if (!lead) return {0.f, 0.f};
     logp[row] = (float)r.logp;
     if (entropy) entropy[row] = (float)r.entropy;

@@ -134,6 +134,7 @@ __global__ __launch_bounds__(256) void token_join_k(const TokenRows in, const f4
     if (lane == 0) op.skip(row);
     return;
   }
+  const typename Op::Given given = op.load(row);
   const float xa = in.x[row * in.c + id];
   const f4* mine = parts + row * np;
   float m = xa;
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(256) void token_join_k(const TokenRows in, const f4
   s = over_block<64, AddF64>(s, (double*)nullptr);
   et = over_block<64, AddF64>(et, (double*)nullptr);
   const RowStats r = row_stats(m, xa, s, et, in.scale2, in.inv_t);
-  op.finish(row, r, lane == 0);
+  op.finish(row, given, r, lane == 0);
 }
 
 // dx of the rows from their saved floats, for the gradients gl and gh (NULL: none) of
@@ -201,6 +202,7 @@ __global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(
   const float* xr = in.x + row * C;
   float* dr = dx + row * C;
   const int64_t id64 = in.ids[row];
+  const typename Op::Given given = op.load(row);
   const RowLay lay(xr, C);
   auto put = [&](const f4& d, int c) {
     f4u* const p = reinterpret_cast<f4u*>(reinterpret_cast<char*>(dr + lay.head) + (uint32_t)c * 16u);
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(
   v1 = add(v1);
   const Two both = over_block<RT, Both<AddF32>>(Two{s, et}, reinterpret_cast<Two*>(lds + RT / 64));
   const RowStats r = row_stats(m, xa, (double)both.a, (double)both.b, in.scale2, in.inv_t);
-  const Two k = op.finish(row, r, t == 0);
+  const Two k = op.finish(row, given, r, t == 0);
   if constexpr (GRAD) {
     const RowGrad g(r, xa, in.scale2, (float)in.inv_t, k.a, ENT ? k.b : 0.f);
     auto grad = [&](float z) {
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4)))
   const int t = threadIdx.x;
   if (t == 0) ticket = atomicAdd(cl.ticket, 1u);
   __syncthreads();
-  const uint32_t b = ticket;
+  const uint32_t b = __builtin_amdgcn_readfirstlane(ticket);
   const int64_t row = b / (unsigned)cl.blocks;
   const int piece = (int)(b % (unsigned)cl.blocks);
   const int C = in.c;
@@ -418,7 +420,7 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4)))
     mean += f * ((double)from[3 * k + 2] + (double)fmaxf(d, LEAST_T) * (double)from[3 * k + 1]);
   }
   const RowStats r = row_stats(m, xa, rest, mean, in.scale2, in.inv_t);
-  const Two k = op.finish(row, r, lead);
+  const Two k = op.finish(row, op.load(row), r, lead);
   if constexpr (GRAD) {
     const RowGrad g(r, xa, in.scale2, (float)in.inv_t, k.a, ENT ? k.b : 0.f);
     const float up = (shift - m) * in.scale2;  // the piece's t from the row's
