@@ -39,51 +39,71 @@ struct PreferenceOp {
 };
 
 struct PairArgs {
-  const int64_t* starts;
-  const int64_t* ids;
+  TokenRows in;
+  const f4* parts;     // the rows' parts, np each; NULL: their log-probabilities are in logp
   const double* logp;
+  int np;
   const float* ref;
-  float *pair_loss, *seq_logp, *coef;
-  int64_t n, pairs;
-  int c, kind, average;
+  float *pair_loss, *seq_logp, *coef, *saved;
+  int64_t pairs;
+  int kind, average;
   double beta, margin, smoothing;
-  int* guard;
 };
 
 // log(1 + e^x)
 __device__ __forceinline__ double softplus(double x) { return (x > 0.0 ? x : 0.0) + log1p64(exp64(-fabs(x))); }
 
-constexpr int PAIR_NT = 256;
+// Threads of a pair's block, half of them to each sequence, and the most parts a row that
+// they join: a row a thread, all of a sequence's rows at once (a wave a row in a launch of
+// its own and 256 threads a pair after it took 15 us at 8 pairs of 760 rows, PAIRUS here).
+constexpr int PAIR_NT = 1024, HALF = PAIR_NT / 2, JOIN_MOST = 16;
 
 // A block a pair.
 __global__ __launch_bounds__(PAIR_NT) void preference_pair_k(const PairArgs g) {
-  __shared__ double red[PAIR_NT / 64];
+  __shared__ double red[3 * (PAIR_NT / 64)];
+  const TokenRows& in = g.in;
+  const int t = threadIdx.x;
   const int64_t p = blockIdx.x;
-  double sum[2], own[2], count[2];
-  int64_t first[2], last[2];
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    int64_t a = g.starts[2 * p + side], b = g.starts[2 * p + side + 1];
-    if (a < 0 || b < a || b > g.n) {  // such a sequence is empty
-      if (threadIdx.x == 0) atomicOr(g.guard, 1);
-      a = b = 0;
-    }
-    first[side] = a;
-    last[side] = b;
-    double s = 0.0, r = 0.0, k = 0.0;
-    for (int64_t i = a + threadIdx.x; i < b; i += PAIR_NT) {
-      const int64_t id = g.ids[i];
-      if (id < 0 || id >= g.c) continue;
+  const int side = t / HALF;
+  int64_t first = in.starts[2 * p + side], last = in.starts[2 * p + side + 1];
+  if (first < 0 || last < first || last > in.n) {  // such a sequence is empty
+    if ((t & (HALF - 1)) == 0) atomicOr(in.guard, 1);
+    first = last = 0;
+  }
+  double s = 0.0, r = 0.0, k = 0.0;
+  for (int64_t i = first + (t & (HALF - 1)); i < last; i += HALF) {
+    const int64_t id = in.ids[i];
+    if (!in.counts(i, id)) continue;
+    if (g.ref) r += (double)g.ref[i];
+    if (g.parts) {
+      const RowStats row = joined_row(in, g.parts + i * g.np, g.np, in.x[i * in.c + id]);
+      save_row(g.saved, i, row);
+      s += row.logp;
+    } else {
       s += g.logp[i];
-      if (g.ref) r += (double)g.ref[i];
-      k += 1.0;
     }
-    s = block_sum<PAIR_NT>(s, red);
-    r = block_sum<PAIR_NT>(r, red);
-    k = block_sum<PAIR_NT>(k, red);
-    count[side] = g.average ? fmax(k, 1.0) : 1.0;
-    own[side] = s / count[side];
-    sum[side] = (s - r) / count[side];
+    k += 1.0;
+  }
+  s = over_block<64, AddF64>(s, (double*)nullptr);
+  r = over_block<64, AddF64>(r, (double*)nullptr);
+  k = over_block<64, AddF64>(k, (double*)nullptr);
+  if ((t & 63) == 0) {
+    red[3 * (t >> 6)] = s;
+    red[3 * (t >> 6) + 1] = r;
+    red[3 * (t >> 6) + 2] = k;
+  }
+  __syncthreads();
+  double sum[2], own[2], count[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    double v[3] = {0.0, 0.0, 0.0};
+#pragma unroll
+    for (int w = 0; w < HALF / 64; ++w)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) v[i] += red[3 * (q * (HALF / 64) + w) + i];
+    count[q] = g.average ? fmax(v[2], 1.0) : 1.0;
+    own[q] = v[0] / count[q];
+    sum[q] = (v[0] - v[1]) / count[q];
   }
   const double u = g.beta * (sum[0] - sum[1]) - g.margin;
   double loss, slope;  // slope: of loss by the log-ratio
@@ -101,30 +121,19 @@ __global__ __launch_bounds__(PAIR_NT) void preference_pair_k(const PairArgs g) {
     loss = d * d;
     slope = 2.0 * d;
   }
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const float k = (float)((side ? -slope : slope) / ((double)g.pairs * count[side]));
-    for (int64_t i = first[side] + threadIdx.x; i < last[side]; i += PAIR_NT) {
-      const int64_t id = g.ids[i];
-      if (id >= 0 && id < g.c) g.coef[i] = k;
-    }
-  }
-  if (threadIdx.x == 0) {
+  const float by = (float)((side ? -slope : slope) / ((double)g.pairs * (side ? count[1] : count[0])));
+  for (int64_t i = first + (t & (HALF - 1)); i < last; i += HALF)
+    if (in.counts(i, in.ids[i])) g.coef[i] = by;
+  if (t == 0) {
     g.pair_loss[p] = (float)loss;
     g.seq_logp[2 * p] = (float)own[0];
     g.seq_logp[2 * p + 1] = (float)own[1];
   }
 }
 
-__global__ __launch_bounds__(PAIR_NT) void preference_mean_k(const float* __restrict__ pair_loss, int64_t pairs,
-                                                             float* __restrict__ loss) {
-  __shared__ double red[PAIR_NT / 64];
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < pairs; i += PAIR_NT) s += (double)pair_loss[i];
-  s = block_sum<PAIR_NT>(s, red);
-  if (threadIdx.x == 0) loss[0] = (float)(s / (double)pairs);
-}
+__global__ __launch_bounds__(MEAN_NT) void preference_mean_k(const MeanOf mean) { mean.by_block(); }
 
+// The parts' sums and the log-probabilities.
 int64_t workspace_bytes(int64_t n, int64_t c) { return token_parts_bytes(n, c) + n * (int64_t)sizeof(double); }
 
 int check_preference(const char* what, int64_t n, int64_t c, int64_t pairs) {
@@ -172,27 +181,35 @@ int oxi_preference_loss_fwd(const float* logits, const int64_t* ids, const int64
   OXI_CHECK_INIT();
   Workspace own(workspace ? 0 : (size_t)workspace_bytes(n, c));
   if (n && !workspace && !own.p) return fail_alloc(what);
+  if (!pairs) {
+    if (int rc = oxi_fill(loss, 1, 0.f)) return rc;
+  }
   f4* parts = static_cast<f4*>(workspace ? workspace : own.p);
   double* logp = reinterpret_cast<double*>(parts + token_parts_bytes(n, c) / (int64_t)sizeof(f4));
+  TokenRows in = token_rows(logits, ids, n, c, 1.f);
+  in.starts = starts;
+  in.sequences = 2 * pairs;
+  in.again = dlogits != nullptr;
+  in.coef = coef;
+  in.saved = saved;
+  const int np = (int)row_parts(c);
+  const bool by_pairs = c > PreferenceOp::READ_MAX && np <= JOIN_MOST;
   if (n) {
-    TokenRows in = token_rows(logits, ids, n, c, 1.f);
-    in.starts = starts;
-    in.sequences = 2 * pairs;
-    in.again = true;
-    if (int rc = token_rows_read(in, parts, PreferenceOp{logp, coef, saved}, what)) return rc;
+    const int rc = by_pairs ? launch_token_parts(in, parts, what)
+                            : token_rows_read(in, parts, PreferenceOp{logp, coef, saved}, what);
+    if (rc) return rc;
   }
   if (pairs) {
-    const PairArgs g{starts, ids, logp, ref_logp, pair_loss, seq_logp, coef, n, pairs, (int)c, kind, average ? 1 : 0,
-                     (double)beta, (double)margin, (double)smoothing, guard_flag()};
+    const PairArgs g{in, by_pairs ? parts : nullptr, logp, np, ref_logp, pair_loss, seq_logp, coef, saved, pairs, kind, average ? 1 : 0, (double)beta, (double)margin, (double)smoothing};
     preference_pair_k<<<dim3((unsigned)pairs), dim3(PAIR_NT), 0, stream()>>>(g);
     if (int rc = check_launch(what)) return rc;
-    preference_mean_k<<<1, PAIR_NT, 0, stream()>>>(pair_loss, pairs, loss);
-    if (int rc = check_launch(what)) return rc;
-  } else if (int rc = oxi_fill(loss, 1, 0.f)) {
-    return rc;
   }
-  if (n && dlogits) return launch_token_bwd(logits, ids, saved, coef, nullptr, nullptr, dlogits, n, c, 1.f, what);
-  return OXI_OK;
+  const MeanOf mean{pair_loss, pairs, loss};
+  if (n && dlogits)  // one of its blocks takes the mean
+    return launch_token_bwd(logits, ids, saved, coef, nullptr, nullptr, dlogits, n, c, 1.f, what, mean);
+  if (!pairs) return OXI_OK;
+  preference_mean_k<<<1, MEAN_NT, 0, stream()>>>(mean);
+  return check_launch(what);
 }
 
 }  // extern "C"

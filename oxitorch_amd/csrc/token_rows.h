@@ -50,7 +50,9 @@ struct TokenRows {
   float scale2;  // log2(e)/T
   double inv_t;
   int* guard;
-  bool again;  // whether the logits are read again by a backward
+  bool again;      // whether the logits are read again by a backward
+  // where the parts' pass writes 0 for every row, and what rows that do not count keep; NULL: nowhere
+  float *coef, *saved;
 
   // An id past the classes raises the guard and is padding.
   __device__ __forceinline__ bool counts(int64_t row, int64_t id) const {
@@ -122,6 +124,30 @@ inline int64_t row_parts(int64_t c) { return c > 0 ? ceil_div(c, (int64_t)PART_N
 // the part's own maximum.
 int launch_token_parts(const TokenRows& in, f4* parts, const char* what);
 
+// The row of the parts mine[first], mine[first + step], .. as far as this lane adds them: maximum of all
+// lanes in m; sums of this lane's.
+__device__ __forceinline__ void join_parts(const f4* mine, int first, int step, int np, float m, float scale2, double& s,
+                                           double& et) {
+  s = et = 0.0;
+  for (int p = first; p < np; p += step) {
+    const f4 v = mine[p];
+    if (v.y == 0.f) continue;  // nothing finite there
+    const float d = (v.x - m) * scale2;
+    const double f = (double)__builtin_amdgcn_exp2f(d);
+    s += f * (double)v.y;
+    et += f * ((double)v.z + (double)fmaxf(d, LEAST_T) * (double)v.y);
+  }
+}
+
+// A row by one thread.
+__device__ __forceinline__ RowStats joined_row(const TokenRows& in, const f4* mine, int np, float xa) {
+  float m = xa;
+  for (int p = 0; p < np; ++p) m = fmaxf(m, mine[p].x);
+  double s, et;
+  join_parts(mine, 0, 1, np, m, in.scale2, s, et);
+  return row_stats(m, xa, s, et, in.scale2, in.inv_t);
+}
+
 // A wave a row: joins its parts; `op` writes what the row gives.
 template <class Op>
 __global__ __launch_bounds__(256) void token_join_k(const TokenRows in, const f4* __restrict__ parts, int np,
@@ -140,25 +166,34 @@ __global__ __launch_bounds__(256) void token_join_k(const TokenRows in, const f4
   float m = xa;
   for (int p = lane; p < np; p += 64) m = fmaxf(m, mine[p].x);
   m = wave_max(m);
-  double s = 0.0, et = 0.0;
-  for (int p = lane; p < np; p += 64) {
-    const f4 v = mine[p];
-    if (v.y == 0.f) continue;  // nothing finite there
-    const float d = (v.x - m) * in.scale2;
-    const double f = (double)__builtin_amdgcn_exp2f(d);
-    s += f * (double)v.y;
-    et += f * ((double)v.z + (double)fmaxf(d, LEAST_T) * (double)v.y);
-  }
+  double s, et;
+  join_parts(mine, lane, 64, np, m, in.scale2, s, et);
   s = over_block<64, AddF64>(s, (double*)nullptr);
   et = over_block<64, AddF64>(et, (double*)nullptr);
   const RowStats r = row_stats(m, xa, s, et, in.scale2, in.inv_t);
   op.finish(row, given, r, lane == 0);
 }
 
+// to[0] = the mean of `count` values, in 64 bits in a fixed order, by a block of MEAN_NT threads.
+constexpr int MEAN_NT = 256;
+struct MeanOf {
+  const float* values;
+  int64_t count;  // 0: nothing to do
+  float* to;
+  __device__ __forceinline__ void by_block() const {
+    __shared__ double red[MEAN_NT / 64];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < count; i += MEAN_NT) s += (double)values[i];
+    s = block_sum<MEAN_NT>(s, red);
+    if (threadIdx.x == 0) to[0] = (float)(s / (double)count);
+  }
+};
+
 // dx of the rows from their saved floats, for the gradients gl and gh (NULL: none) of
-// their log-probabilities and entropies times gloss[0] (NULL: 1).
+// their log-probabilities and entropies times gloss[0] (NULL: 1); and the mean, in a block more.
 int launch_token_bwd(const float* x, const int64_t* ids, const float* saved, const float* gl, const float* gh,
-                     const float* gloss, float* dx, int64_t n, int64_t c, float temperature, const char* what);
+                     const float* gloss, float* dx, int64_t n, int64_t c, float temperature, const char* what,
+                     const MeanOf& mean = {});
 
 // ---------------------------------------------------------------------------
 // A row a group of RT threads (a wave, four to a block, or a block), held in
