@@ -13,8 +13,9 @@ template <bool AGAIN>
 __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* __restrict__ parts, int np,
                                                         int64_t row0) {
   __shared__ float lds[3 * (PART_NT / 64)];
-  const int64_t row = row0 + blockIdx.x / (unsigned)np;
-  const int part = (int)(blockIdx.x % (unsigned)np);
+  const RowPiece of(blockIdx.x, gridDim.x / (unsigned)np, (unsigned)np);
+  const int64_t row = row0 + of.row;
+  const int part = of.piece;
   const int64_t id = in.ids[row];
   const int t = threadIdx.x;
   const bool counts = in.counts(row, id);
@@ -64,10 +65,9 @@ __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* 
   if (t == 0) parts[row * np + part] = f4{m, both.a, both.b, 0.f};
 }
 
-// Float4s a thread: one, with the entropy's longer work two ((6100, 32000) 331 us of a preference
-// loss against 347 with two; (4096, 50257) with entropies 331 of both directions against 336 with one).
-constexpr int BWD_NT = 256;
-constexpr int bwd_unroll(bool ent) { return ent ? 2 : 1; }
+// Two float4s a thread: (6100, 32000) of pairs 322 us, with one 329, with four 335; (4096, 50257) with
+// entropies, both directions, 325 and with four 343.
+constexpr int BWD_NT = 256, BWD_U = 2;
 
 template <bool ENT, bool NTS>
 __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ x, const int64_t* __restrict__ ids,
@@ -75,16 +75,17 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
                                                       const float* __restrict__ gh, const float* __restrict__ gloss,
                                                       float* __restrict__ dx, int c, int chunks, int64_t row0,
                                                       float scale2, float inv_t, int* guard, const MeanOf mean) {
-  constexpr int BWD_U = bwd_unroll(ENT);
   static_assert(BWD_NT == MEAN_NT);
   const unsigned more = mean.count ? 1 : 0;
   if (blockIdx.x < more) {
     mean.by_block();
     return;
   }
-  const unsigned back = gridDim.x - 1 - blockIdx.x;
-  const int64_t row = row0 + back / (unsigned)chunks;
-  const int chunk = (int)(back % (unsigned)chunks);
+  // the last rows first
+  const unsigned rows = (gridDim.x - more) / (unsigned)chunks;
+  const RowPiece of(blockIdx.x - more, rows, (unsigned)chunks);
+  const int64_t row = row0 + rows - 1 - of.row;
+  const int chunk = of.piece;
   const int t = threadIdx.x;
   const int64_t id = ids[row];
   const f4 sv = *reinterpret_cast<const f4u*>(saved + 4 * row);
@@ -221,7 +222,7 @@ int launch_token_parts(const TokenRows& in, f4* parts, const char* what) {
 int launch_token_bwd(const float* x, const int64_t* ids, const float* saved, const float* gl, const float* gh,
                      const float* gloss, float* dx, int64_t n, int64_t c, float temperature, const char* what,
                      const MeanOf& mean) {
-  const int64_t chunks = ceil_div(c, (int64_t)BWD_NT * bwd_unroll(gh != nullptr) * 4), most = rows_a_launch(chunks, BWD_NT);
+  const int64_t chunks = ceil_div(c, (int64_t)BWD_NT * BWD_U * 4), most = rows_a_launch(chunks, BWD_NT);
   const float scale2 = (float)(1.4426950408889634 / temperature), inv_t = (float)(1.0 / (double)temperature);
   const bool nt = nt_stream_stores(n * c * 4);
   for (int64_t r0 = 0; r0 < n; r0 += most) {

@@ -116,6 +116,25 @@ struct RowLay {
   __device__ __forceinline__ int component(int a) const { return (a - head) & 3; }
 };
 
+// Row and piece of block b of a launch of `pieces` blocks a row: a row's blocks on one XCD (blocks
+// go round the 8 of them), so that what they all read of it misses one L2 once: (6100, 32000)
+// of pairs 322 us against 343, log-probabilities of (8192, 32000) 165 against 170.
+struct RowPiece {
+  int64_t row;
+  int piece;
+  __device__ __forceinline__ RowPiece(uint32_t b, uint32_t rows, uint32_t pieces) {
+    const uint32_t whole = rows & ~7u;
+    if (b < whole * pieces) {
+      const uint32_t i = b >> 3;
+      row = (int64_t)(i / pieces * 8 + (b & 7));
+      piece = (int)(i % pieces);
+    } else {
+      row = (int64_t)(b / pieces);
+      piece = (int)(b % pieces);
+    }
+  }
+};
+
 // Rows cut into parts of PART_NT * PART_U float4s, a block each.
 constexpr int PART_NT = 256, PART_U = 8;
 inline int64_t row_parts(int64_t c) { return c > 0 ? ceil_div(c, (int64_t)PART_NT * PART_U * 4) : 1; }
