@@ -25,21 +25,22 @@ __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* 
   }
   if (!counts) return;
   const float* xr = in.x + row * in.c;
-  const RowLay lay(xr, in.c);
+  const RowLay<> lay(xr, in.c);
   const int at = lay.slot((int)id), comp = lay.component((int)id);
   const f4* x4 = reinterpret_cast<const f4*>(xr + lay.head);
-  const int c0 = part * (PART_NT * PART_U) + t;
+  // the row's float4s in parts as long as each other
+  const int each = (lay.c4 + np - 1) / np, c0 = part * each + t, end = min(part * each + each, lay.c4);
   f4 v[PART_U];
   float m = NEG_INF;
 #pragma unroll
   for (int u = 0; u < PART_U; ++u) {
     const int q = c0 + u * PART_NT;
     v[u] = f4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-    if (q < lay.c4) v[u] = AGAIN ? x4[q] : ld_stream(x4 + q);
+    if (q < end) v[u] = AGAIN ? x4[q] : ld_stream(x4 + q);
   }
 #pragma unroll
   for (int u = 0; u < PART_U; ++u)
-    if (c0 + u * PART_NT == at) v[u] = drop(v[u], comp);
+    if (c0 + u * PART_NT == at && at < end) v[u] = drop(v[u], comp);
   const int e = part == 0 ? lay.edge(t, in.c) : -1;
   const float v1 = e >= 0 && e != (int)id ? xr[e] : NEG_INF;
 #pragma unroll
@@ -68,25 +69,29 @@ __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* 
 // Two float4s a thread: (6100, 32000) of pairs 322 us, with one 329, with four 335; (4096, 50257) with
 // entropies, both directions, 325 and with four 343.
 constexpr int BWD_NT = 256, BWD_U = 2;
+// Rows of fewer classes go a wave a chunk.
+constexpr int BWD_SHORT = 4096;
 
-template <bool ENT, bool NTS>
+// A unit of TPU threads (a block, or a wave in rows of few classes) takes a chunk of a row.
+template <int TPU, bool ENT, bool NTS>
 __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ x, const int64_t* __restrict__ ids,
                                                       const float* __restrict__ saved, const float* __restrict__ gl,
                                                       const float* __restrict__ gh, const float* __restrict__ gloss,
-                                                      float* __restrict__ dx, int c, int chunks, int64_t row0,
+                                                      float* __restrict__ dx, int c, int chunks, int64_t row0, unsigned rows,
                                                       float scale2, float inv_t, int* guard, const MeanOf mean) {
-  static_assert(BWD_NT == MEAN_NT);
+  static_assert(BWD_NT == MEAN_NT);  // the block more that takes a mean
   const unsigned more = mean.count ? 1 : 0;
   if (blockIdx.x < more) {
     mean.by_block();
     return;
   }
   // the last rows first
-  const unsigned rows = (gridDim.x - more) / (unsigned)chunks;
-  const RowPiece of(blockIdx.x - more, rows, (unsigned)chunks);
+  const unsigned unit = (blockIdx.x - more) * (BWD_NT / TPU) + threadIdx.x / TPU;
+  if (unit >= rows * (unsigned)chunks) return;
+  const RowPiece of = TPU == BWD_NT ? RowPiece(unit, rows, (unsigned)chunks) : RowPiece(unit, 0, (unsigned)chunks);
   const int64_t row = row0 + rows - 1 - of.row;
   const int chunk = of.piece;
-  const int t = threadIdx.x;
+  const int t = threadIdx.x & (TPU - 1);
   const int64_t id = ids[row];
   const f4 sv = *reinterpret_cast<const f4u*>(saved + 4 * row);
   const float up = (gloss ? gloss[0] : 1.f) * inv_t;
@@ -96,27 +101,28 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
   const float* xr = x + row * c;
   float* dr = dx + row * c;
   // the float4s as the logits lie; the gradient may lie otherwise
-  const RowLay lay(xr, c);
+  const RowLay<> lay(xr, c);
   const f4* x4 = reinterpret_cast<const f4*>(xr + lay.head);
   f4u* d4 = reinterpret_cast<f4u*>(dr + lay.head);
   auto put = [&](const f4& v, int q) {
     if constexpr (NTS) __builtin_nontemporal_store(v, d4 + q);
     else d4[q] = v;
   };
-  const int c0 = chunk * (BWD_NT * BWD_U) + t;
+  // the row's float4s in chunks as long as each other
+  const int each = (lay.c4 + chunks - 1) / chunks, c0 = chunk * each + t, end = min(chunk * each + each, lay.c4);
   const int e = chunk == 0 ? lay.edge(t, c) : -1;
   if (none) {
 #pragma unroll
     for (int u = 0; u < BWD_U; ++u)
-      if (c0 + u * BWD_NT < lay.c4) put(f4{0.f, 0.f, 0.f, 0.f}, c0 + u * BWD_NT);
+      if (c0 + u * TPU < end) put(f4{0.f, 0.f, 0.f, 0.f}, c0 + u * TPU);
     if (e >= 0) dr[e] = 0.f;
     return;
   }
   f4 v[BWD_U];
 #pragma unroll
   for (int u = 0; u < BWD_U; ++u) {
-    const int q = c0 + u * BWD_NT;
-    if (q < lay.c4) v[u] = ld_stream(x4 + q);
+    const int q = c0 + u * TPU;
+    if (q < end) v[u] = ld_stream(x4 + q);
   }
   const float m = sv.x, rest = sv.y, total = sv.z, off = sv.w;
   const float alpha = -(a + b * off) / total, beta = -b * (float)LOG_2 / total;
@@ -133,8 +139,8 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
   const int at = lay.slot((int)id), comp = lay.component((int)id);
 #pragma unroll
   for (int u = 0; u < BWD_U; ++u) {
-    const int q = c0 + u * BWD_NT;
-    if (q >= lay.c4) continue;
+    const int q = c0 + u * TPU;
+    if (q >= end) continue;
     f4 d = f4{grad(v[u].x), grad(v[u].y), grad(v[u].z), grad(v[u].w)};
     if (q == at) d = put_at(d, comp, chosen(xr[id]));
     put(d, q);
@@ -222,20 +228,28 @@ int launch_token_parts(const TokenRows& in, f4* parts, const char* what) {
 int launch_token_bwd(const float* x, const int64_t* ids, const float* saved, const float* gl, const float* gh,
                      const float* gloss, float* dx, int64_t n, int64_t c, float temperature, const char* what,
                      const MeanOf& mean) {
-  const int64_t chunks = ceil_div(c, (int64_t)BWD_NT * BWD_U * 4), most = rows_a_launch(chunks, BWD_NT);
+  const bool waves = c < BWD_SHORT;
+  const int64_t chunks = ceil_div(c, (int64_t)(waves ? 64 : BWD_NT) * BWD_U * 4), most = rows_a_launch(chunks, BWD_NT);
   const float scale2 = (float)(1.4426950408889634 / temperature), inv_t = (float)(1.0 / (double)temperature);
   const bool nt = nt_stream_stores(n * c * 4);
   for (int64_t r0 = 0; r0 < n; r0 += most) {
     const int64_t rows = n - r0 < most ? n - r0 : most;
     const MeanOf also = r0 ? MeanOf{} : mean;
-    const dim3 grid((unsigned)(rows * chunks + (also.count ? 1 : 0)));
-#define OXI_TB(ENT, NTS)                                                                                          \
-  token_bwd_k<ENT, NTS><<<grid, dim3(BWD_NT), 0, stream()>>>(x, ids, saved, gl, gh, gloss, dx, (int)c, (int)chunks, \
-                                                             r0, scale2, inv_t, guard_flag(), also)
-    if (gh && nt) OXI_TB(true, true);
-    else if (gh) OXI_TB(true, false);
-    else if (nt) OXI_TB(false, true);
-    else OXI_TB(false, false);
+    const dim3 grid((unsigned)(ceil_div(rows * chunks, waves ? BWD_NT / 64 : 1) + (also.count ? 1 : 0)));
+#define OXI_TB(TPU, ENT, NTS)                                                                                         \
+  token_bwd_k<TPU, ENT, NTS><<<grid, dim3(BWD_NT), 0, stream()>>>(x, ids, saved, gl, gh, gloss, dx, (int)c, (int)chunks, \
+                                                                  r0, (unsigned)rows, scale2, inv_t, guard_flag(), also)
+#define OXI_TU(TPU)                     \
+  if (gh && nt) OXI_TB(TPU, true, true); \
+  else if (gh) OXI_TB(TPU, true, false); \
+  else if (nt) OXI_TB(TPU, false, true); \
+  else OXI_TB(TPU, false, false)
+    if (waves) {
+      OXI_TU(64);
+    } else {
+      OXI_TU(BWD_NT);
+    }
+#undef OXI_TU
 #undef OXI_TB
   }
   return check_launch(what);

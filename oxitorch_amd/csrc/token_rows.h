@@ -56,7 +56,7 @@ struct TokenRows {
 
   // An id past the classes raises the guard and is padding.
   __device__ __forceinline__ bool counts(int64_t row, int64_t id) const {
-    if (id >= c && (threadIdx.x & 63) == 0) atomicOr(guard, 1);
+    if (id >= c && (threadIdx.x & 15) == 0) atomicOr(guard, 1);
     return id >= 0 && id < c && (!weights || weights[row] != 0.f) &&
            (!starts || (row >= starts[0] && row < starts[sequences]));
   }
@@ -102,14 +102,20 @@ __device__ __forceinline__ f4 put_at(const f4& v, int i, float a) {
   return f4{i == 0 ? a : v.x, i == 1 ? a : v.y, i == 2 ? a : v.z, i == 3 ? a : v.w};
 }
 
-// How a row of C classes lies: `head` classes, float4s, up to 3 classes more.
+// How a row of C classes lies: `head` classes, float4s, up to 3 classes more. The float4s
+// begin at a 128-byte line (WHOLE; short rows: 16 bytes) or at 16 bytes.
+template <bool WHOLE = true>
 struct RowLay {
+  static constexpr int EDGE = WHOLE ? 32 : 4;  // more than a head's classes
   int head, c4;
-  __device__ __forceinline__ RowLay(const float* row, int C) : head(min(row_head(row, C), C)), c4((C - head) >> 2) {}
+  __device__ __forceinline__ RowLay(const float* row, int C) : head(min(row_head(row, C), C)) {
+    if (!WHOLE) head = min((int)(row_head(row, C) & 3), C);
+    c4 = (C - head) >> 2;
+  }
   // The class outside the float4s that thread t takes, or -1.
   __device__ __forceinline__ int edge(int t, int C) const {
-    const int e = t < 32 ? t : head + 4 * c4 + t - 32;
-    return (t < 32 ? t < head : t < 35 && e < C) ? e : -1;
+    const int e = t < EDGE ? t : head + 4 * c4 + t - EDGE;
+    return (t < EDGE ? t < head : t < EDGE + 3 && e < C) ? e : -1;
   }
   // The float4 of class a, or -1 outside of them; its component.
   __device__ __forceinline__ int slot(int a) const { return a >= head && a < head + 4 * c4 ? (a - head) >> 2 : -1; }
@@ -215,7 +221,7 @@ int launch_token_bwd(const float* x, const int64_t* ids, const float* saved, con
                      const MeanOf& mean = {});
 
 // ---------------------------------------------------------------------------
-// A row a group of RT threads (a wave, four to a block, or a block), held in
+// A row a group of RT threads (16 lanes, a wave, or a block), held in
 // registers as NV float4s a thread: the logits cross HBM once for the loss and its
 // gradient. Every thread works the row's few 64-bit formulas out by itself: from the
 // first wave through LDS (8192, 32000) took 324 us against 316.
@@ -241,23 +247,40 @@ __device__ __forceinline__ int64_t row_of_block(uint32_t b, int64_t n) {
   return (int64_t)g + 128 <= n ? (int64_t)(g + (b & 7) * 16 + ((b >> 3) & 15)) : (int64_t)b;
 }
 
-constexpr int rows_block(int rt) { return rt == 64 ? 256 : rt; }
-// Waves a SIMD that the registers must allow.
-constexpr int rows_waves(int nv) { return nv >= 10 ? 4 : 8; }
+// Over a group of RT threads: 16 lanes, a wave or a block.
+template <int RT, class R>
+__device__ __forceinline__ typename R::T over_group(typename R::T v, typename R::T* slots) {
+  if constexpr (RT >= 64) {
+    return over_block<RT, R>(v, slots);
+  } else {
+    static_assert(RT == 16);
+    v = R::op(v, R::template move<DPP_QUAD_XOR1>(v));
+    v = R::op(v, R::template move<DPP_QUAD_XOR2>(v));
+    v = R::op(v, R::template move<DPP_ROW_HALF_MIRROR>(v));
+    return R::op(v, R::template move<DPP_ROW_MIRROR>(v));
+  }
+}
+
+constexpr int rows_block(int rt) { return rt <= 64 ? 256 : rt; }
+// Waves a SIMD: what the registers must allow, and at most, so that rows written as they
+// are read do not crowd each other out.
+constexpr int rows_waves(int rt, int nv) { return rt == 1024 && nv <= 8 ? 8 : 4; }
+constexpr int rows_waves_most(bool grad, int nv) { return grad && nv >= 10 ? 4 : 8; }
 
 template <int RT, int NV, bool GRAD, bool ENT, bool NTS, class Op>
-__global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(RT == 1024 && NV <= 8 ? 8 : 4))) void token_rows_k(
+__global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(rows_waves(RT, NV), rows_waves_most(GRAD, NV)))) void token_rows_k(
     const TokenRows in, const Op op, float* __restrict__ dx) {
-  __shared__ __align__(8) float lds[3 * (RT / 64)];
-  const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
-  const int64_t row = RT == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : row_of_block(blockIdx.x, in.n);
-  if (RT == 64 && row >= in.n) return;
+  __shared__ __align__(8) float lds[RT > 64 ? 3 * (RT / 64) : 2];
+  constexpr int ROWS = rows_block(RT) / RT;  // a block
+  const int t = ROWS > 1 ? threadIdx.x & (RT - 1) : threadIdx.x;
+  const int64_t row = ROWS > 1 ? (int64_t)blockIdx.x * ROWS + threadIdx.x / RT : row_of_block(blockIdx.x, in.n);
+  if (ROWS > 1 && row >= in.n) return;
   const int C = in.c;
   const float* xr = in.x + row * C;
   float* dr = dx + row * C;
   const int64_t id64 = in.ids[row];
   const typename Op::Given given = op.load(row);
-  const RowLay lay(xr, C);
+  const RowLay<(RT > 16)> lay(xr, C);
   auto put = [&](const f4& d, int c) {
     f4u* const p = reinterpret_cast<f4u*>(reinterpret_cast<char*>(dr + lay.head) + (uint32_t)c * 16u);
     if constexpr (NTS) __builtin_nontemporal_store(d, p);
@@ -291,7 +314,7 @@ __global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(
     if (q == at_q && t == at_t) v[q] = drop(v[q], comp);
     m = fmaxf(m, max4(v[q]));
   }
-  m = over_block<RT, MaxF32>(m, lds);
+  m = over_group<RT, MaxF32>(m, lds);
   // With an entropy's gradient the registers keep t, else 2^t.
   float s = 0.f, et = 0.f;
   auto add = [&](float x) {
@@ -304,7 +327,7 @@ __global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(
 #pragma unroll
   for (int q = 0; q < NV; ++q) v[q] = f4{add(v[q].x), add(v[q].y), add(v[q].z), add(v[q].w)};
   v1 = add(v1);
-  const Two both = over_block<RT, Both<AddF32>>(Two{s, et}, reinterpret_cast<Two*>(lds + RT / 64));
+  const Two both = over_group<RT, Both<AddF32>>(Two{s, et}, reinterpret_cast<Two*>(lds + RT / 64));
   const RowStats r = row_stats(m, xa, (double)both.a, (double)both.b, in.scale2, in.inv_t);
   const Two k = op.finish(row, given, r, t == 0);
   if constexpr (GRAD) {
@@ -328,7 +351,7 @@ __global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(
 
 // The row kernel for c classes: as few threads as hold the row; false past ROWS_MAX of
 // them (without a gradient past Op::READ_MAX) and under 8, where none does.
-constexpr int ROWS_MAX = 65536, ROWS_MAX_READ = PART_NT * PART_U * 4;
+constexpr int ROWS_MAX = 32768, ROWS_MAX_READ = 16384;
 template <bool GRAD, bool ENT, bool NTS, class Op>
 bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx) {
   const int c4 = in.c / 4;  // at most
@@ -336,10 +359,11 @@ bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx) {
 #define OXI_TR(RT, NV)                                                                                        \
   if constexpr (GRAD || RT * NV * 4 <= Op::READ_MAX) if (c4 <= RT * NV) {                                    \
     token_rows_k<RT, NV, GRAD, ENT, NTS, Op>                                                                  \
-        <<<dim3((unsigned)(RT == 64 ? ceil_div(in.n, 4) : in.n)), dim3(rows_block(RT)), 0, stream()>>>(in, op, dx); \
+        <<<dim3((unsigned)ceil_div(in.n, rows_block(RT) / RT)), dim3(rows_block(RT)), 0, stream()>>>(in, op, dx);     \
     return true;                                                                                              \
   }
-  OXI_TR(64, 2)
+  OXI_TR(16, 4)
+  OXI_TR(16, 8)
   OXI_TR(64, 4)
   OXI_TR(64, 8)
   OXI_TR(256, 4)
@@ -351,11 +375,6 @@ bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx) {
   OXI_TR(512, 12)
   OXI_TR(512, 14)
   OXI_TR(512, 16)
-  OXI_TR(1024, 10)
-  OXI_TR(1024, 12)
-  OXI_TR(1024, 13)
-  OXI_TR(1024, 14)
-  OXI_TR(1024, 16)
 #undef OXI_TR
   return false;
 }
@@ -395,7 +414,7 @@ __device__ __forceinline__ float take_word(const uint64_t* p) {
 }
 
 template <int NV, bool GRAD, bool ENT, bool NTS, class Op>
-__global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4))) void token_cluster_k(
+__global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4, 4))) void token_cluster_k(
     const TokenRows in, const Op op, float* __restrict__ dx, const Cluster cl) {
   constexpr int RT = CLUSTER_RT;
   __shared__ __align__(8) float lds[3 * (RT / 64)];
@@ -411,7 +430,7 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4)))
   const float* xr = in.x + row * C;
   float* dr = dx + row * C;
   const int64_t id64 = in.ids[row];
-  const RowLay lay(xr, C);
+  const RowLay<> lay(xr, C);
   const int c0 = piece * (RT * NV) + t;
   auto put = [&](const f4& d, int c) {
     f4u* const p = reinterpret_cast<f4u*>(dr + lay.head) + c;
@@ -512,9 +531,19 @@ bool launch_token_cluster(const TokenRows& in, const Op& op, float* dx, void* wo
   const int blocks = cluster_blocks(in.c);
   if (!blocks || !grid_fits(in.n * blocks, CLUSTER_RT)) return false;
   const Cluster cl = start_cluster(workspace, in.n, blocks);
-  token_cluster_k<CLUSTER_NV, GRAD, ENT, NTS, Op>
-      <<<dim3((unsigned)(in.n * blocks)), dim3(CLUSTER_RT), 0, stream()>>>(in, op, dx, cl);
-  return true;
+  const dim3 grid((unsigned)(in.n * blocks));
+#define OXI_TC(NV)                                                                                           \
+  if ((int64_t)blocks * CLUSTER_RT * NV * 4 >= in.c) {                                                       \
+    token_cluster_k<NV, GRAD, ENT, NTS, Op><<<grid, dim3(CLUSTER_RT), 0, stream()>>>(in, op, dx, cl);        \
+    return true;                                                                                             \
+  }
+  OXI_TC(9)
+  OXI_TC(10)
+  OXI_TC(12)
+  OXI_TC(14)
+  OXI_TC(CLUSTER_NV)
+#undef OXI_TC
+  return false;
 }
 
 // Whether sizes and temperature can be taken; 0 or an error's code.
