@@ -19,7 +19,8 @@ namespace oxi {
 namespace {
 
 struct PolicyOp {
-  static constexpr int READ_MAX = ROWS_MAX;  // the same bits with a gradient and without
+  static constexpr bool SAME_BITS = true;  // with a gradient and without
+  static constexpr int FEW_MAX = ROWS_MAX;
   const float *adv, *old, *ref, *weights;
   float *rows, *logp, *coef, *saved;
   int64_t n;

@@ -28,19 +28,18 @@ __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* 
   const RowLay<> lay(xr, in.c);
   const int at = lay.slot((int)id), comp = lay.component((int)id);
   const f4* x4 = reinterpret_cast<const f4*>(xr + lay.head);
-  // the row's float4s in parts as long as each other
-  const int each = (lay.c4 + np - 1) / np, c0 = part * each + t, end = min(part * each + each, lay.c4);
+  const int c0 = part * (PART_NT * PART_U) + t;
   f4 v[PART_U];
   float m = NEG_INF;
 #pragma unroll
   for (int u = 0; u < PART_U; ++u) {
     const int q = c0 + u * PART_NT;
     v[u] = f4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-    if (q < end) v[u] = AGAIN ? x4[q] : ld_stream(x4 + q);
+    if (q < lay.c4) v[u] = AGAIN ? x4[q] : ld_stream(x4 + q);
   }
 #pragma unroll
   for (int u = 0; u < PART_U; ++u)
-    if (c0 + u * PART_NT == at && at < end) v[u] = drop(v[u], comp);
+    if (c0 + u * PART_NT == at) v[u] = drop(v[u], comp);
   const int e = part == 0 ? lay.edge(t, in.c) : -1;
   const float v1 = e >= 0 && e != (int)id ? xr[e] : NEG_INF;
 #pragma unroll
@@ -108,8 +107,9 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
     if constexpr (NTS) __builtin_nontemporal_store(v, d4 + q);
     else d4[q] = v;
   };
-  // the row's float4s in chunks as long as each other
-  const int each = (lay.c4 + chunks - 1) / chunks, c0 = chunk * each + t, end = min(chunk * each + each, lay.c4);
+  // a wave's chunks are as long as each other, in lines of 128 bytes
+  const int each = TPU == BWD_NT ? TPU * BWD_U : ((lay.c4 + chunks - 1) / chunks + 7) & ~7;
+  const int c0 = chunk * each + t, end = min(chunk * each + each, lay.c4);
   const int e = chunk == 0 ? lay.edge(t, c) : -1;
   if (none) {
 #pragma unroll
@@ -149,7 +149,8 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
 }
 
 struct LogpOp {
-  static constexpr int READ_MAX = ROWS_MAX_READ;
+  static constexpr bool SAME_BITS = false;  // there is one way
+  static constexpr int FEW_MAX = 16384;
   float *logp, *entropy, *saved;
   struct Given {};
   __device__ __forceinline__ Given load(int64_t) const { return {}; }
@@ -212,8 +213,7 @@ static int64_t rows_a_launch(int64_t blocks, int threads) { return (0xffffffffll
 
 int launch_token_parts(const TokenRows& in, f4* parts, const char* what) {
   const int64_t np = row_parts(in.c), most = rows_a_launch(np, PART_NT);
-  // the last rows, with which the backward begins, are read with plain loads
-  const int64_t cold = in.again ? in.n - REREAD_BYTES / (4 * (int64_t)in.c) : in.n;
+  const int64_t cold = first_reread(in);
   for (int64_t r0 = 0; r0 < in.n;) {
     const int64_t end = r0 < cold && cold < in.n ? cold : in.n;
     const int64_t rows = end - r0 < most ? end - r0 : most;
