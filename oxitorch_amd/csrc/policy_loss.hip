@@ -95,18 +95,34 @@ bool launch_rows(const TokenRows& in, const PolicyOp& op, float* dx, bool ent, v
 // The parts' sums, or a cluster's words, which are no more than the parts.
 int64_t workspace_bytes(int64_t n, int64_t c) { return 64 + n * row_parts(c) * 3 * (int64_t)sizeof(uint64_t); }
 
-// out[i] = sum over the rows of w rows[i] / divisor in float64, in a fixed order: one block.
-__global__ __launch_bounds__(1024) void policy_mean_k(const TokenRows in, const float* __restrict__ rows, double inv_div,
-                                                      float* __restrict__ out) {
-  __shared__ double red[1024 / 64];
-  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+// A block's four sums over the rows i0, i0 + step, .. of w rows[k], in float64.
+struct FourSums {
+  double v[4];
+};
+template <int N>
+__device__ __forceinline__ FourSums block_sums(FourSums s, double* red) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s.v[k] = block_sum<N>(s.v[k], red);
+  return s;
+}
+
+constexpr int MEAN_THREADS = 1024, MEAN_ROWS = 8192;  // rows a block
+
+// The sums over each MEAN_ROWS rows, a block each in a fixed order: times `by` to out where there is one,
+// else to parts. (8192 rows 6.4 us.)
+__global__ __launch_bounds__(MEAN_THREADS) void policy_mean_k(const TokenRows in, const float* __restrict__ rows,
+                                                              double by, float* __restrict__ out,
+                                                              double* __restrict__ parts) {
+  __shared__ double red[MEAN_THREADS / 64];
+  FourSums acc{};
   constexpr int U = 4;  // rows in flight a thread
-  for (int64_t i0 = threadIdx.x; i0 < in.n; i0 += U * 1024) {
+  const int64_t end = min(in.n, ((int64_t)blockIdx.x + 1) * MEAN_ROWS);
+  for (int64_t i0 = (int64_t)blockIdx.x * MEAN_ROWS + threadIdx.x; i0 < end; i0 += U * MEAN_THREADS) {
     int64_t id[U];
     float w[U], v[4][U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t i = min(i0 + u * 1024, in.n - 1);
+      const int64_t i = min(i0 + u * MEAN_THREADS, end - 1);
       id[u] = in.ids[i];
       w[u] = in.weights ? in.weights[i] : 1.f;
 #pragma unroll
@@ -114,16 +130,31 @@ __global__ __launch_bounds__(1024) void policy_mean_k(const TokenRows in, const 
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (i0 + u * 1024 >= in.n || id[u] < 0 || id[u] >= in.c || w[u] == 0.f) continue;
+      if (i0 + u * MEAN_THREADS >= end || id[u] < 0 || id[u] >= in.c || w[u] == 0.f) continue;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += (double)w[u] * (double)v[k][u];
+      for (int k = 0; k < 4; ++k) acc.v[k] += (double)w[u] * (double)v[k][u];
     }
   }
+  acc = block_sums<MEAN_THREADS>(acc, red);
+  if (threadIdx.x) return;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const double v = block_sum<1024>(acc[k], red);
-    if (threadIdx.x == 0) out[k] = (float)(v * inv_div);
+    if (gridDim.x == 1) out[k] = (float)(acc.v[k] * by);
+    else parts[4 * blockIdx.x + k] = acc.v[k];
   }
+}
+
+__global__ __launch_bounds__(256) void policy_mean_parts_k(const double* __restrict__ parts, int count, double by,
+                                                           float* __restrict__ out) {
+  __shared__ double red[256 / 64];
+  FourSums acc{};
+  for (int i = threadIdx.x; i < count; i += 256)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc.v[k] += parts[4 * i + k];
+  acc = block_sums<256>(acc, red);
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = (float)(acc.v[k] * by);
 }
 
 }  // namespace
@@ -183,7 +214,11 @@ int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* ad
                                     dlogits, n, c, temperature, what))
         return rc;
   }
-  policy_mean_k<<<1, 1024, 0, stream()>>>(in, rows, inv_div, out);
+  // the rows' launches are done with the workspace, which holds more than the means' parts
+  double* sums = static_cast<double*>(at);
+  const int64_t blocks = ceil_div(n, MEAN_ROWS);
+  policy_mean_k<<<dim3((unsigned)blocks), dim3(MEAN_THREADS), 0, stream()>>>(in, rows, inv_div, out, sums);
+  if (blocks > 1) policy_mean_parts_k<<<1, 256, 0, stream()>>>(sums, (int)blocks, inv_div, out);
   return check_launch(what);
 }
 
