@@ -208,7 +208,7 @@ int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* ad
   if (launch_rows(in, op, dlogits, entropy_coef != 0.f, at)) {
     if (int rc = check_launch(what)) return rc;
   } else {
-    if (int rc = token_rows_read(in, static_cast<f4*>(at), op, what)) return rc;
+    if (int rc = token_rows_by_parts(in, static_cast<f4*>(at), op, what)) return rc;
     if (dlogits)
       if (int rc = launch_token_bwd(logits, ids, saved, coef, entropy_coef != 0.f ? coef + n : nullptr, nullptr,
                                     dlogits, n, c, temperature, what))

@@ -392,24 +392,25 @@ bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx, bool man
     OXI_TR(512, 12)
     OXI_TR(512, 14)
     OXI_TR(512, 16)
+  } else {
+    OXI_TR(1024, 5)
+    OXI_TR(1024, 6)
+    OXI_TR(1024, 7)
+    OXI_TR(1024, 8)
   }
-  OXI_TR(1024, 5)
-  OXI_TR(1024, 6)
-  OXI_TR(1024, 7)
-  OXI_TR(1024, 8)
 #undef OXI_TR
   return false;
 }
 
 // ---------------------------------------------------------------------------
 // A row a cluster of blocks, each with a piece of it in registers (RT * NV float4s):
-// rows that one block's registers do not hold. The blocks give each other their piece's maximum and sums by words of
-// a value and a flag each, so that no order of memory accesses matters; the words are
-// zeroed by a launch before. A block's row and piece go by a ticket that it takes as
+// rows that one block's registers do not hold. The blocks give each other their piece's
+// maximum and sums by words of a value and a flag each, so that no order of memory
+// accesses matters; the words are zeroed by a launch before. A block's row and piece go by a ticket that it takes as
 // it starts: a block waits only for those of its own row, which have started or take
 // the next tickets, and the rows before finish without it, so every wait ends.
-// (1024, 131072) with an entropy term 187 us, 5.4 TB/s; parts, their join and the
-// backward's pass 238. For few shorter rows, (64, 32000) on 4 blocks each, the ticket
+// (1024, 131072) with an entropy term 190 us, 5.4 TB/s; parts, their join and the
+// backward's pass 244. (4096, 50257) on two blocks 280, on one of 1024 threads 308. For few shorter rows, (64, 32000) on 4 blocks each, the ticket
 // and the words cost what the other CUs gain: 11.0 us against 10.2 on one block.
 constexpr int CLUSTER_RT = 512, CLUSTER_MOST = 16;
 struct Cluster {
@@ -461,7 +462,9 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4, 4
   };
   const int e = piece == 0 ? lay.edge(t, C) : -1;
   const bool lead = piece == 0 && t == 0;
+  uint64_t* const words = cl.words + 3 * cl.blocks * row;
   if (!in.counts(row, id64)) {
+    if (t < 3) give_word(words + 3 * piece + t, 0.f);  // no wait hangs on all blocks seeing the same
     if (lead) op.skip(row);
     if constexpr (GRAD) {
 #pragma unroll
@@ -500,7 +503,6 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4, 4
   for (int q = 0; q < NV; ++q) v[q] = f4{add(v[q].x), add(v[q].y), add(v[q].z), add(v[q].w)};
   v1 = add(v1);
   const Two both = over_block<RT, Both<AddF32>>(Two{s, et}, reinterpret_cast<Two*>(lds + RT / 64));
-  uint64_t* const words = cl.words + 3 * cl.blocks * row;
   if (t < 3) give_word(words + 3 * piece + t, t == 0 ? own : t == 1 ? both.a : both.b);
   if (t < 3 * cl.blocks) from[t] = take_word(words + t);
   __syncthreads();
@@ -575,20 +577,23 @@ TokenRows token_rows(const float* x, const int64_t* ids, int64_t n, int64_t c, f
 // Bytes of the parts of n rows.
 inline int64_t token_parts_bytes(int64_t n, int64_t c) { return n * row_parts(c) * (int64_t)sizeof(f4); }
 
-// The rows' results without a gradient.
+// The rows' results without a gradient: by parts, or, where it takes them, by the row kernel.
+template <class Op>
+int token_rows_by_parts(const TokenRows& in, f4* parts, const Op& op, const char* what) {
+  if (int rc = launch_token_parts(in, parts, what)) return rc;
+  token_join_k<Op><<<dim3((unsigned)ceil_div(in.n, 4)), dim3(256), 0, stream()>>>(in, parts, (int)row_parts(in.c), op);
+  return check_launch(what);
+}
 template <class Op>
 int token_rows_read(const TokenRows& in, f4* parts, const Op& op, const char* what) {
   const int64_t cold = first_reread(in);
   TokenRows some = in;
   some.n = cold;
-  if (launch_token_rows_as<false, false, true>(some, op, nullptr, in.n >= MANY_ROWS)) {
-    some = in;
-    some.row0 = cold;
-    if (cold < in.n) launch_token_rows_as<false, false, false>(some, op, nullptr);
-    return check_launch(what);
-  }
-  if (int rc = launch_token_parts(in, parts, what)) return rc;
-  token_join_k<Op><<<dim3((unsigned)ceil_div(in.n, 4)), dim3(256), 0, stream()>>>(in, parts, (int)row_parts(in.c), op);
+  if (!launch_token_rows_as<false, false, true>(some, op, nullptr, in.n >= MANY_ROWS))
+    return token_rows_by_parts(in, parts, op, what);
+  some = in;
+  some.row0 = cold;
+  if (cold < in.n) launch_token_rows_as<false, false, false>(some, op, nullptr);
   return check_launch(what);
 }
 
