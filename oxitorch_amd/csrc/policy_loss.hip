@@ -20,7 +20,6 @@ namespace {
 
 struct PolicyOp {
   static constexpr bool SAME_BITS = true;  // with a gradient and without
-  static constexpr int FEW_MAX = ROWS_MAX;
   const float *adv, *old, *ref, *weights;
   float *rows, *logp, *coef, *saved;
   int64_t n;

@@ -20,7 +20,6 @@ namespace {
 
 struct PreferenceOp {
   static constexpr bool SAME_BITS = false;  // there is one way
-  static constexpr int FEW_MAX = 16384;
   double* logp;
   float *coef, *saved;
   struct Given {};
@@ -194,7 +193,7 @@ int oxi_preference_loss_fwd(const float* logits, const int64_t* ids, const int64
   in.coef = coef;
   in.saved = saved;
   const int np = (int)row_parts(c);
-  const bool by_pairs = c > (n < MANY_ROWS ? PreferenceOp::FEW_MAX : ROWS_MAX) && np <= JOIN_MOST;
+  const bool by_pairs = c > ROWS_MAX && np <= JOIN_MOST;
   if (n) {
     const int rc = by_pairs ? launch_token_parts(in, parts, what)
                             : token_rows_read(in, parts, PreferenceOp{logp, coef, saved}, what);

@@ -150,7 +150,6 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
 
 struct LogpOp {
   static constexpr bool SAME_BITS = false;  // there is one way
-  static constexpr int FEW_MAX = 16384;
   float *logp, *entropy, *saved;
   struct Given {};
   __device__ __forceinline__ Given load(int64_t) const { return {}; }

@@ -365,14 +365,13 @@ __global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(
 }
 
 // The row kernel for c classes: as few threads as hold the row; false past ROWS_MAX of
-// them and under 8, where none does, and for few rows of more than Op::FEW_MAX, which go
-// by parts over more of the chip where that is open to them.
-constexpr int64_t MANY_ROWS = 512;
+// them and under 8, where none does. Few rows too: 64 of 32000 are read in 7.5 us, by parts
+// over more of the chip and their join in 7.7 (4 rows 7.0 and 6.5, 256 rows 9.7 and 11.4).
 constexpr int ROWS_MAX = 32768;
 template <bool GRAD, bool ENT, bool NTS, class Op>
-bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx, bool many = true) {
+bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx) {
   const int c4 = in.c / 4;  // at most
-  if (in.c < 8 || in.c > ROWS_MAX || (!many && in.c > Op::FEW_MAX)) return false;
+  if (in.c < 8 || in.c > ROWS_MAX) return false;
 #define OXI_TR(RT, NV)                                                                                        \
   if (c4 <= RT * NV) {                                                                                        \
     token_rows_k<RT, NV, GRAD, ENT, NTS, Op>                                                                  \
@@ -589,7 +588,7 @@ int token_rows_read(const TokenRows& in, f4* parts, const Op& op, const char* wh
   const int64_t cold = first_reread(in);
   TokenRows some = in;
   some.n = cold;
-  if (!launch_token_rows_as<false, false, true>(some, op, nullptr, in.n >= MANY_ROWS))
+  if (!launch_token_rows_as<false, false, true>(some, op, nullptr))
     return token_rows_by_parts(in, parts, op, what);
   some = in;
   some.row0 = cold;
