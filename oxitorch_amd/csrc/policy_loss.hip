@@ -19,6 +19,7 @@ namespace oxi {
 namespace {
 
 struct PolicyOp {
+  static constexpr bool SUMMED = false;
   static constexpr bool SAME_BITS = true;  // with a gradient and without
   const float *adv, *old, *ref, *weights;
   float *rows, *logp, *coef, *saved;

@@ -19,6 +19,7 @@ namespace oxi {
 namespace {
 
 struct PreferenceOp {
+  static constexpr bool SUMMED = true;
   static constexpr bool SAME_BITS = false;  // there is one way
   double* logp;
   float *coef, *saved;

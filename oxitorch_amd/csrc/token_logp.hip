@@ -149,6 +149,7 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
 }
 
 struct LogpOp {
+  static constexpr bool SUMMED = true;
   static constexpr bool SAME_BITS = false;  // there is one way
   float *logp, *entropy, *saved;
   struct Given {};
@@ -202,6 +203,7 @@ TokenRows token_rows(const float* x, const int64_t* ids, int64_t n, int64_t c, f
   in.c = (int)c;
   in.scale2 = (float)(1.4426950408889634 / temperature);
   in.inv_t = 1.0 / (double)temperature;
+  in.skew = (double)in.scale2 * (LOG_2 * (double)temperature) - 1.0;
   in.guard = guard_flag();
   return in;
 }

@@ -49,6 +49,7 @@ struct TokenRows {
   int64_t row0;  // the row kernel's first; up to n
   int c;
   float scale2;  // log2(e)/T
+  double skew;   // by how much of itself scale2 is off
   double inv_t;
   int* guard;
   bool again;      // whether the logits are read again by a backward
@@ -69,16 +70,20 @@ struct RowStats {
 };
 
 // From the maximum m, the chosen logit xa and the sums over the other classes of 2^t
-// and 2^t t.
-__device__ __forceinline__ RowStats row_stats(float m, float xa, double rest, double et, float scale2, double inv_t) {
-  const float ta = (xa - m) * scale2;
+// and 2^t t. For values that are SUMMED over a sequence's tokens, what scale2 lost to its
+// rounding, the same in every row, is taken back from logp to first order: d ln s = skew ln 2
+// (sum 2^t t)/s. (A token's own ratio has it in its last bit; there it would cost registers:
+// the policy loss of (8192, 32000) 325 us against 319.)
+template <bool SUMMED>
+__device__ __forceinline__ RowStats row_stats(float m, float xa, double rest, double et, const TokenRows& in) {
+  const float ta = (xa - m) * in.scale2;
   const double ea = (double)__builtin_amdgcn_exp2f(ta);
   const double total = rest + ea;
-  const double d = ((double)xa - (double)m) * inv_t;  // NaN where no class is left
+  const double d = ((double)xa - (double)m) * in.inv_t;  // NaN where no class is left
   const double lt = d == 0.0 ? log1p64(rest) : log64(total);
   const double mean = (et + ea * (double)fmaxf(ta, LEAST_T)) / total;
   RowStats r;
-  r.logp = d - lt;
+  r.logp = d - (SUMMED ? lt - in.skew * (LOG_2 * mean) : lt);
   r.entropy = lt - LOG_2 * mean;
   r.m = m;
   r.rest = (float)rest;
@@ -179,7 +184,7 @@ __device__ __forceinline__ RowStats joined_row(const TokenRows& in, const f4* mi
   for (int p = 0; p < np; ++p) m = fmaxf(m, mine[p].x);
   double s, et;
   join_parts(mine, 0, 1, np, m, in.scale2, s, et);
-  return row_stats(m, xa, s, et, in.scale2, in.inv_t);
+  return row_stats<true>(m, xa, s, et, in);
 }
 
 // A wave a row: joins its parts; `op` writes what the row gives.
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(256) void token_join_k(const TokenRows in, const f4
   join_parts(mine, lane, 64, np, m, in.scale2, s, et);
   s = over_block<64, AddF64>(s, (double*)nullptr);
   et = over_block<64, AddF64>(et, (double*)nullptr);
-  const RowStats r = row_stats(m, xa, s, et, in.scale2, in.inv_t);
+  const RowStats r = row_stats<Op::SUMMED>(m, xa, s, et, in);
   op.finish(row, given, r, lane == 0);
 }
 
@@ -343,7 +348,7 @@ __global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(
   for (int q = 0; q < NV; ++q) v[q] = f4{add(v[q].x), add(v[q].y), add(v[q].z), add(v[q].w)};
   v1 = add(v1);
   const Two both = over_group<RT, Both<AddF32>>(Two{s, et}, reinterpret_cast<Two*>(lds + RT / 64));
-  const RowStats r = row_stats(m, xa, (double)both.a, (double)both.b, in.scale2, in.inv_t);
+  const RowStats r = row_stats<Op::SUMMED>(m, xa, (double)both.a, (double)both.b, in);
   const Two k = op.finish(row, given, r, t == 0);
   if constexpr (GRAD) {
     const RowGrad g(r, xa, in.scale2, (float)in.inv_t, k.a, ENT ? k.b : 0.f);
@@ -515,7 +520,7 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4, 4
     rest += f * (double)from[3 * k + 1];
     mean += f * ((double)from[3 * k + 2] + (double)fmaxf(d, LEAST_T) * (double)from[3 * k + 1]);
   }
-  const RowStats r = row_stats(m, xa, rest, mean, in.scale2, in.inv_t);
+  const RowStats r = row_stats<Op::SUMMED>(m, xa, rest, mean, in);
   const Two k = op.finish(row, op.load(row), r, lead);
   if constexpr (GRAD) {
     const RowGrad g(r, xa, in.scale2, (float)in.inv_t, k.a, ENT ? k.b : 0.f);
