@@ -200,7 +200,6 @@ int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* ad
   if (!workspace && !own.p) return fail_alloc(what);
   TokenRows in = token_rows(logits, ids, n, c, temperature);
   in.weights = weights;
-  in.again = true;
   const double inv_div = 1.0 / (double)divisor;
   const PolicyOp op{advantages, old_logp, ref_logp, weights, rows, logp, coef, saved, n, 1.0 - (double)clip_low,
                     1.0 + (double)clip_high, (double)clip_max, (double)kl_coef, (double)entropy_coef, inv_div};

@@ -190,7 +190,6 @@ int oxi_preference_loss_fwd(const float* logits, const int64_t* ids, const int64
   TokenRows in = token_rows(logits, ids, n, c, 1.f);
   in.starts = starts;
   in.sequences = 2 * pairs;
-  in.again = dlogits != nullptr;
   in.coef = coef;
   in.saved = saved;
   const int np = (int)row_parts(c);

@@ -120,10 +120,6 @@ inline bool nt_stores(int64_t bytes) { return bytes < (int64_t)OXI_NT_STORE_LO |
 // against 45; distillation of (2048, 32000), 262 MB, 97 against 108.
 inline bool nt_stream_stores(int64_t bytes) { return bytes < (int64_t)OXI_NT_STORE_LO || bytes >= (int64_t)128 << 20; }
 
-// What of a tensor that a second pass reads from its end the 256 MB Infinity Cache
-// still holds then: the first pass loads it with plain loads.
-constexpr int64_t REREAD_BYTES = (int64_t)208 << 20;
-
 // How a kernel's rows lie. ROW_FULL: exactly TPR * NV float4s at 16-byte
 // addresses, the length a compile-time constant; ROW_VEC: any multiple of 4
 // floats at 16-byte addresses; ROW_ODD: 4 or more floats at any float address.

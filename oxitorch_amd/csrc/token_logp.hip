@@ -8,8 +8,6 @@
 namespace oxi {
 namespace {
 
-// AGAIN: plain loads, for rows that a backward then finds in the Infinity Cache.
-template <bool AGAIN>
 __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* __restrict__ parts, int np,
                                                         int64_t row0) {
   __shared__ float lds[3 * (PART_NT / 64)];
@@ -35,7 +33,7 @@ __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* 
   for (int u = 0; u < PART_U; ++u) {
     const int q = c0 + u * PART_NT;
     v[u] = f4{NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-    if (q < lay.c4) v[u] = AGAIN ? x4[q] : ld_stream(x4 + q);
+    if (q < lay.c4) v[u] = ld_stream(x4 + q);
   }
 #pragma unroll
   for (int u = 0; u < PART_U; ++u)
@@ -84,7 +82,7 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
     mean.by_block();
     return;
   }
-  // the last rows first
+  // the last rows first: the Infinity Cache still has some of what the forward read last
   const unsigned unit = (blockIdx.x - more) * (BWD_NT / TPU) + threadIdx.x / TPU;
   if (unit >= rows * (unsigned)chunks) return;
   const RowPiece of = TPU == BWD_NT ? RowPiece(unit, rows, (unsigned)chunks) : RowPiece(unit, 0, (unsigned)chunks);
@@ -214,14 +212,9 @@ static int64_t rows_a_launch(int64_t blocks, int threads) { return (0xffffffffll
 
 int launch_token_parts(const TokenRows& in, f4* parts, const char* what) {
   const int64_t np = row_parts(in.c), most = rows_a_launch(np, PART_NT);
-  const int64_t cold = first_reread(in);
-  for (int64_t r0 = 0; r0 < in.n;) {
-    const int64_t end = r0 < cold && cold < in.n ? cold : in.n;
-    const int64_t rows = end - r0 < most ? end - r0 : most;
-    const dim3 grid((unsigned)(rows * np));
-    if (r0 < cold) token_part_k<false><<<grid, dim3(PART_NT), 0, stream()>>>(in, parts, (int)np, r0);
-    else token_part_k<true><<<grid, dim3(PART_NT), 0, stream()>>>(in, parts, (int)np, r0);
-    r0 += rows;
+  for (int64_t r0 = 0; r0 < in.n; r0 += most) {
+    const int64_t rows = in.n - r0 < most ? in.n - r0 : most;
+    token_part_k<<<dim3((unsigned)(rows * np)), dim3(PART_NT), 0, stream()>>>(in, parts, (int)np, r0);
   }
   return check_launch(what);
 }
@@ -281,9 +274,7 @@ int oxi_token_logp_fwd(const float* logits, const int64_t* ids, float* logp, flo
   Workspace own(workspace ? 0 : (size_t)token_parts_bytes(n, c));
   if (!workspace && !own.p) return fail_alloc(what);
   f4* parts = static_cast<f4*>(workspace ? workspace : own.p);
-  TokenRows in = token_rows(logits, ids, n, c, temperature);
-  in.again = saved != nullptr;
-  return token_rows_read(in, parts, LogpOp{logp, entropy, saved}, what);
+  return token_rows_read(token_rows(logits, ids, n, c, temperature), parts, LogpOp{logp, entropy, saved}, what);
 }
 
 int oxi_token_logp_bwd(const float* logits, const int64_t* ids, const float* saved, const float* glogp,

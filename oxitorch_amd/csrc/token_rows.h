@@ -46,13 +46,11 @@ struct TokenRows {
   const int64_t* starts;  // rows outside [starts[0], starts[sequences]) do not; NULL: all do
   int64_t sequences;
   int64_t n;
-  int64_t row0;  // the row kernel's first; up to n
   int c;
   float scale2;  // log2(e)/T
   double skew;   // by how much of itself scale2 is off
   double inv_t;
   int* guard;
-  bool again;      // whether the logits are read again by a backward
   // where the parts' pass writes 0 for every row, and what rows that do not count keep; NULL: nowhere
   float *coef, *saved;
 
@@ -127,14 +125,6 @@ struct RowLay {
   __device__ __forceinline__ int slot(int a) const { return a >= head && a < head + 4 * c4 ? (a - head) >> 2 : -1; }
   __device__ __forceinline__ int component(int a) const { return (a - head) & 3; }
 };
-
-// The first of the rows that are read with plain loads: those with which a backward begins, of
-// more logits than the Infinity Cache holds. Fewer are read as fast with the others (12000 rows of
-// 2048 in pairs 65 us, with plain loads 74).
-inline int64_t first_reread(const TokenRows& in) {
-  const int64_t cold = in.n - REREAD_BYTES / (4 * (int64_t)in.c);
-  return in.again && cold > in.n / 8 ? cold : in.n;
-}
 
 // Row and piece of block b of a launch of `pieces` blocks a row: a row's blocks on one XCD (blocks
 // go round the 8 of them), so that what they all read of it misses one L2 once: (6100, 32000)
@@ -281,16 +271,13 @@ constexpr int rows_block(int rt) { return rt <= 64 ? 256 : rt; }
 constexpr int rows_waves(int rt, int nv) { return rt == 1024 && nv <= 8 ? 8 : 4; }
 constexpr int rows_waves_most(bool grad, int nv) { return grad && nv >= 10 ? 4 : 8; }
 
-// Without a gradient, NTS false: plain loads, for rows that a backward then finds in the
-// Infinity Cache.
 template <int RT, int NV, bool GRAD, bool ENT, bool NTS, class Op>
 __global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(rows_waves(RT, NV), rows_waves_most(GRAD, NV)))) void token_rows_k(
     const TokenRows in, const Op op, float* __restrict__ dx) {
   __shared__ __align__(8) float lds[RT > 64 ? 3 * (RT / 64) : 2];
   constexpr int ROWS = rows_block(RT) / RT;  // a block
   const int t = ROWS > 1 ? threadIdx.x & (RT - 1) : threadIdx.x;
-  const int64_t row = in.row0 + (ROWS > 1 ? (int64_t)blockIdx.x * ROWS + threadIdx.x / RT
-                                          : row_of_block(blockIdx.x, in.n - in.row0));
+  const int64_t row = ROWS > 1 ? (int64_t)blockIdx.x * ROWS + threadIdx.x / RT : row_of_block(blockIdx.x, in.n);
   if (ROWS > 1 && row >= in.n) return;
   const int C = in.c;
   const float* xr = in.x + row * C;
@@ -320,12 +307,9 @@ __global__ __launch_bounds__(rows_block(RT)) __attribute__((amdgpu_waves_per_eu(
   const float xa = xr[id];
   f4 v[NV];
 #pragma unroll
-  for (int q = 0; q < NV; ++q) {
-    const f4* const p = reinterpret_cast<const f4*>(reinterpret_cast<const char*>(xr + lay.head) +
-                                                    (uint32_t)min(q * RT + t, lay.c4 - 1) * 16u);
-    if constexpr (GRAD || NTS) v[q] = ld_stream(p);
-    else v[q] = *p;
-  }
+  for (int q = 0; q < NV; ++q)
+    v[q] = ld_stream(reinterpret_cast<const f4*>(reinterpret_cast<const char*>(xr + lay.head) +
+                                                 (uint32_t)min(q * RT + t, lay.c4 - 1) * 16u));
   float v1 = e >= 0 && e != id ? xr[e] : NEG_INF;
   float m = fmaxf(v1, xa);
 #pragma unroll
@@ -380,7 +364,7 @@ bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx) {
 #define OXI_TR(RT, NV)                                                                                        \
   if (c4 <= RT * NV) {                                                                                        \
     token_rows_k<RT, NV, GRAD, ENT, NTS, Op>                                                                  \
-        <<<dim3((unsigned)ceil_div(in.n - in.row0, rows_block(RT) / RT)), dim3(rows_block(RT)), 0, stream()>>>(in, op, dx);     \
+        <<<dim3((unsigned)ceil_div(in.n, rows_block(RT) / RT)), dim3(rows_block(RT)), 0, stream()>>>(in, op, dx); \
     return true;                                                                                              \
   }
   OXI_TR(16, 4)
@@ -590,15 +574,8 @@ int token_rows_by_parts(const TokenRows& in, f4* parts, const Op& op, const char
 }
 template <class Op>
 int token_rows_read(const TokenRows& in, f4* parts, const Op& op, const char* what) {
-  const int64_t cold = first_reread(in);
-  TokenRows some = in;
-  some.n = cold;
-  if (!launch_token_rows_as<false, false, true>(some, op, nullptr))
-    return token_rows_by_parts(in, parts, op, what);
-  some = in;
-  some.row0 = cold;
-  if (cold < in.n) launch_token_rows_as<false, false, false>(some, op, nullptr);
-  return check_launch(what);
+  return launch_token_rows_as<false, false, false>(in, op, nullptr) ? check_launch(what)
+                                                                    : token_rows_by_parts(in, parts, op, what);
 }
 
 }  // namespace oxi
