@@ -179,6 +179,7 @@ int oxi_preference_loss_fwd(const float* logits, const int64_t* ids, const int64
     return fail(OXI_INVALID_ARGUMENT, "%s: NULL tensor pointer", what);
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(OXI_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
+  if (n && dlogits == logits) return fail(OXI_INVALID_ARGUMENT, "%s: dlogits must not be the logits", what);
   OXI_CHECK_INIT();
   Workspace own(workspace ? 0 : (size_t)workspace_bytes(n, c));
   if (n && !workspace && !own.p) return fail_alloc(what);

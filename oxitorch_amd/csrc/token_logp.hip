@@ -284,6 +284,7 @@ int oxi_token_logp_bwd(const float* logits, const int64_t* ids, const float* sav
   if (int rc = check_token_rows(what, n, c, temperature)) return rc;
   if (n && (!logits || !ids || !saved || !dlogits || (!glogp && !gentropy)))
     return fail(OXI_INVALID_ARGUMENT, "%s: NULL tensor pointer", what);
+  if (n && dlogits == logits) return fail(OXI_INVALID_ARGUMENT, "%s: dlogits must not be the logits", what);
   OXI_CHECK_INIT();
   if (n == 0) return OXI_OK;
   return launch_token_bwd(logits, ids, saved, glogp, gentropy, gloss, dlogits, n, c, temperature, what);

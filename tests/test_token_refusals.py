@@ -6,6 +6,7 @@ import pytest
 
 N = 1 << 40
 P = 1 << 20  # a non-NULL address that no refused call touches
+Q = 1 << 21  # another
 BAD = (0.0, -1.0, float("nan"), float("inf"))
 
 
@@ -126,6 +127,15 @@ def test_preference_loss(capi):
         call(kind=1, smoothing=0.1)
     with pytest.raises(ValueError, match="16-byte aligned"):
         call(ws=P + 4)
+
+
+def test_gradient_in_place_of_the_logits(capi):
+    with pytest.raises(ValueError, match="must not be the logits"):
+        capi.call("oxi_token_logp_bwd", P, Q, Q, Q, Q, Q, P, 2, 50, 1.0)
+    with pytest.raises(ValueError, match="must not be the logits"):
+        capi.call("oxi_policy_loss_fwd", P, *[Q] * 10, P, Q, 2, 50, 1.0, 0.2, 0.2, 0.0, 0.0, 0.0, 1.0)
+    with pytest.raises(ValueError, match="must not be the logits"):
+        capi.call("oxi_preference_loss_fwd", P, *[Q] * 8, P, Q, 2, 50, 1, 0, 0, 0.1, 0.0, 0.0)
 
 
 def test_grad_norm_and_clip(capi):
