@@ -3,11 +3,13 @@
 //   total = (sum |g|^p)^(1/p), p = 1 or 2, or max |g|
 //   out = g * min(1, max_norm / (total + 1e-6))
 //
-// Every tensor is cut into chunks, a block each; the tensors' places
-// travel in the kernel arguments, up to MOST_SLICES a launch. The terms are squared and
-// summed in 64 bits (no overflow, and a sum over 10^9 terms keeps its digits), a sum a
-// chunk, then one block adds the chunks' in a fixed order. The clipping reads total on
-// the device, so nothing waits for the host between the two.
+// Every tensor is cut into chunks, a block each; the tensors' places travel in the kernel
+// arguments, up to MOST_SLICES a launch. The terms are squared and summed in 64 bits (no
+// overflow, and a sum over 10^9 terms keeps its digits), a sum a chunk, then one block
+// adds the chunks' in a fixed order. The clipping reads total on the device, so nothing
+// waits for the host between the two.
+//
+// HBM bounds it: 354 M floats in 242 tensors, norm 220 us (6.4 TB/s) and clipping 450 (6.3).
 #include <cmath>
 
 #include "internal.h"
@@ -21,12 +23,13 @@ namespace {
 constexpr int NT = 256;
 constexpr int UNROLL = 4;               // float4s in flight a thread
 constexpr int STEP = NT * UNROLL * 4;   // floats that a block has in flight
-// Floats a block of the norm's: STEP, or many of them where that still fills the chip
-// many times over, so that the chunks' sums are few.
+// Floats a block of the norm's: STEP, or, from MANY floats on, several of them, so that the
+// chunks' sums are few (10^8 floats 71 us against 75, 4 * 10^7 32 against 34; with 4 steps 72 and 36).
 constexpr int LONG_STEPS = 8;
 constexpr int64_t MANY = (int64_t)1 << 25;
 inline int64_t chunk_of(int64_t total) { return total >= MANY ? (int64_t)STEP * LONG_STEPS : STEP; }
-// Of the clipping's: loads in a loop would wait behind the stores before them.
+// Of the clipping's, without a loop, whose loads would wait behind the stores before them: two float4s
+// a thread (354 M floats, norm and clipping 673 us; one 682, four 675, in a loop of 8 784).
 constexpr int CLIP_UNROLL = 2, CLIP_CHUNK = NT * CLIP_UNROLL * 4;
 constexpr int MOST_SLICES = 96;
 // What of the gradients the clipping, which begins at their end, finds in the 256 MB Infinity Cache:

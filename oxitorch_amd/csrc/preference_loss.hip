@@ -55,7 +55,7 @@ struct PairArgs {
 __device__ __forceinline__ double softplus(double x) { return (x > 0.0 ? x : 0.0) + log1p64(exp64(-fabs(x))); }
 
 // Threads of a pair's block, half of them to each sequence; the most parts a row of rows that
-// they join, a row a thread (96 rows of 32000 in 2 pairs 7 us; a wave a row in a launch of its
+// they join, a row a thread (92 rows of 32000 in 2 pairs 7 us; a wave a row in a launch of its
 // own, 256 threads a pair and a launch for the mean took 10.5).
 constexpr int PAIR_NT = 1024, HALF = PAIR_NT / 2, JOIN_MOST = 16;
 

@@ -63,7 +63,7 @@ __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* 
   if (t == 0) parts[row * np + part] = f4{m, both.a, both.b, 0.f};
 }
 
-// Two float4s a thread: (6100, 32000) of pairs 322 us, with one 329, with four 335; (4096, 50257) with
+// Two float4s a thread: (6288, 32000) of pairs 322 us, with one 329, with four 335; (4096, 50257) with
 // entropies, both directions, 325 and with four 343.
 constexpr int BWD_NT = 256, BWD_U = 2;
 // Rows of fewer classes go a wave a chunk.

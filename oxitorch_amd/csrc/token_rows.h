@@ -127,7 +127,7 @@ struct RowLay {
 };
 
 // Row and piece of block b of a launch of `pieces` blocks a row: a row's blocks on one XCD (blocks
-// go round the 8 of them), so that what they all read of it misses one L2 once: (6100, 32000)
+// go round the 8 of them), so that what they all read of it misses one L2 once: (6288, 32000)
 // of pairs 322 us against 343, log-probabilities of (8192, 32000) 165 against 170.
 struct RowPiece {
   int64_t row;
