@@ -66,7 +66,8 @@ __global__ __launch_bounds__(PART_NT) void token_part_k(const TokenRows in, f4* 
 // Two float4s a thread: (6288, 32000) of pairs 322 us, with one 329, with four 335; (4096, 50257) with
 // entropies, both directions, 325 and with four 343.
 constexpr int BWD_NT = 256, BWD_U = 2;
-// Rows of fewer classes go a wave a chunk.
+// Rows of fewer classes go a wave a chunk: both directions of (16384, 256) 17 us against 31, of (16384,
+// 2051) 76 against 91.
 constexpr int BWD_SHORT = 4096;
 
 // A unit of TPU threads (a block, or a wave in rows of few classes) takes a chunk of a row.
