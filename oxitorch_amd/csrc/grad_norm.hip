@@ -9,7 +9,7 @@
 // adds the chunks' in a fixed order. The clipping reads total on the device, so nothing
 // waits for the host between the two.
 //
-// HBM bounds it: 354 M floats in 242 tensors, norm 220 us (6.4 TB/s) and clipping 450 (6.3).
+// HBM bounds it: 354 M floats in 242 tensors, norm 220 us (6.4 TB/s) and clipping 447 (6.3).
 #include <cmath>
 
 #include "internal.h"
@@ -115,18 +115,25 @@ __global__ __launch_bounds__(NT) void clip_k(const Slices a, const double* __res
   const int64_t n = min(a.n[s], e0 + CLIP_CHUNK);
   const float* g = a.g[s];
   float* out = a.out[s];
+  const bool whole = n - e0 == CLIP_CHUNK;
+  f4 v[CLIP_UNROLL];
+  auto load = [&]() {
+#pragma unroll
+    for (int u = 0; u < CLIP_UNROLL; ++u)
+      v[u] = __builtin_nontemporal_load(reinterpret_cast<const f4u*>(g + e0) + u * NT + threadIdx.x);
+  };
+  // into another tensor the gradients are read in any case: before the norm is known
+  // (354 M floats, both together 668 us; behind it 676)
+  if (whole && out != g) load();
   const double ratio = max_norm / (total[0] + 1e-6);
   const bool clip = ratio < 1.0;  // not for a NaN
   if (!clip && out == g) return;
   const float k = clip ? (float)ratio : 1.f;
-  if (n - e0 < CLIP_CHUNK) {
+  if (!whole) {
     for (int64_t e = e0 + threadIdx.x; e < n; e += NT) out[e] = g[e] * k;
     return;
   }
-  f4 v[CLIP_UNROLL];
-#pragma unroll
-  for (int u = 0; u < CLIP_UNROLL; ++u)
-    v[u] = __builtin_nontemporal_load(reinterpret_cast<const f4u*>(g + e0) + u * NT + threadIdx.x);
+  if (out == g) load();
 #pragma unroll
   for (int u = 0; u < CLIP_UNROLL; ++u) {
     f4u* p = reinterpret_cast<f4u*>(out + e0) + u * NT + threadIdx.x;
