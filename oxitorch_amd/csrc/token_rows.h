@@ -508,7 +508,9 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4, 4
   const Two k = op.finish(row, op.load(row), r, lead);
   if constexpr (GRAD) {
     const RowGrad g(r, xa, in.scale2, (float)in.inv_t, k.a, ENT ? k.b : 0.f);
-    const float up = (shift - m) * in.scale2;  // the piece's t from the row's
+    // The piece's t from the row's, never above 0: a piece without a finite logit has a shift of 0, which
+    // may lie far over m, and its 2^t of 0 must not meet an infinite factor.
+    const float up = fminf((shift - m) * in.scale2, 0.f);
     const float alpha = ENT ? g.alpha : g.alpha * __builtin_amdgcn_exp2f(up);
     auto grad = [&](float z) {
       if constexpr (ENT) {
