@@ -498,7 +498,10 @@ int oxi_token_logp_workspace(int64_t n, int64_t c, int64_t* bytes);
  * go to the backward: for an upstream gradient gloss[0] it is
  *   oxi_token_logp_bwd(logits, ids, saved, coef, entropy_coef ? coef + n : NULL, gloss, ..)
  * With `dlogits` (n, c) set, the call also writes that for an upstream of 1. The
- * workspace as above, oxi_policy_loss_workspace bytes. */
+ * workspace as above, oxi_policy_loss_workspace bytes. Rows of more than 32768 classes
+ * lie over several blocks, which wait for each other; a wait that does not end (a
+ * workspace that two calls use at once) gives up after some seconds: NaN in the row, and
+ * oxi_hip_sync returns OXI_OTHER. */
 int oxi_policy_loss_fwd(const float* logits, const int64_t* ids, const float* advantages, const float* old_logp,
                         const float* ref_logp, const float* weights, float* out, float* rows, float* logp, float* coef,
                         float* saved, float* dlogits, void* workspace, int64_t n, int64_t c, float temperature,

@@ -357,7 +357,9 @@ int oxi_hip_sync(void) {
     (void)hipMemcpy(guard_flag(), &zero, sizeof(int), hipMemcpyHostToDevice);
     if (flag & 3)
       return fail(OXI_OUT_OF_BOUNDS, "a device kernel met an index outside its valid range; the affected output was written with zeros");
-    return fail(OXI_OTHER, "masked_select: a tile's offset wait did not finish; that tile's picks were not written");
+    if (flag & 4)
+      return fail(OXI_OTHER, "masked_select: a tile's offset wait did not finish; that tile's picks were not written");
+    return fail(OXI_OTHER, "policy_loss: a wait between the blocks of a row did not finish (do two calls share a workspace?); the row holds NaN");
   }
   return OXI_OK;
 }

@@ -2,6 +2,8 @@
 // were chosen from, over rows of logits, with their gradient; the passes that the
 // policy and preference losses share (the mathematics is in token_rows.h).
 #include <cmath>
+#include <cstdlib>
+#include <cstring>
 
 #include "token_rows.h"
 
@@ -179,7 +181,11 @@ __global__ __launch_bounds__(256) void zero_words_k(uint64_t* __restrict__ p, in
 Cluster start_cluster(void* at, int64_t n, int blocks) {
   const int64_t words = cluster_bytes(n, blocks) / (int64_t)sizeof(uint64_t);
   zero_words_k<<<dim3((unsigned)ceil_div(words, 256)), dim3(256), 0, stream()>>>(static_cast<uint64_t*>(at), words);
-  return {static_cast<uint64_t*>(at) + 8, static_cast<uint32_t*>(at), blocks};
+  // polls of about 1 us: a wait past some seconds is a failure (never seen); OXI_CLUSTER_SPIN_LIMIT=-1 fails
+  // every wait, to test that path
+  const char* sl = std::getenv("OXI_CLUSTER_SPIN_LIMIT");
+  const int spin_limit = sl && std::strcmp(sl, "-1") == 0 ? -1 : 1 << 22;
+  return {static_cast<uint64_t*>(at) + 8, static_cast<uint32_t*>(at), blocks, spin_limit};
 }
 
 int check_token_rows(const char* what, int64_t n, int64_t c, float temperature) {

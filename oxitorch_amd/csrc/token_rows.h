@@ -396,7 +396,8 @@ bool launch_token_rows_as(const TokenRows& in, const Op& op, float* dx) {
 // maximum and sums by words of a value and a flag each, so that no order of memory
 // accesses matters; the words are zeroed by a launch before. A block's row and piece go by a ticket that it takes as
 // it starts: a block waits only for those of its own row, which have started or take
-// the next tickets, and the rows before finish without it, so every wait ends.
+// the next tickets, and the rows before finish without it, so every wait ends; one that does not, as where
+// two calls share a workspace, gives up: the guard flag (bit 8), and NaN in what that block writes of its row.
 // (1024, 131072) with an entropy term 190 us, 5.4 TB/s; parts, their join and the
 // backward's pass 244. (4096, 50257) on two blocks 280, on one of 1024 threads 308. For few shorter rows, (64, 32000) on 4 blocks each, the ticket
 // and the words cost what the other CUs gain: 11.0 us against 10.2 on one block.
@@ -405,6 +406,7 @@ struct Cluster {
   uint64_t* words;  // 3 a block
   uint32_t* ticket;
   int blocks;  // a row
+  int spin_limit;
 };
 inline int64_t cluster_bytes(int64_t n, int blocks) { return 64 + n * blocks * 3 * (int64_t)sizeof(uint64_t); }
 // words and ticket zeroed, in `at`
@@ -414,14 +416,15 @@ constexpr uint64_t WORD_SET = (uint64_t)1 << 32;
 __device__ __forceinline__ void give_word(uint64_t* p, float v) {
   __hip_atomic_store(p, WORD_SET | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// The word once it is set.
-__device__ __forceinline__ float take_word(const uint64_t* p) {
-  uint64_t v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  while (!(v & WORD_SET)) {
+// The word once it is set; NaN after spin_limit polls more (a negative limit: at once).
+__device__ __forceinline__ float take_word(const uint64_t* p, int spin_limit, int* guard) {
+  for (int spins = 0; spins <= spin_limit; ++spins) {
+    const uint64_t v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (v & WORD_SET) return __uint_as_float((uint32_t)v);
     __builtin_amdgcn_s_sleep(1);
-    v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  return __uint_as_float((uint32_t)v);
+  atomicOr(guard, 8);
+  return __builtin_nanf("");
 }
 
 template <int NV, bool GRAD, bool ENT, bool NTS, class Op>
@@ -435,6 +438,10 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4, 4
   if (t == 0) ticket = atomicAdd(cl.ticket, 1u);
   __syncthreads();
   const uint32_t b = __builtin_amdgcn_readfirstlane(ticket);
+  if (b >= gridDim.x) {  // another call has taken tickets from this workspace: there is no such row
+    if (t == 0) atomicOr(in.guard, 8);
+    return;
+  }
   const int64_t row = b / (unsigned)cl.blocks;
   const int piece = (int)(b % (unsigned)cl.blocks);
   const int C = in.c;
@@ -492,7 +499,7 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4, 4
   v1 = add(v1);
   const Two both = over_block<RT, Both<AddF32>>(Two{s, et}, reinterpret_cast<Two*>(lds + RT / 64));
   if (t < 3) give_word(words + 3 * piece + t, t == 0 ? own : t == 1 ? both.a : both.b);
-  if (t < 3 * cl.blocks) from[t] = take_word(words + t);
+  if (t < 3 * cl.blocks) from[t] = take_word(words + t, cl.spin_limit, in.guard);
   __syncthreads();
   float m = xa;
   for (int k = 0; k < cl.blocks; ++k) m = fmaxf(m, from[3 * k]);
