@@ -490,7 +490,8 @@ int oxi_token_logp_workspace(int64_t n, int64_t c, int64_t* bytes);
  * ref_logp NULL: no k. weights NULL: w = 1; a row of weight 0 counts as padding.
  * clip_high may be inf; clip_max 0: none. kl_coef 0 (entropy_coef 0) leaves its term
  * out of the loss, not out of `rows`. The divisor is the number of counted rows for
- * their mean.
+ * their mean. A row with no finite logit gives NaN, in the loss and in its gradient,
+ * whatever the advantage; an advantage of 0 gains nothing at an infinite r.
  * out (4 floats): sums of w/divisor times the rows' loss, k, entropy, and whether s is
  * bounded (the clipped share), in 64 bits in a fixed order; rows (4, n): the same for
  * each row, without w; logp (n, may be NULL). Padded rows are 0 in all of them.

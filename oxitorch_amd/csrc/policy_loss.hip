@@ -37,8 +37,9 @@ struct PolicyOp {
   // Writes the row's results; the loss's derivatives by its logp and entropy.
   __device__ __forceinline__ Two finish(int64_t row, const Given& in, const RowStats& r, bool lead) const {
     const double A = (double)in.adv;
-    const double ratio = old ? exp64(r.logp - (double)in.old) : 1.0;
-    const double free = A == 0.0 ? 0.0 : ratio * A;
+    const bool broken = r.logp != r.logp;  // the row holds no distribution: NaN whatever the ratio and the advantage
+    const double ratio = broken ? r.logp : old ? exp64(r.logp - (double)in.old) : 1.0;
+    const double free = A == 0.0 && !broken ? 0.0 : ratio * A;
     const double bounded = (ratio < low ? low : ratio > high ? high : ratio) * A;
     bool clipped = free > bounded;
     double s = clipped ? bounded : free;
