@@ -473,7 +473,7 @@ int oxi_token_logp_fwd(const float* logits, const int64_t* ids, float* logp, flo
  * floats each; one of them may be NULL, for none; gloss NULL: 1), from the saved floats
  * of oxi_token_logp_fwd, oxi_policy_loss_fwd or oxi_preference_loss_fwd over the same
  * logits, ids and temperature. Padded rows get zeros, and so do rows whose gradients
- * are 0, whose logits are not read. Takes no workspace. */
+ * are 0, whose logits are not read, whatever gloss[0] is. Takes no workspace. */
 int oxi_token_logp_bwd(const float* logits, const int64_t* ids, const float* saved, const float* glogp,
                        const float* gentropy, const float* gloss, float* dlogits, int64_t n, int64_t c,
                        float temperature);
