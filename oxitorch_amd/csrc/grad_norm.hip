@@ -4,7 +4,7 @@
 //   out = g * min(1, max_norm / (total + 1e-6))
 //
 // Every tensor is cut into chunks, a block each; the tensors' places travel in the kernel
-// arguments, up to MOST_SLICES a launch. The terms are squared and summed in 64 bits (no
+// arguments, up to MOST_SLICES a launch, and one that passes a launch is cut (grad_slices.h). The terms are squared and summed in 64 bits (no
 // overflow, and a sum over 10^9 terms keeps its digits), a sum a chunk, then one block
 // adds the chunks' in a fixed order. The clipping reads total on the device, so nothing
 // waits for the host between the two.
@@ -12,6 +12,7 @@
 // HBM bounds it: 354 M floats in 242 tensors, norm 220 us (6.4 TB/s) and clipping 447 (6.3).
 #include <cmath>
 
+#include "grad_slices.h"
 #include "internal.h"
 #include "launch_limits.h"
 #include "row64.h"
@@ -164,7 +165,7 @@ int64_t chunks_of(const oxi_grad_slice* slices, int count, int64_t total) {
   return chunks;
 }
 
-// Calls launch(slices, blocks, blocks before) for as many slices at once as fit, in
+// Calls launch(slices, blocks, blocks before) for as many slices at once as fit (grad_slices.h), in
 // order or from the last on.
 template <class F>
 int for_slices(const oxi_grad_slice* slices, int count, int64_t chunk, bool back, const char* what, F launch) {
@@ -172,26 +173,22 @@ int for_slices(const oxi_grad_slice* slices, int count, int64_t chunk, bool back
   a.chunk = chunk;
   int64_t blocks = 0, before = 0;
   int rc = OXI_OK;
-  auto flush = [&]() {
-    if (!a.count) return;
-    launch(a, (unsigned)blocks, before);
-    if (rc == OXI_OK) rc = check_launch(what);
-    before += blocks;
-    blocks = 0;
-    a.count = 0;
-  };
-  for (int j = 0; j < count; ++j) {
-    const oxi_grad_slice& q = slices[back ? count - 1 - j : j];
-    if (q.n == 0) continue;
-    const int64_t nb = ceil_div(q.n, a.chunk);
-    if (a.count == MOST_SLICES || !grid_fits(blocks + nb, NT)) flush();
-    a.g[a.count] = q.g;
-    a.out[a.count] = q.out;
-    a.n[a.count] = q.n;
-    blocks += nb;
-    a.end[a.count++] = (uint32_t)blocks;
-  }
-  flush();
+  walk_slices(
+      [&](int i) { return slices[i].n; }, count, chunk, NT, MOST_SLICES, back,
+      [&](int i, int64_t e0, int64_t n, int64_t nb) {
+        a.g[a.count] = slices[i].g + e0;
+        a.out[a.count] = slices[i].out ? slices[i].out + e0 : nullptr;
+        a.n[a.count] = n;
+        blocks += nb;
+        a.end[a.count++] = (uint32_t)blocks;
+      },
+      [&]() {
+        launch(a, (unsigned)blocks, before);
+        if (rc == OXI_OK) rc = check_launch(what);
+        before += blocks;
+        blocks = 0;
+        a.count = 0;
+      });
   return rc;
 }
 
