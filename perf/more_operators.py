@@ -231,8 +231,9 @@ def _own_logp(s, case):
     from oxitorch_amd import capi
 
     n, c = s["x"].shape
+    # without a backward to come nothing is saved for it, as in F.token_log_probs under no_grad
     capi.call("oxi_token_logp_fwd", _ptr(s["x"]), _ptr(s["ids"]), _ptr(s["logp"]), _ptr(s["entropy"]),
-              _ptr(s["saved"]), None, n, c, case["temperature"])
+              _ptr(s["saved"]) if case["grad"] else None, None, n, c, case["temperature"])
     out = {"logp": s["logp"], "entropy": s["entropy"]}
     if case["grad"]:
         capi.call("oxi_token_logp_bwd", _ptr(s["x"]), _ptr(s["ids"]), _ptr(s["saved"]), _ptr(s["gl"]), _ptr(s["ge"]),
