@@ -95,11 +95,11 @@ __global__ __launch_bounds__(BWD_NT) void token_bwd_k(const float* __restrict__ 
   const int64_t id = ids[row];
   const f4 sv = *reinterpret_cast<const f4u*>(saved + 4 * row);
   const float up = (gloss ? gloss[0] : 1.f) * inv_t;
-  const float gli = gl ? gl[row] : 0.f, ghi = ENT ? gh[row] : 0.f;
-  const float a = gl ? gli * up : 0.f, b = ENT ? ghi * up : 0.f;
+  // a gradient of 0 stays 0 under an upstream that is not finite too
+  auto times = [&](float g) { return g == 0.f ? 0.f : g * up; };
+  const float a = gl ? times(gl[row]) : 0.f, b = ENT ? times(gh[row]) : 0.f;
   if (id >= c && t == 0) atomicOr(guard, 1);
-  // a row whose own gradients are 0 gets zeros under an upstream that is not finite too
-  const bool none = id < 0 || id >= c || (gli == 0.f && ghi == 0.f) || (a == 0.f && b == 0.f);
+  const bool none = id < 0 || id >= c || (a == 0.f && b == 0.f);
   const float* xr = x + row * c;
   float* dr = dx + row * c;
   // the float4s as the logits lie; the gradient may lie otherwise
