@@ -438,11 +438,11 @@ __global__ __launch_bounds__(CLUSTER_RT) __attribute__((amdgpu_waves_per_eu(4, 4
   if (t == 0) ticket = atomicAdd(cl.ticket, 1u);
   __syncthreads();
   const uint32_t b = __builtin_amdgcn_readfirstlane(ticket);
-  if (b >= gridDim.x) {  // another call has taken tickets from this workspace: there is no such row
+  const int64_t row = b / (unsigned)cl.blocks;
+  if (row >= in.n) {  // another call has taken tickets from this workspace: there is no such row
     if (t == 0) atomicOr(in.guard, 8);
     return;
   }
-  const int64_t row = b / (unsigned)cl.blocks;
   const int piece = (int)(b % (unsigned)cl.blocks);
   const int C = in.c;
   const float* xr = in.x + row * C;
