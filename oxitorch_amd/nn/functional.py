@@ -346,6 +346,9 @@ def policy_loss(logits, tokens, advantages, old_log_probs=None, reference_log_pr
     tokens * sequences)). With `stats`, (loss, (3,) tensor of the same means of the KL
     term's exp(d) - 1 - d, H and whether r was clipped).
 
+    A row with no finite logit, or with NaN, gives NaN in the loss and in its gradient,
+    whatever its advantage.
+
     Fused as cross_entropy is: one pass over the logits writes the loss and the
     gradient for backward()'s implicit seed."""
     n, classes = logits.shape
